@@ -57,6 +57,25 @@ inline int round_up(int v, int m) { return (v + m - 1) / m * m; }
 inline size_t round_up_sz(size_t v, size_t m) { return (v + m - 1) / m * m; }
 inline int dtype_size(int32_t dt) { return dt == kF32 ? 4 : 2; }
 
+// The context's device made current for a launch, and the caller's again afterwards.
+struct DeviceScope {
+    int before = -1;
+    cudaError_t error;
+    explicit DeviceScope(const iq_ctx* ctx) {
+        int now = 0;
+        error = cudaGetDevice(&now);
+        if (error == cudaSuccess && now != ctx->device) {
+            error = cudaSetDevice(ctx->device);
+            if (error == cudaSuccess) before = now;
+        }
+    }
+    ~DeviceScope() {
+        if (before >= 0) cudaSetDevice(before);
+    }
+    DeviceScope(const DeviceScope&) = delete;
+    DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
 // A launch that may start before its predecessor in the stream has ended; the kernel calls pdl_wait() before it touches
 // anything the predecessor may still write or read.
 template <class... P, class... A>

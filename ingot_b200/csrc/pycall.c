@@ -18,11 +18,13 @@ static void* fn_had_rows;
 static void* fn_embed_rows;
 static void* fn_argmax_rows;
 static void* fn_topk64;
+static void* fn_add_rmsnorm;
 
 static const struct { const char* name; void** slot; } table[] = {
     {"iq_qmv", &fn_qmv},           {"iq_qmm", &fn_qmm},               {"iq_dense_ffn", &fn_dense_ffn},
     {"iq_moe_forward", &fn_moe_forward}, {"iq_rmsnorm", &fn_rmsnorm}, {"iq_had_rows", &fn_had_rows},
     {"iq_embed_rows", &fn_embed_rows},   {"iq_argmax_rows", &fn_argmax_rows}, {"iq_topk64", &fn_topk64},
+    {"iq_add_rmsnorm", &fn_add_rmsnorm},
 };
 
 static PyObject* py_bind(PyObject* self, PyObject* args) {
@@ -155,9 +157,20 @@ ENTRY(topk64, 13, topk_t, {
     LAUNCH(f(c, s, x, ldx, rows, vocab, t, nt, ix, v, z, sc, sb));
 })
 
+typedef int32_t (*add_norm_t)(iq_ctx*, void*, const void*, int32_t, int64_t, const void*, int32_t, int64_t, void*, int64_t, const void*, int32_t,
+                              float, float, int32_t, int32_t, void*, int32_t, int64_t, int8_t*, int64_t, float*, int32_t);
+ENTRY(add_rmsnorm, 23, add_norm_t, {
+    void *c = P(0), *s = P(1), *x = P(2), *r = P(5), *ro = P(8), *w = P(10), *o = P(16), *q = P(19), *sc = P(21);
+    int32_t xd = I32(3), rd = I32(6), wd = I32(11), rows = I32(14), d = I32(15), od = I32(17), rot = I32(22);
+    int64_t ldx = I64(4), ldr = I64(7), ldro = I64(9), ldo = I64(18), ldc = I64(20);
+    float off = F32(12), eps = F32(13);
+    CHECKED;
+    LAUNCH(f(c, s, x, xd, ldx, r, rd, ldr, ro, ldro, w, wd, off, eps, rows, d, o, od, ldo, q, ldc, sc, rot));
+})
+
 #define M(NAME) {#NAME, (PyCFunction)(void (*)(void))py_##NAME, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {
     {"bind", py_bind, METH_VARARGS, NULL}, M(qmv), M(qmm), M(dense_ffn), M(moe_forward), M(rmsnorm), M(had_rows), M(embed_rows),
-    M(argmax_rows), M(topk64), {NULL, NULL, 0, NULL}};
+    M(argmax_rows), M(topk64), M(add_rmsnorm), {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_iqcall", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__iqcall(void) { return PyModule_Create(&module); }

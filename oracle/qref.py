@@ -432,3 +432,33 @@ def w8a8_ternary_emulated(xr: np.ndarray, w: np.ndarray, scales_f16: np.ndarray)
     wq = t * np.repeat(qg * sign, 128, axis=1)
     y = (xq.astype(np.float64) @ wq.astype(np.float64).T).astype(np.float32)
     return y * sx[:, None] * srow[None, :]
+
+
+# ----------------------------------------------------------------------------------------------------------------
+# what stands between the linears (no counterpart in the reference's kernels: iq_add_rmsnorm)
+
+
+def add_rmsnorm(kept: np.ndarray, w: np.ndarray, eps: float):
+    """RMSNorm(kept) * w in float64 and the rows' factors 1 / rms [rows, 1]; kept: the sum as it is stored, w with its offset."""
+    k = np.asarray(kept, dtype=np.float64)
+    with np.errstate(invalid="ignore", over="ignore", divide="ignore"):
+        q = 1.0 / np.sqrt((k * k).mean(axis=1, keepdims=True) + eps)
+        return k * q * np.asarray(w, dtype=np.float64), q
+
+
+def norm_codes(kept: np.ndarray, w: np.ndarray, n: int):
+    """(int8 codes, s = max|u| / 127 per row) of u = H_n(kept * w), one fp32 operation at a time; n = 1: no rotation."""
+    v = np.asarray(kept, dtype=np.float32) * np.asarray(w, dtype=np.float32)
+    u = fwht(v.reshape(v.shape[0], -1, n)).reshape(v.shape)
+    s = (np.abs(u).max(axis=1) / np.float32(127)).astype(np.float32)
+    with np.errstate(invalid="ignore", divide="ignore"):
+        q = np.clip(np.rint(u / s[:, None]), -127, 127)
+    return np.where(s[:, None] > 0, q, 0).astype(np.int8), s
+
+
+def hadamard(n: int) -> np.ndarray:
+    """The n x n matrix of +1 / -1 that fwht multiplies with, by Sylvester's doubling."""
+    h = np.ones((1, 1))
+    while h.shape[0] < n:
+        h = np.block([[h, h], [h, -h]])
+    return h

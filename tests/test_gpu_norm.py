@@ -1,0 +1,227 @@
+"""iq_add_rmsnorm through norm.add_rmsnorm: the sum and the codes bit for bit, the norm against 64 bits."""
+import numpy as np
+import pytest
+import torch
+
+from ingot_b200 import capi, norm
+from ingot_b200.norm import add_rmsnorm
+from oracle import qref
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+# q's relative error: the fp32 sum of squares adds at most 32 fma per thread and ten levels of two trees (42 * 2^-24, halved by the root),
+# division, addition of eps and rsqrt another four; with the weight's addition and two products 21 + 4 + 3 = 28
+Q_TOL = 32 * 2.0**-24
+
+
+def rows_of(gen, rows, d, pad, dtype, scale=1.0):
+    """[rows + 1, d] inside wider rows, the rest filled with NaN: nothing of it may be read into a result, nor written."""
+    t = torch.full((rows + 1, d + pad), float("nan"))
+    t[:rows, :d] = scale * torch.randn(rows, d, generator=gen)
+    return t.to(dtype)
+
+
+def run(gen, rows, d, xt, rt, wt, ot, rotate, pad, offset=0.0, eps=1e-6, device="cuda", want_out=True, want_codes=True, spread=1.0):
+    x = None if xt is None else rows_of(gen, rows, d, pad, xt)
+    r = rows_of(gen, rows, d, pad, rt, spread)
+    w = None if wt is None else (1 - offset + 0.3 * torch.randn(d, generator=gen)).to(wt)
+    up = lambda t: None if t is None else t.to(device)
+    xd, rd, wd = up(x), up(r), up(w)
+    ro = None if x is None else torch.full_like(rd, 7)
+    out = torch.full((rows + 1, d + pad), 7, dtype=ot, device=device) if want_out else None
+    codes = torch.full((rows + 1, d + pad), 99, dtype=torch.int8, device=device) if want_codes else None
+    scales = torch.full((rows + 1,), 7, dtype=F32, device=device) if want_codes else None
+    cut = lambda t: None if t is None else t[:, :d]
+    add_rmsnorm(cut(xd), cut(rd), wd, rows, eps=eps, weight_offset=offset, residual_out=cut(ro), out=cut(out), codes=cut(codes), scales=scales, rotate=rotate)
+    torch.cuda.synchronize()
+    for t, fill in ((ro, 7), (out, 7), (codes, 99)):  # what lies beside the rows and behind the last one stays
+        if t is not None:
+            t = t.float().cpu()
+            assert (t[rows] == fill).all() and (t[:rows, d:] == fill).all()
+    down = lambda t: None if t is None else t[:rows].cpu() if t.dim() == 1 else t[:rows, :d].cpu()
+    return tuple(None if t is None else t[:rows, :d] for t in (x, r)) + (w, down(ro), down(out), down(codes), down(scales))
+
+
+def check(got, offset, eps, rotate):
+    x, r, w, ro, out, codes, scales = got
+    total = r if x is None else (r.float() + x.float()).to(r.dtype)
+    if x is not None:
+        assert torch.equal(ro, total)
+    kept = total.float().numpy()
+    w32 = np.ones(kept.shape[1], np.float32) if w is None else w.float().numpy() + np.float32(offset)
+    ref, q = qref.add_rmsnorm(kept, w32, eps)
+    if out is not None:
+        half = torch.finfo(out.dtype).eps / 2
+        tiny = float(torch.finfo(out.dtype).tiny) * half * 2  # half a step of a subnormal
+        assert (np.abs(out.double().numpy() - ref) <= np.abs(ref) * (Q_TOL + half * (1 + Q_TOL)) + tiny).all()
+    if codes is not None:
+        want, s = qref.norm_codes(kept, w32, max(rotate, 1))
+        assert np.array_equal(codes.numpy(), want)
+        assert np.allclose(scales.double().numpy(), s.astype(np.float64) * q[:, 0], rtol=Q_TOL, atol=0)
+
+
+@pytest.mark.parametrize("rows,d,pad", [(1, 1, 0), (3, 7, 1), (1, 64, 0), (2, 256, 8), (5, 2880, 0), (4, 2880, 5), (1, 2048, 0), (37, 4096, 0), (3, 8191, 0),
+                                        (2, 8192, 0), (2, 8200, 0), (2, 16384, 16), (2, 16385, 3), (2, 32768, 0), (1, 32767, 0)])
+@pytest.mark.parametrize("xt,rt,wt,ot", [(BF16, F32, BF16, BF16), (F16, F16, F32, F32), (F32, BF16, None, F16), (None, F32, F16, F32)])
+def test_sum_norm_and_codes(cuda_device, rows, d, pad, xt, rt, wt, ot):
+    gen = torch.Generator().manual_seed(rows * 100003 + d + pad)
+    check(run(gen, rows, d, xt, rt, wt, ot, 0, pad), 0.0, 1e-6, 0)
+
+
+@pytest.mark.parametrize("rotate", [32, 256])
+@pytest.mark.parametrize("rows,blocks,pad", [(1, 1, 0), (3, 7, 0), (2, 16, 3), (65, 8, 0), (2, 33, 0), (2, 72, 0), (1, 128, 1)])
+def test_rotated_codes(cuda_device, rotate, rows, blocks, pad):
+    gen = torch.Generator().manual_seed(rotate + rows * 31 + blocks)
+    d = 256 * blocks if rotate == 256 else 256 * blocks - 32 * (blocks % 3)
+    got = run(gen, rows, d, BF16, F32, BF16, F16, rotate, pad)
+    check(got, 0.0, 1e-6, rotate)
+    # and against the transform in 64 bits: half a step of the codes, and the butterflies' roundings
+    x, r, w, ro, out, codes, scales = got
+    v = ro.double().numpy() * w.double().numpy()
+    u = (v.reshape(rows, -1, rotate) @ qref.hadamard(rotate)).reshape(rows, d)
+    sums = np.repeat(np.abs(v).reshape(rows, -1, rotate).sum(-1), rotate, axis=1)
+    s = qref.norm_codes(ro.float().numpy(), w.float().numpy(), rotate)[1].astype(np.float64)[:, None]
+    assert (np.abs(codes.numpy() * s - u) <= s * (0.5 + 127 * 2.0**-22) + 10 * 2.0**-24 * sums).all()
+
+
+def test_one_output_alone_and_the_weights_offset(cuda_device):
+    gen = torch.Generator().manual_seed(3)
+    check(run(gen, 9, 1408, BF16, BF16, BF16, BF16, 0, 0, offset=1.0, want_codes=False), 1.0, 1e-6, 0)
+    check(run(gen, 9, 1408, BF16, BF16, BF16, BF16, 32, 0, offset=1.0, want_out=False), 1.0, 1e-6, 32)
+    check(run(gen, 9, 1408, F16, F32, F32, F32, 0, 0, eps=0.5), 0.0, 0.5, 0)
+
+
+@pytest.mark.parametrize("spread", [1e-3, 1e4])
+def test_wide_ranges(cuda_device, spread):
+    gen = torch.Generator().manual_seed(4)
+    check(run(gen, 5, 768, F32, F32, F32, F32, 256, 0, spread=spread), 0.0, 1e-6, 256)
+
+
+def test_codes_next_to_a_border(cuda_device):
+    """Quotients at and beside halves: the codes are the division's, not those of a product with the reciprocal."""
+    d = 4096
+    s = np.float32(0.7) / np.float32(127)
+    k = np.arange(d) % 253 - 126
+    r = (np.float32(0.5) + np.float32(k)) * s
+    r[1::3] = np.nextafter(r[1::3], np.float32(9))
+    r[2::3] = np.nextafter(r[2::3], np.float32(-9))
+    r[0] = 0.7
+    t = torch.from_numpy(r)[None].cuda()
+    codes, scales = torch.empty(1, d, dtype=torch.int8, device="cuda"), torch.empty(1, device="cuda")
+    add_rmsnorm(None, t, None, 1, codes=codes, scales=scales)
+    want, _ = qref.norm_codes(r[None], np.ones(d, np.float32), 1)
+    assert np.array_equal(codes.cpu().numpy(), want)
+
+
+def test_rows_of_zeros_infinities_and_nan(cuda_device):
+    d = 512
+    r = torch.randn(6, d, generator=torch.Generator().manual_seed(5))
+    r[0] = 0
+    r[1, 17] = float("inf")
+    r[2, 300] = float("nan")
+    r[3] *= 1e-42  # below the normal numbers
+    x = torch.zeros(6, d)
+    codes = torch.full((6, d), 99, dtype=torch.int8, device="cuda")
+    scales, out, ro = torch.full((6,), 7.0, device="cuda"), torch.empty(6, d, device="cuda"), torch.empty(6, d, device="cuda")
+    for rotate in (0, 32, 256):
+        add_rmsnorm(x.cuda(), r.cuda(), None, 6, residual_out=ro, out=out, codes=codes, scales=scales, rotate=rotate)
+        c, s, o = codes.cpu(), scales.cpu(), out.cpu()
+        assert (c[:3] == 0).all() and s[0] == 0 and s[1].isnan() and s[2].isnan()
+        assert (o[0] == 0).all() and o[1, 17].isnan() and (o[1, :17] == 0).all() and o[2].isnan().all()
+        want, _ = qref.norm_codes(r[3:].numpy(), np.ones(d, np.float32), max(rotate, 1))
+        assert np.array_equal(c[3:].numpy(), want)  # a poisoned row is alone
+
+
+def test_in_place_and_the_rows_alone(cuda_device):
+    """residual_out = residual (the default), out = x; a row's codes do not depend on the others."""
+    gen = torch.Generator().manual_seed(6)
+    rows, d = 33, 2880
+    x, r, w = torch.randn(rows, d, generator=gen).to(BF16), torch.randn(rows, d, generator=gen), torch.randn(d, generator=gen)
+    sep = {"residual_out": torch.empty(rows, d, device="cuda"), "out": torch.empty(rows, d, dtype=BF16, device="cuda")}
+    codes, scales = torch.empty(rows, d, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    add_rmsnorm(x.cuda(), r.cuda(), w.cuda(), rows, codes=codes, scales=scales, **sep)
+    xi, ri = x.cuda(), r.cuda()
+    add_rmsnorm(xi, ri, w.cuda(), rows, out=xi)
+    assert torch.equal(xi, sep["out"]) and torch.equal(ri, sep["residual_out"])
+    for t in (0, 17, 32):
+        c, s = torch.empty(1, d, dtype=torch.int8, device="cuda"), torch.empty(1, device="cuda")
+        add_rmsnorm(None, sep["residual_out"][t:t + 1], w.cuda(), 1, codes=c, scales=s)
+        assert torch.equal(c[0], codes[t]) and torch.equal(s[0], scales[t])
+
+
+def test_the_w8a8_gemms_own_conversion(cuda_device):
+    """On rows of unit weight the codes are those that the reference's activations' conversion gives to r' itself (the norm's factor is in the scale)."""
+    rng = np.random.default_rng(8)
+    r = rng.normal(size=(4, 2048)).astype(np.float32)
+    codes, scales = torch.empty(4, 2048, dtype=torch.int8, device="cuda"), torch.empty(4, device="cuda")
+    add_rmsnorm(None, torch.from_numpy(r).cuda(), None, 4, codes=codes, scales=scales, rotate=256)
+    want, _ = qref.quant_i8_rows(qref.fwht(r.reshape(4, 8, 256)).reshape(4, 2048))
+    assert np.array_equal(codes.cpu().numpy(), want)
+
+
+def test_streams_graphs_and_no_rows(cuda_device):
+    gen = torch.Generator().manual_seed(9)
+    rows, d = 8, 4096
+    x, r, w = (torch.randn(*s, generator=gen).cuda() for s in ((rows, d), (rows, d), (d,)))
+    out, ro = torch.empty(rows, d, device="cuda"), torch.empty(rows, d, device="cuda")
+    codes, scales = torch.zeros(rows, d, dtype=torch.int8, device="cuda"), torch.zeros(rows, device="cuda")
+    call = lambda **k: add_rmsnorm(x, r, w, rows, residual_out=ro, out=out, codes=codes, scales=scales, rotate=256, **k)
+    call()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in (out, ro, codes, scales)]
+    side = torch.cuda.Stream()
+    for t in (out, ro, codes, scales):
+        t.zero_()
+    side.wait_stream(torch.cuda.current_stream())
+    call(stream=side)
+    side.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((out, ro, codes, scales), want))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        call()
+    x2 = torch.randn(rows, d, generator=gen).cuda()
+    old = x.clone()
+    x.copy_(x2)
+    g.replay()
+    assert torch.equal(ro, r + x2)
+    x.copy_(old)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip((out, ro, codes, scales), want))
+    out.fill_(5)
+    add_rmsnorm(x, r, w, 0, residual_out=ro, out=out)
+    assert (out == 5).all()
+
+
+def test_long_strides_pass_32_bits(cuda_device):
+    """Rows 1.2 G elements apart."""
+    d, ld = 256, 1_200_000_000
+    buf = torch.empty(2 * ld + d, dtype=F16, device="cuda")
+    r = torch.as_strided(buf, (3, d), (ld, 1))
+    gen = torch.Generator().manual_seed(10)
+    v = torch.randn(3, d, generator=gen).to(F16)
+    r.copy_(v)
+    out = torch.empty(3, d, device="cuda")
+    add_rmsnorm(None, r, None, 3, out=out)
+    ref, _ = qref.add_rmsnorm(v.float().numpy(), np.ones(d, np.float32), 1e-6)
+    assert (np.abs(out.double().cpu().numpy() - ref) <= np.abs(ref) * (Q_TOL + 2.0**-24)).all()
+
+
+def test_many_rows(cuda_device):
+    """More rows than a second grid dimension would take."""
+    rows, d = 70001, 64
+    r = torch.randn(rows, d, device="cuda")
+    out = torch.empty_like(r)
+    add_rmsnorm(None, r, None, rows, out=out)
+    ref, _ = qref.add_rmsnorm(r.cpu().numpy(), np.ones(d, np.float32), 1e-6)
+    assert (np.abs(out.double().cpu().numpy() - ref) <= np.abs(ref) * (Q_TOL + 2.0**-24)).all()
+    assert capi.context(0).device_status() == 0
+
+
+def test_refusals_reach_no_kernel(cuda_device):
+    r = torch.randn(2, 64, device="cuda")
+    with pytest.raises(ValueError, match="different devices"):
+        add_rmsnorm(None, r, torch.ones(64), 2, out=r.clone())
+    assert norm.MAX_WIDTH == 32768
