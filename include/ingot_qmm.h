@@ -491,7 +491,7 @@ int32_t iq_rmsnorm(iq_ctx* ctx, void* stream, const float* x, int64_t ldx, void*
  * u holds an infinity or NaN has codes 0 and scale NaN. The sum of squares is fp32: rows beyond 1e19 overflow it.
  * x null (with residual_out null): no addition, r' = residual. weight null: weights of 1, the offset unused. out null or codes (with scales) null: not
  * wanted. weight_offset: 1 where the checkpoint stores w - 1 (Gemma), else 0. residual_out may be residual and out may be x,
- * where row stride and element size are the same; other overlaps are not allowed. Any alignment and strides of at least d; groups of eight aligned to 16 bytes (codes: 8) are faster. d up to 32768; rows = 0 does nothing.
+ * where row stride and element size are the same; other overlaps are not allowed. Any alignment and strides of at least d; where groups of eight lie on their own size (fp32: 32 bytes, 16 bits: 16, codes: 8) it is faster. d up to 32768; rows = 0 does nothing.
  * The reference has norm and addition as kernels of their own (Shaders/verify.metal:503-523) and converts activations inside its W8A8
  * GEMM (Layers/Dense.swift:99-172). */
 int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int32_t x_dtype, int64_t ldx, const void* residual, int32_t r_dtype,

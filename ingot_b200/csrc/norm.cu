@@ -12,6 +12,8 @@
 // the W8A8 GEMM's own conversion (w8a8.cu).
 #include <cuda_bf16.h>
 
+#include <algorithm>
+
 #include "common.cuh"
 #include "internal.h"
 #include "ptx.cuh"
@@ -31,68 +33,172 @@ struct NormParams {
     float* scales;
     int64_t ldx, ldr, ldro, ldo, ldc;
     int32_t x_dtype, r_dtype, w_dtype, out_dtype;
-    int32_t d;
+    int32_t rows, d;
     float offset, eps;
 };
 
-// Eight values as they lie in memory, and as floats. dtype is the same for a whole launch: a branch costs an issue slot.
+// Eight values as they lie in memory, and as floats. A dtype is the same for a whole launch; HT is the 16-bit type where all 16-bit tensors
+// of the call have the same one, else kF32: chosen at run time, where both conversions are made (2048 rows of 4096 in fp16: 15.5 us for 12.4).
+template <int HT>
+__device__ __forceinline__ int32_t known_type(int32_t dtype) { return HT == kF32 || dtype == kF32 ? dtype : HT; }
+
 struct Raw8 {
     uint4 a, b;
 };
-__device__ __forceinline__ Raw8 raw8_load(const void* p, int32_t dtype, size_t i) {
+__device__ __forceinline__ Raw8 load8(const void* p, int32_t dtype, size_t i) {
     Raw8 r;
     r.b = make_uint4(0, 0, 0, 0);
     if (dtype == kF32) {
-        const uint4* q = reinterpret_cast<const uint4*>(static_cast<const float*>(p) + i);
-        r.a = q[0];
-        r.b = q[1];
+        const float* q = static_cast<const float*>(p) + i;
+        asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                     : "=r"(r.a.x), "=r"(r.a.y), "=r"(r.a.z), "=r"(r.a.w), "=r"(r.b.x), "=r"(r.b.y), "=r"(r.b.z), "=r"(r.b.w)
+                     : "l"(q)
+                     : "memory");
     } else {
         r.a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
     }
     return r;
 }
-__device__ __forceinline__ float scalar_load(const void* p, int32_t dtype, size_t i) {
+template <int HT>
+__device__ __forceinline__ void unpack8(const Raw8& r, int32_t dtype, float (&v)[8]) {
+    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
+    if (dtype == kF32) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = __uint_as_float(w[j]);
+    } else if (known_type<HT>(dtype) == kBF16) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            v[2 * j] = __uint_as_float(w[j] << 16);
+            v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[j]));
+            v[2 * j] = f.x;
+            v[2 * j + 1] = f.y;
+        }
+    }
+}
+template <int HT>
+__device__ __forceinline__ uint32_t pack2(float lo, float hi, int32_t dtype) {
+    if (known_type<HT>(dtype) == kF16) return pack_half2(lo, hi);
+    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&b);
+}
+// v rounded to the type, as it lies in memory; v becomes what was stored
+template <int HT>
+__device__ __forceinline__ Raw8 pack8(int32_t dtype, const float (&v)[8]) {
+    Raw8 r;
+    if (dtype == kF32) {
+        r.a = make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+        r.b = make_uint4(__float_as_uint(v[4]), __float_as_uint(v[5]), __float_as_uint(v[6]), __float_as_uint(v[7]));
+    } else {
+        r.a = make_uint4(pack2<HT>(v[0], v[1], dtype), pack2<HT>(v[2], v[3], dtype), pack2<HT>(v[4], v[5], dtype), pack2<HT>(v[6], v[7], dtype));
+        r.b = make_uint4(0, 0, 0, 0);
+    }
+    return r;
+}
+__device__ __forceinline__ void store8(void* p, int32_t dtype, size_t i, const Raw8& r) {
+    if (dtype == kF32) {
+        // (whole sectors: two stores of 16 bytes, 32 apart between lanes, are 30 % of the kernel's time)
+        asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(static_cast<float*>(p) + i), "r"(r.a.x), "r"(r.a.y), "r"(r.a.z), "r"(r.a.w),
+                     "r"(r.b.x), "r"(r.b.y), "r"(r.b.z), "r"(r.b.w)
+                     : "memory");
+    } else {
+        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = r.a;
+    }
+}
+// One value at a time, for rows that are not aligned
+__device__ __forceinline__ float load1(const void* p, int32_t dtype, size_t i) {
     if (dtype == kF32) return static_cast<const float*>(p)[i];
     const uint16_t h = static_cast<const uint16_t*>(p)[i];
     return dtype == kBF16 ? bf16_bits_to_f32(h) : __half2float(__ushort_as_half(h));
 }
-__device__ __forceinline__ float round_to(float v, int32_t dtype) {
+__device__ __forceinline__ float round1(float v, int32_t dtype) {
     if (dtype == kF32) return v;
     return dtype == kBF16 ? __bfloat162float(__float2bfloat16_rn(v)) : __half2float(__float2half_rn(v));
 }
-__device__ __forceinline__ uint32_t pack2(float lo, float hi, int32_t dtype) {
-    if (dtype == kF16) return pack_half2(lo, hi);
-    const __nv_bfloat162 b = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&b);
-}
-__device__ __forceinline__ void store8(void* p, int32_t dtype, size_t i, const float (&v)[8]) {
-    if (dtype == kF32) {
-        float4* q = reinterpret_cast<float4*>(static_cast<float*>(p) + i);
-        q[0] = make_float4(v[0], v[1], v[2], v[3]);
-        q[1] = make_float4(v[4], v[5], v[6], v[7]);
-    } else {
-        *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) =
-            make_uint4(pack2(v[0], v[1], dtype), pack2(v[2], v[3], dtype), pack2(v[4], v[5], dtype), pack2(v[6], v[7], dtype));
-    }
-}
-__device__ __forceinline__ void scalar_store(void* p, int32_t dtype, size_t i, float v) {
+__device__ __forceinline__ void store1(void* p, int32_t dtype, size_t i, float v) {
     if (dtype == kF32) static_cast<float*>(p)[i] = v;
     else static_cast<uint16_t*>(p)[i] = dtype == kBF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+}
+// max(a, |b|), NaN if one of them is
+__device__ __forceinline__ float max_abs(float a, float b) {
+    float r;
+    asm("{\n.reg .f32 t;\nabs.f32 t, %2;\nmax.NaN.f32 %0, %1, t;\n}\n" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// Butterflies of spans FROM, 2 FROM, ... below TO inside a thread, and between lanes h apart: a + b in the lower one, a - b in the upper one,
+// one rounding each.
+template <int FROM, int TO>
+__device__ __forceinline__ void rotate_spans(float (&u)[8]) {
+#pragma unroll
+    for (int h = FROM; h < TO; h <<= 1)
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if ((j & h) == 0) {
+                const float a = u[j], b = u[j + h];
+                u[j] = __fadd_rn(a, b);
+                u[j + h] = __fsub_rn(a, b);
+            }
+}
+__device__ __forceinline__ void rotate_lanes(float (&u)[8], int lane, int h) {
+    const float sign = (lane & h) ? -1.f : 1.f;
+#pragma unroll
+    for (int j = 0; j < 8; j++) u[j] = fmaf(sign, u[j], __shfl_xor_sync(0xffffffffu, u[j], h));
+}
+// Blocks of ROT inputs of which a thread has eight in a row
+template <int ROT>
+__device__ __forceinline__ void rotate8(float (&u)[8], int lane) {
+    if (ROT == 1) return;
+    rotate_spans<1, 8>(u);
+#pragma unroll
+    for (int h = 1; h < ROT / 8; h <<= 1) rotate_lanes(u, lane, h);
+}
+
+// Eight codes rint(u / s), s > 0. m = u * inv + 1.5 * 2^23 holds the rounded product in its low bits. u * inv (inv = 1 / s) is within 1.6e-5 of the
+// quotient as fp32 rounds it (127 times 2^-24 for inv and for the quotient), so the division itself is only made where the product is next to
+// a border (or inv is no number: s below 2^-128).
+__device__ __forceinline__ uint2 codes8(const float (&u)[8], float s, float inv) {
+    constexpr float kMagic = 12582912.f, kFar = 0.49998f;
+    uint32_t m[8];
+    bool far = true;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const float v = fmaf(u[j], inv, kMagic), n = v - kMagic;
+        m[j] = __float_as_uint(v);
+        far = far && fabsf(fmaf(u[j], inv, -n)) <= kFar;
+    }
+    if (!far) {
+#pragma unroll
+        for (int j = 0; j < 8; j++)
+            if (!(fabsf(fmaf(u[j], inv, kMagic - __uint_as_float(m[j]))) <= kFar)) m[j] = (uint32_t)max(-127, min(127, __float2int_rn(__fdiv_rn(u[j], s))));
+    }
+    return make_uint2(__byte_perm(__byte_perm(m[0], m[1], 0x0040), __byte_perm(m[2], m[3], 0x0040), 0x5410),
+                      __byte_perm(__byte_perm(m[4], m[5], 0x0040), __byte_perm(m[6], m[7], 0x0040), 0x5410));
 }
 
 // A row per block, NCH times eight values per thread.
 // VEC: rows of whole, 16-byte aligned groups of eight (codes: 8-byte aligned). Else value by value: neighbouring threads take
 // neighbouring values, except where the rotation wants a thread to have eight in a row.
-// CODES, ROT: int8 codes, rotated in blocks of ROT inputs (1: not): spans 1, 2, 4 inside a thread, the others between lanes.
-template <int NCH, bool VEC, bool CODES, int ROT>
-__global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const __grid_constant__ NormParams p) {
-    __shared__ float wsum[32];
-    __shared__ uint32_t wmax[32];
+// CODES, ROT: int8 codes, rotated in blocks of ROT inputs (1: not).
+template <int NCH, int MAXT, bool VEC, bool CODES, int ROT, int HT>
+__global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant__ NormParams p) {
+    constexpr int PARTS = NCH * MAXT / 32;  // runs of 256 values
+    __shared__ float wsum[PARTS], wmax[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
     const size_t row = blockIdx.x;
     pdl_launch_dependents();
     constexpr bool RUNS = VEC || ROT > 1;  // a thread's eight values lie in a row
     auto at = [&](int c, int j) { return RUNS ? (c * (int)blockDim.x + tid) * 8 + j : (c * 8 + j) * (int)blockDim.x + tid; };
+    Raw8 rw[VEC ? NCH : 1];
+    if (VEC && p.w != nullptr) {  // (weights may be read ahead of the wait)
+#pragma unroll
+        for (int c = 0; c < NCH; c++)
+            if (at(c, 0) < p.d) rw[VEC ? c : 0] = load8(p.w, p.w_dtype, at(c, 0));
+    }
     pdl_wait();
     float v[NCH][8];  // r'
     if (VEC) {
@@ -100,21 +206,23 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const __grid_constant
 #pragma unroll
         for (int c = 0; c < NCH; c++)
             if (at(c, 0) < p.d) {
-                rr[c] = raw8_load(p.r, p.r_dtype, row * p.ldr + at(c, 0));
-                if (p.x != nullptr) xx[c] = raw8_load(p.x, p.x_dtype, row * p.ldx + at(c, 0));
+                rr[c] = load8(p.r, p.r_dtype, row * p.ldr + at(c, 0));
+                if (p.x != nullptr) xx[c] = load8(p.x, p.x_dtype, row * p.ldx + at(c, 0));
             }
 #pragma unroll
         for (int c = 0; c < NCH; c++) {
 #pragma unroll
             for (int j = 0; j < 8; j++) v[c][j] = 0.f;
             if (at(c, 0) < p.d) {
-                unpack_x8(RawX8{rr[c].a, rr[c].b}, p.r_dtype, v[c]);
+                unpack8<HT>(rr[c], p.r_dtype, v[c]);
                 if (p.x != nullptr) {
                     float xv[8];
-                    unpack_x8(RawX8{xx[c].a, xx[c].b}, p.x_dtype, xv);
+                    unpack8<HT>(xx[c], p.x_dtype, xv);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[c][j] = round_to(v[c][j] + xv[j], p.r_dtype);
-                    store8(p.r_out, p.r_dtype, row * p.ldro + at(c, 0), v[c]);
+                    for (int j = 0; j < 8; j++) v[c][j] += xv[j];
+                    const Raw8 stored = pack8<HT>(p.r_dtype, v[c]);
+                    store8(p.r_out, p.r_dtype, row * p.ldro + at(c, 0), stored);
+                    unpack8<HT>(stored, p.r_dtype, v[c]);
                 }
             }
         }
@@ -125,8 +233,8 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const __grid_constant
             for (int j = 0; j < 8; j++) {
                 v[c][j] = 0.f;
                 if (at(c, j) < p.d) {
-                    v[c][j] = scalar_load(p.r, p.r_dtype, row * p.ldr + at(c, j));
-                    if (p.x != nullptr) v[c][j] = round_to(v[c][j] + scalar_load(p.x, p.x_dtype, row * p.ldx + at(c, j)), p.r_dtype);
+                    v[c][j] = load1(p.r, p.r_dtype, row * p.ldr + at(c, j));
+                    if (p.x != nullptr) v[c][j] = round1(v[c][j] + load1(p.x, p.x_dtype, row * p.ldx + at(c, j)), p.r_dtype);
                 }
             }
         if (p.x != nullptr) {  // (behind all loads: r_out may be r)
@@ -134,70 +242,60 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const __grid_constant
             for (int c = 0; c < NCH; c++)
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    if (at(c, j) < p.d) scalar_store(p.r_out, p.r_dtype, row * p.ldro + at(c, j), v[c][j]);
+                    if (at(c, j) < p.d) store1(p.r_out, p.r_dtype, row * p.ldro + at(c, j), v[c][j]);
         }
     }
-    float sum = 0.f;
+    // The squares of 256 neighbouring values are a sum of their own, in an order that does not depend on the launch, and so are the sums' sum.
+    float sums[NCH];
 #pragma unroll
-    for (int c = 0; c < NCH; c++)
+    for (int c = 0; c < NCH; c++) {
+        sums[c] = 0.f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) sum = fmaf(v[c][j], v[c][j], sum);
+        for (int j = 0; j < 8; j++) sums[c] = fmaf(v[c][j], v[c][j], sums[c]);
+    }
     // w + offset of the thread's values
     auto weights = [&](int c, float (&w)[8]) {
 #pragma unroll
         for (int j = 0; j < 8; j++) w[j] = 1.f;
         if (p.w == nullptr) return;
         if (VEC) {
-            if (at(c, 0) < p.d) {
-                const Raw8 r = raw8_load(p.w, p.w_dtype, at(c, 0));
-                unpack_x8(RawX8{r.a, r.b}, p.w_dtype, w);
-            }
+            if (at(c, 0) < p.d) unpack8<HT>(rw[VEC ? c : 0], p.w_dtype, w);
         } else {
 #pragma unroll
             for (int j = 0; j < 8; j++)
-                if (at(c, j) < p.d) w[j] = scalar_load(p.w, p.w_dtype, at(c, j));
+                if (at(c, j) < p.d) w[j] = load1(p.w, p.w_dtype, at(c, j));
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) w[j] = __fadd_rn(w[j], p.offset);
     };
     float u[CODES ? NCH : 1][8];
-    uint32_t most = 0;  // largest |u| as bits: NaN and infinity are above every number
     if (CODES) {
+        float most = 0.f;
 #pragma unroll
         for (int c = 0; c < NCH; c++) {
             float w[8];
             weights(c, w);
 #pragma unroll
             for (int j = 0; j < 8; j++) u[c][j] = __fmul_rn(v[c][j], w[j]);
-            if (ROT > 1) {
+            rotate8<ROT>(u[c], lane);
 #pragma unroll
-                for (int h = 1; h < 8; h <<= 1)
-#pragma unroll
-                    for (int j = 0; j < 8; j++)
-                        if ((j & h) == 0) {
-                            const float a = u[c][j], b = u[c][j + h];
-                            u[c][j] = __fadd_rn(a, b);
-                            u[c][j + h] = __fsub_rn(a, b);
-                        }
-#pragma unroll
-                for (int h = 1; h < ROT / 8; h <<= 1)
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float o = __shfl_xor_sync(0xffffffffu, u[c][j], h);
-                        u[c][j] = (lane & h) ? __fsub_rn(o, u[c][j]) : __fadd_rn(u[c][j], o);
-                    }
-            }
-#pragma unroll
-            for (int j = 0; j < 8; j++) most = max(most, __float_as_uint(u[c][j]) & 0x7FFFFFFFu);
+            for (int j = 0; j < 8; j++) most = max_abs(most, u[c][j]);
         }
-        most = __reduce_max_sync(0xffffffffu, most);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = max_abs(most, __shfl_xor_sync(0xffffffffu, most, o));
         if (lane == 0) wmax[warp] = most;
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-    if (lane == 0) wsum[warp] = sum;
+    for (int c = 0; c < NCH; c++) {
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sums[c] += __shfl_xor_sync(0xffffffffu, sums[c], o);
+        if (lane == 0) wsum[c * warps + warp] = sums[c];
+    }
     __syncthreads();
-    sum = lane < warps ? wsum[lane] : 0.f;
+    float sum = 0.f;
+#pragma unroll
+    for (int c = 0; c < (PARTS + 31) / 32; c++)  // (parts beyond the row are zeros)
+        if (32 * c + lane < NCH * warps) sum += wsum[32 * c + lane];
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     const float q = rsqrtf(__fadd_rn(__fdiv_rn(sum, (float)p.d), p.eps));
@@ -209,65 +307,250 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_kernel(const __grid_constant
 #pragma unroll
             for (int j = 0; j < 8; j++) o[j] = (v[c][j] * q) * w[j];
             if (VEC) {
-                if (at(c, 0) < p.d) store8(p.out, p.out_dtype, row * p.ldo + at(c, 0), o);
+                if (at(c, 0) < p.d) store8(p.out, p.out_dtype, row * p.ldo + at(c, 0), pack8<HT>(p.out_dtype, o));
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    if (at(c, j) < p.d) scalar_store(p.out, p.out_dtype, row * p.ldo + at(c, j), o[j]);
+                    if (at(c, j) < p.d) store1(p.out, p.out_dtype, row * p.ldo + at(c, j), o[j]);
             }
         }
     }
     if (CODES) {
-        most = __reduce_max_sync(0xffffffffu, lane < warps ? wmax[lane] : 0u);
-        const bool finite = most < 0x7F800000u;
-        const float s = __fdiv_rn(__uint_as_float(most), 127.f), inv = __fdiv_rn(1.f, s);
-        if (tid == 0) p.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : most == 0 ? 0.f : __fmul_rn(s, q);
-        const bool none = !finite || most == 0;
+        float most = lane < warps ? wmax[lane] : 0.f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) most = max_abs(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const bool finite = most < INFINITY;  // (not with a NaN either)
+        const float s = __fdiv_rn(most, 127.f), inv = __fdiv_rn(1.f, s);
+        if (tid == 0) p.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : most == 0.f ? 0.f : __fmul_rn(s, q);
+        const bool none = !finite || most == 0.f;
 #pragma unroll
         for (int c = 0; c < NCH; c++) {
-            int k[8];
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                // u * (1 / s) is within 2.3e-5 of u / s (127 times two roundings and the quotient's own), so that only where it is
-                // next to a border the division has to be made (and where 1 / s is no number: rows below 1e-36)
-                const float t = u[c][j] * inv;
-                float n = rintf(t);
-                if (!(fabsf(t - n) <= 0.4999f)) n = rintf(__fdiv_rn(u[c][j], s));
-                k[j] = none ? 0 : max(-127, min(127, (int)n));
-            }
+            const uint2 k = none ? make_uint2(0, 0) : codes8(u[c], s, inv);
             if (VEC) {
-                if (at(c, 0) < p.d) {
-                    uint2 o;
-                    o.x = (uint32_t)(k[0] & 255) | (uint32_t)(k[1] & 255) << 8 | (uint32_t)(k[2] & 255) << 16 | (uint32_t)k[3] << 24;
-                    o.y = (uint32_t)(k[4] & 255) | (uint32_t)(k[5] & 255) << 8 | (uint32_t)(k[6] & 255) << 16 | (uint32_t)k[7] << 24;
-                    *reinterpret_cast<uint2*>(p.codes + row * p.ldc + at(c, 0)) = o;
-                }
+                if (at(c, 0) < p.d) *reinterpret_cast<uint2*>(p.codes + row * p.ldc + at(c, 0)) = k;
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    if (at(c, j) < p.d) p.codes[row * p.ldc + at(c, j)] = (int8_t)k[j];
+                    if (at(c, j) < p.d) p.codes[row * p.ldc + at(c, j)] = (int8_t)((j < 4 ? k.x : k.y) >> (8 * (j & 3)));
             }
+        }
+    }
+}
+
+// Many rows of up to 16384: a block takes one row after the other, a warp 512 values of it: sixteen lanes share 256 of them, and a lane has two
+// groups of eight, 128 apart, so that spans 8 to 64 of a rotation go from lane to lane. The next row is under way into shared memory
+// meanwhile, copied by the warp that uses it, so that no barrier stands between copy and use. One barrier per row, the sums of two rows in turn.
+//
+// Bound: issue slots where codes are wanted (a lane's reductions, quotients and addresses are some 120 instructions per row, a rotated value some 25), else the
+// memory. 4096 rows of 4096, bf16 added to bf16, us, the kernel of a row per block / this one: out 28.1 / 23.3 (floor 20.5), codes
+// 32.4 / 29.3, rotated 44.7 / 34.0 (18.0); 7680 wide 70 / 44, 81 / 55, 95 / 65. With one group per lane 26.2, 33.0, 37.4; with four 27.9, 30.5, 35.3; a third
+// stage 25.4, 29.5, 34.3.
+constexpr int kNormStages = 2;
+constexpr int kNormRowsSmem = 200 * 1024;  // of an SM's blocks
+template <bool OUT, bool CODES, int ROT, int HT>
+__global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const __grid_constant__ NormParams p) {
+    extern __shared__ uint4 ring[];  // r, then x: [stage][group of the lane][warp][lane]
+    __shared__ float wsum[2][64], wmax[2][32];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+    constexpr int K = 2, LB = 32 / K, APART = 256 / K;  // groups of a lane, lanes of 256 values, values between a lane's groups
+    const int first = warp * 256 * K + (lane / LB) * 256 + (lane % LB) * 8;  // the lane's first value
+    pdl_launch_dependents();
+    Raw8 rw[K];
+    if (p.w != nullptr) {  // (weights may be read ahead of the wait)
+#pragma unroll
+        for (int k = 0; k < K; k++)
+            if (first + APART * k < p.d) rw[k] = load8(p.w, p.w_dtype, first + APART * k);
+    }
+    const uint32_t r_size = p.r_dtype == kF32 ? 4 : 2, x_size = p.x == nullptr ? 0 : p.x_dtype == kF32 ? 4 : 2;
+    const uint32_t r_stage = warps * 256 * K * r_size, x_stage = warps * 256 * K * x_size;
+    const uint32_t base = smem_u32(ring), x_base = base + kNormStages * r_stage;
+    // the warp's values of a row; fp32: 32 LB bytes per LB lanes and group, each copy half of them
+    auto copy = [&](uint32_t to, const char* row, uint32_t size) {
+        const int at = size == 4 ? warp * 256 * K + (lane / LB) * 256 + (lane % LB) * 4 : first;
+        to += (warp * 32 * 8) * size + (size == 4 ? (lane / LB) * (LB * 32) + (lane % LB) * 16 : lane * 16);
+        const char* src = row + at * size;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            if (at + APART * k < p.d) cp_async_cg16(to + k * warps * 256 * size, src + APART * k * size);
+            if (size == 4 && at + APART * k + LB * 4 < p.d) cp_async_cg16(to + k * warps * 256 * size + LB * 16, src + APART * k * size + LB * 16);
+        }
+    };
+    auto fetch = [&](int s, int64_t row) {
+        if (row < p.rows) {
+            copy(base + s * r_stage, static_cast<const char*>(p.r) + row * p.ldr * r_size, r_size);
+            if (x_size != 0) copy(x_base + s * x_stage, static_cast<const char*>(p.x) + row * p.ldx * x_size, x_size);
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    auto take = [&](uint32_t from, uint32_t size, int k) {
+        from += ((k * warps + warp) * 32 + lane) * 8 * size;
+        Raw8 v;
+        v.a = lds128(from);
+        v.b = size == 4 ? lds128(from + 16) : make_uint4(0, 0, 0, 0);
+        return v;
+    };
+    auto weights = [&](int k, float (&w)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) w[j] = 1.f;
+        if (p.w == nullptr) return;
+        if (first + APART * k < p.d) unpack8<HT>(rw[k], p.w_dtype, w);
+        if (p.offset != 0.f) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = __fadd_rn(w[j], p.offset);
+        }
+    };
+    auto turned = [&](float (&u)[K][8]) {  // the rotation
+        if (ROT == 1) return;
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+            rotate_spans<1, 8>(u[k]);
+#pragma unroll
+            for (int h = 1; h < (ROT < APART ? ROT / 8 : LB); h <<= 1) rotate_lanes(u[k], lane, h);
+        }
+#pragma unroll
+        for (int h = 1; h < ROT / APART; h <<= 1)
+#pragma unroll
+            for (int k = 0; k < K; k++)
+                if ((k & h) == 0) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const float a = u[k][j], b = u[k + h][j];
+                        u[k][j] = __fadd_rn(a, b);
+                        u[k + h][j] = __fsub_rn(a, b);
+                    }
+                }
+    };
+    pdl_wait();
+#pragma unroll
+    for (int s = 0; s < kNormStages - 1; s++) fetch(s, blockIdx.x + (int64_t)s * gridDim.x);
+    int s = 0, turn = 0;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+        // (into the stage of the row before: a barrier has passed since it was read)
+        fetch(s == 0 ? kNormStages - 1 : s - 1, row + (int64_t)(kNormStages - 1) * gridDim.x);
+        asm volatile("cp.async.wait_group %0;" ::"n"(kNormStages - 1) : "memory");
+        __syncwarp();
+        float v[K][8], sums[K];
+#pragma unroll
+        for (int k = 0; k < K; k++) {
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[k][j] = 0.f;
+            if (first + APART * k < p.d) {
+                unpack8<HT>(take(base + s * r_stage, r_size, k), p.r_dtype, v[k]);
+                if (x_size != 0) {
+                    float xv[8];
+                    unpack8<HT>(take(x_base + s * x_stage, x_size, k), p.x_dtype, xv);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[k][j] += xv[j];
+                    const Raw8 stored = pack8<HT>(p.r_dtype, v[k]);
+                    store8(p.r_out, p.r_dtype, row * p.ldro + first + APART * k, stored);
+                    unpack8<HT>(stored, p.r_dtype, v[k]);
+                }
+            }
+            sums[k] = 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; j++) sums[k] = fmaf(v[k][j], v[k][j], sums[k]);
+        }
+        s = s == kNormStages - 1 ? 0 : s + 1;
+        // (the order of the other kernel's lanes: 16, 8, 4, 2 and 1 groups apart)
+        float sum = sums[0] + sums[1];
+#pragma unroll
+        for (int o = LB / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane % LB == 0) wsum[turn][warp * K + lane / LB] = sum;
+        float most = 0.f;
+        float kept[OUT && CODES ? K : 1][8];  // r', where both outputs are wanted; v is u from here on
+        if (CODES) {
+#pragma unroll
+            for (int k = 0; k < K; k++) {
+                float w[8];
+                weights(k, w);
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    if (OUT) kept[OUT ? k : 0][j] = v[k][j];
+                    v[k][j] = __fmul_rn(v[k][j], w[j]);
+                }
+            }
+            turned(v);
+#pragma unroll
+            for (int k = 0; k < K; k++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) most = max_abs(most, v[k][j]);
+            const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(most));  // (bits order as the values do, NaN last)
+            if (lane == 0) wmax[turn][warp] = __uint_as_float(m);
+        }
+        __syncthreads();
+        sum = lane < K * warps ? wsum[turn][lane] : 0.f;
+        if (32 + lane < K * warps) sum += wsum[turn][32 + lane];
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        const float q = rsqrtf(__fadd_rn(__fdiv_rn(sum, (float)p.d), p.eps));
+        if (OUT) {
+#pragma unroll
+            for (int k = 0; k < K; k++)
+                if (first + APART * k < p.d) {
+                    float w[8], o[8];
+                    weights(k, w);
+#pragma unroll
+                    for (int j = 0; j < 8; j++) o[j] = ((CODES ? kept[CODES ? k : 0][j] : v[k][j]) * q) * w[j];
+                    store8(p.out, p.out_dtype, row * p.ldo + first + APART * k, pack8<HT>(p.out_dtype, o));
+                }
+        }
+        if (CODES) {
+            most = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < warps ? __float_as_uint(wmax[turn][lane]) : 0u));
+            const bool finite = most < INFINITY;  // (not with a NaN either)
+            const float step = __fdiv_rn(most, 127.f), inv = __fdiv_rn(1.f, step);
+            const bool none = !finite || most == 0.f;
+            if (tid == 0) p.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : most == 0.f ? 0.f : __fmul_rn(step, q);
+#pragma unroll
+            for (int k = 0; k < K; k++)
+                if (first + APART * k < p.d) {
+                    const uint2 c = none ? make_uint2(0, 0) : codes8(v[k], step, inv);
+                    *reinterpret_cast<uint2*>(p.codes + row * p.ldc + first + APART * k) = c;
+                }
         }
     }
 }
 
 typedef void (*NormKernel)(NormParams);
-template <int NCH, bool VEC>
-NormKernel norm_pick(bool codes, int rotate) {
-    if (!codes) return add_rmsnorm_kernel<NCH, VEC, false, 1>;
-    return rotate == 256 ? add_rmsnorm_kernel<NCH, VEC, true, 256> : rotate == 32 ? add_rmsnorm_kernel<NCH, VEC, true, 32> : add_rmsnorm_kernel<NCH, VEC, true, 1>;
+template <int HT>
+NormKernel norm_pick_rows(bool out, bool codes, int rotate) {
+    if (!codes) return add_rmsnorm_rows_kernel<true, false, 1, HT>;
+    if (out) return rotate == 256 ? add_rmsnorm_rows_kernel<true, true, 256, HT> : rotate == 32 ? add_rmsnorm_rows_kernel<true, true, 32, HT> : add_rmsnorm_rows_kernel<true, true, 1, HT>;
+    return rotate == 256 ? add_rmsnorm_rows_kernel<false, true, 256, HT> : rotate == 32 ? add_rmsnorm_rows_kernel<false, true, 32, HT> : add_rmsnorm_rows_kernel<false, true, 1, HT>;
 }
-template <bool VEC>
-NormKernel norm_pick(int nch, bool codes, int rotate) {
-    return nch == 1 ? norm_pick<1, VEC>(codes, rotate) : nch == 2 ? norm_pick<2, VEC>(codes, rotate) : norm_pick<4, VEC>(codes, rotate);
+NormKernel norm_pick_rows(int half, bool out, bool codes, int rotate) {
+    return half == kF16 ? norm_pick_rows<kF16>(out, codes, rotate) : half == kBF16 ? norm_pick_rows<kBF16>(out, codes, rotate) : norm_pick_rows<kF32>(out, codes, rotate);
+}
+template <int NCH, int MAXT, bool VEC, int HT>
+NormKernel norm_pick(bool codes, int rotate) {
+    if (!codes) return add_rmsnorm_kernel<NCH, MAXT, VEC, false, 1, HT>;
+    return rotate == 256 ? add_rmsnorm_kernel<NCH, MAXT, VEC, true, 256, HT> : rotate == 32 ? add_rmsnorm_kernel<NCH, MAXT, VEC, true, 32, HT>
+                                                                                            : add_rmsnorm_kernel<NCH, MAXT, VEC, true, 1, HT>;
+}
+template <int NCH, int MAXT>
+NormKernel norm_pick(bool vec, int half, bool codes, int rotate) {
+    if (!vec) return norm_pick<NCH, MAXT, false, kF32>(codes, rotate);
+    return half == kF16 ? norm_pick<NCH, MAXT, true, kF16>(codes, rotate) : half == kBF16 ? norm_pick<NCH, MAXT, true, kBF16>(codes, rotate)
+                                                                                          : norm_pick<NCH, MAXT, true, kF32>(codes, rotate);
 }
 
 bool known(int32_t dtype) { return dtype >= 0 && dtype <= 2; }
-bool aligned(const void* p, int64_t ld, int esz, int to) {
-    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % to == 0 && ld * esz % to == 0);
+// whether every group of eight of the rows lies on its own size
+bool aligned(const void* p, int64_t ld, int esz) {
+    return p == nullptr || (reinterpret_cast<uintptr_t>(p) % (8 * esz) == 0 && ld % 8 == 0);
 }
 
 }  // namespace
+
+int32_t norm_init(iq_ctx* ctx) {
+    for (int half = 0; half < 3; half++)
+        for (int mode = 0; mode < 7; mode++) {  // out; out and codes of three rotations; codes of three
+            const NormKernel k = norm_pick_rows(half, mode < 4, mode != 0, mode % 3 == 2 ? 32 : mode % 3 == 0 ? 256 : 0);
+            const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributeMaxDynamicSharedMemorySize, kNormRowsSmem);
+            if (e != cudaSuccess) return check_cuda(ctx, e, "cudaFuncSetAttribute(add_rmsnorm_rows)");
+        }
+    return kOk;
+}
+
 }  // namespace iq
 
 using namespace iq;
@@ -296,14 +579,34 @@ extern "C" int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int3
     p.x = x; p.r = residual; p.r_out = residual_out; p.w = weight; p.out = out; p.codes = codes; p.scales = scales;
     p.ldx = ldx; p.ldr = ldr; p.ldro = ldro; p.ldo = ldo; p.ldc = ldc;
     p.x_dtype = x_dtype; p.r_dtype = r_dtype; p.w_dtype = w_dtype; p.out_dtype = out_dtype;
-    p.d = d; p.offset = weight_offset; p.eps = eps;
-    const bool vec = d % 8 == 0 && aligned(x, ldx, dtype_size(x_dtype), 16) && aligned(residual, ldr, dtype_size(r_dtype), 16) &&
-                     aligned(residual_out, ldro, dtype_size(r_dtype), 16) && aligned(weight, 0, 1, 16) && aligned(out, ldo, dtype_size(out_dtype), 16) &&
-                     aligned(codes, ldc, 1, 8);
-    const int groups = (d + 7) / 8, nch = groups <= 1024 ? 1 : groups <= 2048 ? 2 : 4;
-    const int threads = round_up((groups + nch - 1) / nch, 32);
-    const NormKernel kernel = vec ? norm_pick<true>(nch, codes != nullptr, rotate) : norm_pick<false>(nch, codes != nullptr, rotate);
+    p.rows = rows; p.d = d; p.offset = weight_offset; p.eps = eps;
+    const bool vec = d % 8 == 0 && aligned(x, ldx, dtype_size(x_dtype)) && aligned(residual, ldr, dtype_size(r_dtype)) && aligned(residual_out, ldro, dtype_size(r_dtype)) &&
+                     aligned(weight, 0, dtype_size(w_dtype)) && aligned(out, ldo, dtype_size(out_dtype)) && aligned(codes, ldc, 1);
+    const int groups = (d + 7) / 8, nch = groups <= 1024 ? 1 : 4;
+    int threads = round_up((groups + nch - 1) / nch, 32), blocks = rows;
+    size_t smem = 0;
+    // the one 16-bit type of the call (bf16 where it has none), kF32 where it has both
+    int half = -1;
+    auto meet = [&](const void* t, int32_t dtype) {
+        if (t != nullptr && dtype != kF32) half = half == -1 || half == dtype ? dtype : kF32;
+    };
+    meet(x, x_dtype); meet(residual, r_dtype); meet(weight, w_dtype); meet(out, out_dtype);
+    if (half == -1) half = kBF16;
+    const bool c8 = codes != nullptr;
+    NormKernel kernel = nch == 1 ? norm_pick<1, 1024>(vec, half, c8, rotate) : threads <= 512 ? norm_pick<4, 512>(vec, half, c8, rotate)
+                                                                                              : norm_pick<4, 1024>(vec, half, c8, rotate);
+    // Many rows: more than the blocks that run at once (of 64 registers a thread, the stages in shared memory). The norm alone of an fp32 sum is at the memory's
+    // rate up to some 5000 values with a row per block as well, and faster (4096 rows of 4096: 31.9 against 37.0 us; of 7680: 75 against 69).
+    const int row_threads = (d + 511) / 512 * 32;
+    const size_t row_smem = (size_t)kNormStages * row_threads * 16 * (dtype_size(r_dtype) + (x == nullptr ? 0 : dtype_size(x_dtype)));
+    const int at_once = row_threads > 1024 ? 0 : ctx->sms * (int)std::min<size_t>({(size_t)(1024 / row_threads), kNormRowsSmem / row_smem, 16});
+    if (vec && at_once > 0 && rows > at_once && (c8 || r_dtype != kF32 || d > 5120)) {
+        kernel = norm_pick_rows(half, out != nullptr, c8, rotate);
+        threads = row_threads;
+        blocks = at_once;
+        smem = row_smem;
+    }
     DeviceScope on(ctx);
     if (on.error != cudaSuccess) return check_cuda(ctx, on.error, "add_rmsnorm device");
-    return check_cuda(ctx, launch_dependent(kernel, dim3(rows), threads, 0, reinterpret_cast<cudaStream_t>(stream), p), "add_rmsnorm launch");
+    return check_cuda(ctx, launch_dependent(kernel, dim3(blocks), threads, smem, reinterpret_cast<cudaStream_t>(stream), p), "add_rmsnorm launch");
 }

@@ -225,3 +225,44 @@ def test_refusals_reach_no_kernel(cuda_device):
     with pytest.raises(ValueError, match="different devices"):
         add_rmsnorm(None, r, torch.ones(64), 2, out=r.clone())
     assert norm.MAX_WIDTH == 32768
+
+
+@pytest.mark.parametrize("rows,d,xt,rt,wt,ot,rotate,out,codes", [
+    (2400, 512, BF16, BF16, BF16, BF16, 256, True, True), (2400, 520, F16, F32, F32, F16, 0, False, True), (700, 2880, F16, F16, F16, F32, 32, True, True),
+    (700, 4096, BF16, F32, BF16, BF16, 256, False, True), (650, 4096, BF16, BF16, BF16, BF16, 0, True, False), (500, 5128, None, F32, None, F16, 0, True, False),
+    (460, 7680, F32, F16, BF16, F32, 256, True, True), (300, 8192, F32, F32, F32, F32, 32, False, True), (160, 16384, BF16, BF16, BF16, BF16, 256, False, True),
+    (160, 14344, BF16, BF16, F32, BF16, 0, True, True), (160, 16384, F32, F32, F32, F32, 0, True, True)])
+def test_the_kernel_of_many_rows(cuda_device, rows, d, xt, rt, wt, ot, rotate, out, codes):
+    """More rows than blocks that run at once, up to more than two per block; the bits of a row are those of a call of its own."""
+    gen = torch.Generator().manual_seed(rows + d)
+    got = run(gen, rows, d, xt, rt, wt, ot, rotate, 32, want_out=out, want_codes=codes)
+    check(got, 0.0, 1e-6, rotate)
+    x, r, w, ro, o, c, s = got
+    for t in (0, rows // 2, rows - 1):
+        one = {}
+        if out:
+            one["out"] = torch.empty(1, d, dtype=ot, device="cuda")
+        if codes:
+            one.update(codes=torch.empty(1, d, dtype=torch.int8, device="cuda"), scales=torch.empty(1, device="cuda"), rotate=rotate)
+        add_rmsnorm(None if x is None else x[t:t + 1].cuda(), r[t:t + 1].cuda(), None if w is None else w.cuda(), 1, **one)
+        if out:
+            assert torch.equal(one["out"][0].cpu(), o[t])
+        if codes:
+            assert torch.equal(one["codes"][0].cpu(), c[t]) and torch.equal(one["scales"].cpu()[0], s[t])
+
+
+def test_many_rows_in_place_and_poisoned(cuda_device):
+    rows, d = 1500, 4096
+    gen = torch.Generator().manual_seed(12)
+    x, r = torch.randn(rows, d, generator=gen).to(F16), torch.randn(rows, d, generator=gen).to(F16)
+    r[700, 5], r[701] = float("nan"), 0
+    x[701] = 0
+    xd, rd = x.cuda(), r.cuda()
+    codes, scales = torch.empty(rows, d, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    add_rmsnorm(xd, rd, None, rows, out=xd, codes=codes, scales=scales, rotate=256)
+    total = (x.float() + r.float()).to(F16)
+    assert torch.equal(torch.nan_to_num(rd.cpu(), 99), torch.nan_to_num(total, 99))
+    assert (codes[700:702] == 0).all() and scales[700].isnan() and scales[701] == 0 and (xd[701] == 0).all() and xd[700].isnan().all()
+    keep = [t for t in range(rows) if t not in (700, 701)]
+    want, _ = qref.norm_codes(total[keep].float().numpy(), np.ones(d, np.float32), 256)
+    assert np.array_equal(codes[keep].cpu().numpy(), want)
