@@ -195,6 +195,21 @@ int32_t iq_qmm_w8a8_workspace_bytes(iq_ctx* ctx, const iq_qlinear* m, int32_t ro
 int32_t iq_qmm_w8a8(iq_ctx* ctx, void* stream, const void* x, int32_t x_dtype, int64_t ldx, const iq_qlinear* m, void* y,
                     int32_t y_dtype, int64_t ldy, int32_t rows, uint32_t flags, void* workspace, size_t workspace_bytes);
 
+/* W8A8 linear on rows that are int8 already: Y[rows, n] (+)= (sum_k X[t, k] W[o, k]) * x_scales[t] * w_scales[o]. iq_qmm_w8a8 converts both
+ * sides in every call and takes 64 rows at a time; here the weights are packed once (iq_i8_pack, or any int8 matrix with a scale
+ * per row), the activations come from iq_add_rmsnorm (or any int8 rows), and any number of rows from one on is taken.
+ * x: int8 [rows, ldx], 16-byte aligned, ldx a multiple of 16; w: int8 [n, k] without gaps, 16-byte aligned; k a multiple of 16 up to
+ * 131,056, where the sums are exact in 32 bits for all codes (-128 too): the result does not depend on the other rows, nor on how a
+ * call is divided. y of fp32, fp16 or bf16: fp32(fp32(sum) * x_scale) * w_scale, rounded once more for 16 bits; with
+ * IQ_FLAG_ACCUMULATE added to y in fp32. Rows and columns of y beyond rows and n stay as they are. rows = 0 does nothing.
+ * y may not overlap the operands. */
+int32_t iq_qmm_i8(iq_ctx* ctx, void* stream, const int8_t* x, int64_t ldx, const float* x_scales, const int8_t* w, const float* w_scales,
+                  int32_t n, int32_t k, void* y, int32_t y_dtype, int64_t ldy, int32_t rows, uint32_t flags);
+/* A 4-bit affine matrix (group 64 or 32; k a multiple of 64, at most 49,152) as int8 rows [n, k] with a scale per row, rotated in blocks of `rotate`
+ * inputs (0, 32 or 256, a divisor of k) as the activations will be; the scales take the transform's factor, so that codes of H x meet
+ * codes of H w as they are. Done once, at load time. */
+int32_t iq_i8_pack(iq_ctx* ctx, void* stream, const iq_qlinear* m, int32_t rotate, int8_t* w, float* scales);
+
 /* ---- dense gated FFN ------------------------------------------------------------------------------------------------
  * out[rows, d] (+)= down( act(gate x) * up x ) with gate|up concatenated by rows as one [2*d_ff, d] matrix (gate rows
  * first). Replaces DenseMLP.encode / encodePrefill (Sources/Ingot/Layers/Dense.swift:56-96) and dswiglu*

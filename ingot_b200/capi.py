@@ -34,7 +34,7 @@ SYMBOLS = [
     "iq_ctx_set_wait_cycles", "iq_colsplit_create", "iq_colsplit_destroy", "iq_linear_colsplit_workspace_bytes",
     "iq_linear_colsplit", "iq_had_rows", "iq_embed_rows_ternary", "iq_qmm_w8a8_workspace_bytes", "iq_qmm_w8a8",
     "iq_qmm_plan", "iq_qmv_plan", "iq_ep_index", "iq_moe_experts_indexed", "iq_ep_pack_push_tokens", "iq_ep_index_tokens",
-    "iq_add_rmsnorm",
+    "iq_add_rmsnorm", "iq_i8_pack", "iq_qmm_i8",
 ]
 
 
@@ -192,7 +192,10 @@ def lib() -> C.CDLL:
             getattr(l, name).restype = i32
         l.iq_add_rmsnorm.argtypes = [vp, vp, vp, i32, i64, vp, i32, i64, vp, i64, vp, i32, C.c_float, C.c_float, i32, i32, vp, i32, i64,
                                      vp, i64, vp, i32]
-        l.iq_add_rmsnorm.restype = i32
+        l.iq_i8_pack.argtypes = [vp, vp, C.POINTER(QLinear), i32, vp, vp]
+        l.iq_qmm_i8.argtypes = [vp, vp, vp, i64, vp, vp, vp, i32, i32, vp, i32, i64, i32, u32]
+        for name in ("iq_add_rmsnorm", "iq_i8_pack", "iq_qmm_i8"):
+            getattr(l, name).restype = i32
         for name in ("iq_ctx_create", "iq_qmv", "iq_qmm_workspace_bytes", "iq_qmm", "iq_dense_ffn_workspace_bytes",
                      "iq_dense_ffn", "iq_moe_create", "iq_moe_workspace_bytes", "iq_moe_forward", "iq_moe_route",
                      "iq_moe_set_external_routing", "iq_moe_get_views"):
@@ -216,7 +219,7 @@ def call():
         mod = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_iqcall", CALL_PATH, loader=loader))
         loader.exec_module(mod)
         for name in ("iq_qmv", "iq_qmm", "iq_dense_ffn", "iq_moe_forward", "iq_rmsnorm", "iq_had_rows", "iq_embed_rows",
-                     "iq_argmax_rows", "iq_topk64", "iq_add_rmsnorm"):
+                     "iq_argmax_rows", "iq_topk64", "iq_add_rmsnorm", "iq_qmm_i8"):
             mod.bind(name, C.cast(getattr(l, name), C.c_void_p).value)
         _call = mod
     return _call

@@ -19,12 +19,13 @@ static void* fn_embed_rows;
 static void* fn_argmax_rows;
 static void* fn_topk64;
 static void* fn_add_rmsnorm;
+static void* fn_qmm_i8;
 
 static const struct { const char* name; void** slot; } table[] = {
     {"iq_qmv", &fn_qmv},           {"iq_qmm", &fn_qmm},               {"iq_dense_ffn", &fn_dense_ffn},
     {"iq_moe_forward", &fn_moe_forward}, {"iq_rmsnorm", &fn_rmsnorm}, {"iq_had_rows", &fn_had_rows},
     {"iq_embed_rows", &fn_embed_rows},   {"iq_argmax_rows", &fn_argmax_rows}, {"iq_topk64", &fn_topk64},
-    {"iq_add_rmsnorm", &fn_add_rmsnorm},
+    {"iq_add_rmsnorm", &fn_add_rmsnorm}, {"iq_qmm_i8", &fn_qmm_i8},
 };
 
 static PyObject* py_bind(PyObject* self, PyObject* args) {
@@ -168,9 +169,20 @@ ENTRY(add_rmsnorm, 23, add_norm_t, {
     LAUNCH(f(c, s, x, xd, ldx, r, rd, ldr, ro, ldro, w, wd, off, eps, rows, d, o, od, ldo, q, ldc, sc, rot));
 })
 
+typedef int32_t (*qmm_i8_t)(iq_ctx*, void*, const int8_t*, int64_t, const float*, const int8_t*, const float*, int32_t, int32_t, void*, int32_t, int64_t,
+                            int32_t, uint32_t);
+ENTRY(qmm_i8, 14, qmm_i8_t, {
+    void *c = P(0), *s = P(1), *x = P(2), *sx = P(4), *w = P(5), *sw = P(6), *y = P(9);
+    int32_t nn = I32(7), k = I32(8), yd = I32(10), rows = I32(12);
+    int64_t ldx = I64(3), ldy = I64(11);
+    uint32_t fl = U32(13);
+    CHECKED;
+    LAUNCH(f(c, s, x, ldx, sx, w, sw, nn, k, y, yd, ldy, rows, fl));
+})
+
 #define M(NAME) {#NAME, (PyCFunction)(void (*)(void))py_##NAME, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {
     {"bind", py_bind, METH_VARARGS, NULL}, M(qmv), M(qmm), M(dense_ffn), M(moe_forward), M(rmsnorm), M(had_rows), M(embed_rows),
-    M(argmax_rows), M(topk64), M(add_rmsnorm), {NULL, NULL, 0, NULL}};
+    M(argmax_rows), M(topk64), M(add_rmsnorm), M(qmm_i8), {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_iqcall", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__iqcall(void) { return PyModule_Create(&module); }

@@ -14,12 +14,12 @@ namespace {
 
 // One block per row: the row's K floats in shared memory, the Hadamard transform of every block of n inputs (spans
 // 1, 2, ..., n / 2: a + b and a - b), the row's largest magnitude, then the int8 codes.
-// SRC 0: 4-bit affine weights (w, scales, biases; group 64 or 32); SRC 1: activations of any dtype.
+// SRC 0: 4-bit affine weights (w, scales, biases; group 64 or 32); SRC 1: activations of any dtype. The scales are stored times factor.
 template <int SRC>
 __global__ void __launch_bounds__(256) rot_quant_rows_kernel(const void* __restrict__ src, const uint16_t* __restrict__ sc,
                                                             const uint16_t* __restrict__ bi, int group, int32_t x_dtype,
                                                             int64_t ld, int K, int n, int8_t* __restrict__ q,
-                                                            float* __restrict__ scale_out) {
+                                                            float* __restrict__ scale_out, float factor) {
     extern __shared__ float row[];  // [K]
     __shared__ float wmax[8];
     const int tid = threadIdx.x, r = blockIdx.x;
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(256) rot_quant_rows_kernel(const void* __restr
 #pragma unroll
     for (int i = 1; i < 8; i++) amax = fmaxf(amax, wmax[i]);
     const float s = amax > 0.f ? __fdiv_rn(amax, 127.0f) : 1.0f;
-    if (tid == 0) scale_out[r] = s;
+    if (tid == 0) scale_out[r] = s * factor;
     for (int i = tid; i < K / 4; i += 256) {
         char4 o;
         int c[4];
@@ -194,8 +194,8 @@ extern "C" int32_t iq_qmm_w8a8(iq_ctx* ctx, void* stream, const void* x, int32_t
     else
         rot_quant_rows_kernel<0><<<m->n, 256, smem, cs>>>(m->w, static_cast<const uint16_t*>(m->scales),
                                                           static_cast<const uint16_t*>(m->biases), m->group, 0, 0, m->k, n, w.wq,
-                                                          w.sw);
-    rot_quant_rows_kernel<1><<<rows, 256, smem, cs>>>(x, nullptr, nullptr, 0, x_dtype, ldx, m->k, n, w.xq, w.sx);
+                                                          w.sw, 1.0f);
+    rot_quant_rows_kernel<1><<<rows, 256, smem, cs>>>(x, nullptr, nullptr, 0, x_dtype, ldx, m->k, n, w.xq, w.sx, 1.0f);
     st = check_cuda(ctx, cudaGetLastError(), "rot_quant_rows launch");
     if (st != kOk) return st;
     QmmCall c;
@@ -208,4 +208,23 @@ extern "C" int32_t iq_qmm_w8a8(iq_ctx* ctx, void* stream, const void* x, int32_t
     c.accumulate = (flags & IQ_FLAG_ACCUMULATE) ? 1 : 0;
     c.limit = 1.0f / (float)n;  // (H x) . (H w) = n x . w with the unnormalised transform of size n
     return launch_qmm(ctx, cs, c);
+}
+
+extern "C" int32_t iq_i8_pack(iq_ctx* ctx, void* stream, const iq_qlinear* m, int32_t rotate, int8_t* w, float* scales) {
+    // (the checks come before the context is looked at: they are the same without a GPU)
+    if (m == nullptr || m->w == nullptr || m->scales == nullptr || m->biases == nullptr || w == nullptr || scales == nullptr || reinterpret_cast<uintptr_t>(w) % 16 != 0)
+        return fail(ctx, kErrInvalidArg, "i8_pack: null pointer, or w is not 16-byte aligned");
+    if (m->mode != IQ_MODE_AFFINE || m->experts > 1 || m->bits != 4 || (m->group != 64 && m->group != 32))
+        return fail(ctx, kErrUnsupported, "i8_pack: %d-bit group %d mode %d (4-bit affine with group 64 or 32)", m->bits, m->group, m->mode);
+    if (m->n < 1 || m->k < 64 || m->k % 64 != 0 || m->k > 49152) return fail(ctx, kErrInvalidArg, "i8_pack: n = %d, k = %d (a multiple of 64, at most 49152)", m->n, m->k);
+    if ((rotate != 0 && rotate != 32 && rotate != 256) || (rotate != 0 && m->k % rotate != 0))
+        return fail(ctx, kErrInvalidArg, "i8_pack: rotation in blocks of %d (0, 32 or 256 inputs that divide k = %d)", rotate, m->k);
+    if (ctx == nullptr) return kErrInvalidArg;
+    DeviceScope on(ctx);
+    if (on.error != cudaSuccess) return check_cuda(ctx, on.error, "i8_pack device");
+    const int n = rotate == 0 ? 1 : rotate;
+    // (H x) . (H w) = n x . w: the weights' scales take the 1 / n
+    rot_quant_rows_kernel<0><<<m->n, 256, (size_t)m->k * sizeof(float), reinterpret_cast<cudaStream_t>(stream)>>>(
+        m->w, static_cast<const uint16_t*>(m->scales), static_cast<const uint16_t*>(m->biases), m->group, 0, 0, m->k, n, w, scales, 1.0f / (float)n);
+    return check_cuda(ctx, cudaGetLastError(), "i8_pack launch");
 }

@@ -273,6 +273,74 @@ class VQMV:
             ctx.check(st)
 
 
+class I8Linear:
+    """A W8A8 linear on weights packed once: int8 rows [N, K] and a float32 scale per row (iq_qmm_i8). `rotate`: the block of the Hadamard transform
+    that its inputs have gone through as well (0: none), for add_rmsnorm(rotate=)."""
+
+    MAX_K = 131056
+
+    def __init__(self, w: torch.Tensor, scales: torch.Tensor, rotate: int = 0):
+        if w.dim() != 2 or w.dtype != torch.int8 or scales.dtype != torch.float32:
+            raise TypeError("weights are int8 [N, K], scales float32 [N]")
+        if scales.numel() != w.shape[0] or not w.is_contiguous() or not scales.is_contiguous():
+            raise ValueError(f"weights {tuple(w.shape)} and one scale per row, both contiguous")
+        if w.shape[0] < 1 or w.shape[1] < 16 or w.shape[1] % 16 or w.shape[1] > self.MAX_K:
+            raise ValueError(f"K is a multiple of 16 up to {self.MAX_K}, not {w.shape[1]}")
+        if rotate not in (0, 32, 256) or (rotate and w.shape[1] % rotate):
+            raise ValueError(f"the rotation has blocks of 32 or 256 inputs that divide K = {w.shape[1]}, not {rotate}")
+        if w.device != scales.device:
+            raise ValueError("weights and scales are on different devices")
+        _need_cuda(w, scales)
+        self.w, self.scales, self.rotate = w, scales, rotate
+        self.N, self.K = w.shape
+
+    @classmethod
+    def pack(cls, m: DenseQ, rotate: Optional[int] = None, stream: Optional[torch.cuda.Stream] = None) -> "I8Linear":
+        """The int8 form of a 4-bit affine matrix. rotate None: blocks of 256 inputs where they divide K, else of 32."""
+        if rotate is None:
+            rotate = 256 if m.K % 256 == 0 else 32
+        dev = m.w.device
+        w, s = torch.empty(m.N, m.K, dtype=torch.int8, device=dev), torch.empty(m.N, dtype=torch.float32, device=dev)
+        ctx, q = capi.context(m.device_index), m.qlinear()
+        ctx.check(capi.lib().iq_i8_pack(ctx.handle, stream.cuda_stream if stream is not None else _raw_stream(m.device_index), C.byref(q), rotate, w.data_ptr(), s.data_ptr()))
+        return cls(w, s, rotate)
+
+    def _check(self, x, x_scales, y, rows):
+        """Shapes, types and devices, whatever device they are on."""
+        if x.dtype != torch.int8 or x_scales.dtype != torch.float32 or y.dtype not in _DT:
+            raise TypeError("x is int8, x_scales float32, y float32, float16 or bfloat16")
+        if x.dim() != 2 or y.dim() != 2 or rows < 0 or x.shape[0] < rows or y.shape[0] < rows or x.shape[1] != self.K or y.shape[1] != self.N:
+            raise ValueError(f"x is [at least {rows}, {self.K}], y [at least {rows}, {self.N}], not {tuple(x.shape)} and {tuple(y.shape)}")
+        if x.stride(1) != 1 or (self.N > 1 and y.stride(1) != 1) or (rows > 1 and x.stride(0) % 16) or x.data_ptr() % 16:
+            raise ValueError("rows of neighbouring elements, x's 16-byte aligned")
+        if x_scales.dim() != 1 or x_scales.shape[0] < rows or (rows > 1 and x_scales.stride(0) != 1):
+            raise ValueError(f"x_scales is [at least {rows}], contiguous")
+        if not x.device == x_scales.device == y.device == self.w.device:
+            raise ValueError("the tensors are on different devices")
+
+    def encode(self, x: torch.Tensor, x_scales: torch.Tensor, y: torch.Tensor, rows: int, accumulate: bool = False,
+               stream: Optional[torch.cuda.Stream] = None):
+        """y[rows, N] (+)= (x codes · wᵀ codes) · x_scales · scales for int8 rows x [rows, K], any number of them."""
+        dev = self.w.get_device()
+        if not (dev >= 0 and x.get_device() == dev and x_scales.get_device() == dev and y.get_device() == dev and x.dim() == 2 and y.dim() == 2 and x_scales.dim() == 1):
+            self._check(x, x_scales, y, rows)
+            _need_cuda(x)
+            raise ValueError("I8Linear does not take these tensors")
+        (xr, xk), (ldx, xs), (yr, yn), (ldy, ys) = x.shape, x.stride(), y.shape, y.stride()
+        yt = _DT.get(y.dtype, -1)
+        if not (0 <= rows <= xr and rows <= yr and xk == self.K and yn == self.N and xs == 1 and (ys == 1 or yn == 1) and yt >= 0 and x.dtype == torch.int8
+                and x_scales.dtype == torch.float32 and x_scales.shape[0] >= rows and (rows <= 1 or x_scales.stride(0) == 1)):
+            self._check(x, x_scales, y, rows)
+            raise ValueError("I8Linear does not take these tensors")
+        if rows <= 1:  # (one row has no stride)
+            ldx, ldy = xk, yn
+        ctx = capi.context(dev)
+        st = capi.call().qmm_i8(ctx.address, stream.cuda_stream if stream is not None else _raw_stream(dev), x.data_ptr(), ldx, x_scales.data_ptr(), self.w.data_ptr(),
+                                self.scales.data_ptr(), yn, xk, y.data_ptr(), yt, ldy, rows, capi.IQ_FLAG_ACCUMULATE if accumulate else 0)
+        if st:
+            ctx.check(st)
+
+
 class DenseMLP:
     """Dense gated FFN with gate|up concatenated by rows ([2·I, D], gate rows first; Dense.swift:4-6,21-49)."""
 

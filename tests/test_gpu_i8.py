@@ -1,0 +1,156 @@
+"""W8A8 linears on packed int8 rows (iq_qmm_i8 through linear.I8Linear): bit for bit, since the sums are exact integers and what follows is
+a fixed order of fp32 operations. And the packing of 4-bit matrices."""
+import numpy as np
+import pytest
+import torch
+
+from ingot_b200 import capi
+from ingot_b200.linear import I8Linear
+from ingot_b200.norm import add_rmsnorm
+from oracle import qref
+from gpu_util import affine_case, deq
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def codes(gen, rows, k, low=-127):
+    return torch.randint(low, 128, (rows, k), generator=gen, dtype=torch.int8)
+
+
+def reference(x, sx, w, sw, base=None):
+    """fp32(fp32(sum) * sx) * sw (+ base), the sums in 64 bits"""
+    s = torch.from_numpy(x.numpy().astype(np.float64) @ w.numpy().astype(np.float64).T)  # exact: below 2^53
+    y = s.to(F32) * sx[:, None] * sw[None, :]
+    return y if base is None else y + base.float()
+
+
+def run(gen, rows, n, k, dtype=F32, accumulate=False, pad=0, low=-127, x=None, w=None):
+    x = codes(gen, rows, k, low) if x is None else x
+    w = codes(gen, n, k, low) if w is None else w
+    sx, sw = torch.rand(rows, generator=gen) + 0.01, torch.rand(n, generator=gen) * 1e-3 + 1e-5
+    wide = torch.full((rows + 1, k + 16 * pad), 55, dtype=torch.int8, device="cuda")  # (what lies beside the rows is not read)
+    wide[:rows, :k] = x.cuda()
+    base = torch.randn(rows + 2, n + pad, generator=gen).to(dtype)
+    y = base.cuda()
+    m = I8Linear(w.cuda(), sw.cuda())
+    m.encode(wide[:, :k], sx.cuda(), y[:, :n], rows, accumulate=accumulate)
+    assert capi.context(0).device_status() == 0
+    got = y.cpu()
+    want = reference(x, sx, w, sw, base[:rows, :n] if accumulate else None).to(dtype)
+    assert torch.equal(got[:rows, :n], want)
+    assert torch.equal(got[rows:], base[rows:]) and torch.equal(got[:, n:], base[:, n:])
+
+
+@pytest.mark.parametrize("rows", [1, 2, 15, 16, 17, 31, 33, 48, 64, 65, 100, 128, 129, 200, 256, 257, 300, 513])
+@pytest.mark.parametrize("n,k", [(256, 512), (300, 1040), (129, 4096)])
+def test_rows(cuda_device, rows, n, k):
+    run(torch.Generator().manual_seed(rows * 7 + n), rows, n, k)
+
+
+@pytest.mark.parametrize("n,k", [(1, 16), (1, 4096), (3, 48), (127, 128), (128, 144), (2880, 2880), (4097, 640), (1000, 8208), (512, 14336), (9472, 256), (37888, 128)])
+@pytest.mark.parametrize("rows", [1, 9, 70])
+def test_features_and_inputs(cuda_device, rows, n, k):
+    run(torch.Generator().manual_seed(rows + n + k), rows, n, k)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("rows,n,k,pad", [(1, 384, 2048, 0), (5, 130, 2048, 3), (40, 257, 512, 1), (300, 200, 384, 5), (700, 1030, 512, 2)])
+def test_types_accumulation_and_strides(cuda_device, dtype, accumulate, rows, n, k, pad):
+    run(torch.Generator().manual_seed(rows + n), rows, n, k, dtype, accumulate, pad)
+
+
+@pytest.mark.parametrize("rows,n,k", [(1100, 1500, 1024), (2048, 4096, 528), (1030, 300, 2064), (4100, 256, 256), (600, 9000, 144)])
+def test_many_tiles(cuda_device, rows, n, k):
+    run(torch.Generator().manual_seed(rows), rows, n, k, BF16)
+
+
+def test_the_largest_sums(cuda_device):
+    """Every code -128 at the most inputs: 131,056 * 2^14 is below 2^31."""
+    k = I8Linear.MAX_K
+    full = torch.full((2, k), -128, dtype=torch.int8)
+    run(torch.Generator().manual_seed(1), 2, 2, k, x=full, w=full)
+    run(torch.Generator().manual_seed(2), 3, 130, k, low=-128)
+
+
+def test_a_row_does_not_depend_on_the_others(cuda_device):
+    gen = torch.Generator().manual_seed(3)
+    x, w = codes(gen, 600, 2048).cuda(), codes(gen, 1000, 2048).cuda()
+    sx, sw = torch.rand(600, generator=gen).cuda(), torch.rand(1000, generator=gen).cuda()
+    m = I8Linear(w, sw)
+    y = torch.empty(600, 1000, device="cuda")
+    m.encode(x, sx, y, 600)
+    for lo, hi in ((0, 1), (17, 33), (100, 140), (500, 600), (0, 257)):
+        part = torch.empty(hi - lo, 1000, device="cuda")
+        m.encode(x[lo:hi], sx[lo:hi], part, hi - lo)
+        assert torch.equal(part, y[lo:hi])
+
+
+@pytest.mark.parametrize("rows", [3, 400])
+def test_streams_and_graphs(cuda_device, rows):
+    gen = torch.Generator().manual_seed(4)
+    n, k = 520, 1024
+    x, w = codes(gen, rows, k).cuda(), codes(gen, n, k).cuda()
+    sx, sw = torch.rand(rows, generator=gen).cuda(), torch.rand(n, generator=gen).cuda()
+    m, y = I8Linear(w, sw), torch.zeros(rows, n, device="cuda")
+    m.encode(x, sx, y, rows)
+    want = y.clone()
+    side = torch.cuda.Stream()
+    y.zero_()
+    side.wait_stream(torch.cuda.current_stream())
+    m.encode(x, sx, y, rows, stream=side)
+    side.synchronize()
+    assert torch.equal(y, want)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        m.encode(x, sx, y, rows)
+        m.encode(x, sx, y, rows, accumulate=True)
+    y.zero_()
+    g.replay()
+    x.neg_()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want + want)
+    g.replay()
+    assert torch.equal(y, -want - want)
+    y.fill_(5)
+    m.encode(x, sx, y, 0)
+    assert (y == 5).all()
+
+
+@pytest.mark.parametrize("N,K,group,rotate", [(64, 1024, 64, 256), (100, 1024, 64, 32), (3, 64, 64, 0), (48, 2880, 64, 32), (130, 768, 32, 256), (16, 128, 32, 0)])
+def test_packing(cuda_device, N, K, group, rotate):
+    rng = np.random.default_rng(N + K)
+    m, host = affine_case(rng, N, K, 4, cuda_device, group=group)
+    wf = deq(host, 4, group=group)
+    got = I8Linear.pack(m, rotate)
+    n = max(rotate, 1)
+    want, s = qref.quant_i8_rows(qref.fwht(wf.reshape(N, K // n, n)).reshape(N, K))
+    assert np.array_equal(got.w.cpu().numpy(), want) and np.array_equal(got.scales.cpu().numpy(), s / np.float32(n)) and got.rotate == rotate
+
+
+@pytest.mark.parametrize("rows,K,rotate", [(1, 2048, 256), (7, 2880, 32), (130, 1024, 256), (700, 2048, 256)])
+def test_codes_into_linear(cuda_device, rows, K, rotate):
+    """The step as it is used: residual, norm and codes, then the linear, against the exact norm and weights. Rounding to 127 steps of the largest of a row
+    on both sides: each product's error is at most half a step of one side times the other's value, independent and of either sign; for rows of
+    normal values (largest some 4 times the root mean square) that is 4 / 127 / sqrt(12) = 0.9 % per side, 1.3 % of the result's root mean square in all,
+    and its largest of 10^5 values some 4.5 times that."""
+    rng = np.random.default_rng(rows)
+    N = 192
+    m, host = affine_case(rng, N, K, 4, cuda_device)
+    lin = I8Linear.pack(m)
+    assert lin.rotate == rotate
+    x, r = torch.from_numpy(rng.normal(size=(rows, K)).astype(np.float32)), torch.from_numpy(rng.normal(size=(rows, K)).astype(np.float32))
+    g = torch.from_numpy((1 + 0.1 * rng.normal(size=K)).astype(np.float32))
+    xq, sx = torch.empty(rows, K, dtype=torch.int8, device="cuda"), torch.empty(rows, device="cuda")
+    y, ro = torch.empty(rows, N, device="cuda"), torch.empty(rows, K, device="cuda")
+    add_rmsnorm(x.cuda(), r.cuda(), g.cuda(), rows, residual_out=ro, codes=xq, scales=sx, rotate=lin.rotate)
+    lin.encode(xq, sx, y, rows)
+    ref = qref.add_rmsnorm((x + r).numpy(), g.numpy(), 1e-6)[0] @ deq(host, 4).astype(np.float64).T
+    err = y.double().cpu().numpy() - ref
+    rms = np.sqrt((ref ** 2).mean())
+    assert np.sqrt((err ** 2).mean()) <= 0.02 * rms and np.abs(err).max() <= 0.1 * rms
+    # and exactly, from the codes
+    want = reference(xq.cpu(), sx.cpu(), lin.w.cpu(), lin.scales.cpu())
+    assert torch.equal(y.cpu(), want)

@@ -1,0 +1,57 @@
+"""What the W8A8 linear on packed rows refuses, in Python and at the C entry, without a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+from ingot_b200 import capi
+from ingot_b200.linear import I8Linear
+
+W, S = torch.zeros(8, 64, dtype=torch.int8), torch.ones(8)
+
+
+@pytest.mark.parametrize("w,s,rotate,error", [
+    (W.float(), S, 0, TypeError), (W, S.half(), 0, TypeError), (W, S[:7], 0, ValueError), (W.t().contiguous().t(), S, 0, ValueError), (W[:, :24].contiguous(), S, 0, ValueError),
+    (torch.zeros(1, 131072, dtype=torch.int8), S[:1], 0, ValueError), (W, S, 64, ValueError), (W, S, 256, ValueError), (W[0], S, 0, TypeError), (W, S, 32, ValueError)])
+def test_weights(w, s, rotate, error):
+    with pytest.raises(error):  # (the last: nothing wrong but the device)
+        I8Linear(w, s, rotate)
+
+
+@pytest.mark.parametrize("change,error", [
+    ({"x": torch.zeros(4, 64)}, TypeError), ({"sx": torch.zeros(4, dtype=torch.float16)}, TypeError), ({"y": torch.zeros(4, 8, dtype=torch.int32)}, TypeError), ({"rows": 5}, ValueError),
+    ({"rows": -1}, ValueError), ({"x": torch.zeros(4, 48, dtype=torch.int8)}, ValueError), ({"y": torch.zeros(4, 7)}, ValueError), ({"y": torch.zeros(8, 4).t()}, ValueError),
+    ({"x": torch.zeros(4, 72, dtype=torch.int8)[:, :64]}, ValueError), ({"x": torch.zeros(4, 80, dtype=torch.int8)[:, 8:72]}, ValueError), ({"sx": torch.zeros(3)}, ValueError),
+    ({"sx": torch.zeros(8)[::2]}, ValueError), ({"x": torch.zeros(64, dtype=torch.int8)}, ValueError), ({}, ValueError)])
+def test_calls(change, error):
+    m = object.__new__(I8Linear)
+    m.w, m.scales, m.N, m.K, m.rotate = W, S, 8, 64, 0
+    a = {"x": torch.zeros(4, 64, dtype=torch.int8), "sx": torch.zeros(4), "y": torch.zeros(4, 8), "rows": 4}
+    a.update(change)
+    if change:
+        with pytest.raises(error):
+            m._check(a["x"], a["sx"], a["y"], a["rows"])
+    with pytest.raises((ValueError, TypeError)):
+        m.encode(a["x"], a["sx"], a["y"], a["rows"])
+
+
+P = 1 << 20  # an address that is never used: the checks come first
+
+
+@pytest.mark.parametrize("change,status", [
+    ({"x": 0}, -1), ({"sx": 0}, -1), ({"w": 0}, -1), ({"sw": 0}, -1), ({"y": 0}, -1), ({"yd": 3}, -1), ({"rows": -1}, -1), ({"n": 0}, -1), ({"k": 0}, -1), ({"k": 40}, -1),
+    ({"k": 131072, "ldx": 131072}, -2), ({"ldx": 48}, -1), ({"ldx": 72}, -1), ({"ldy": 7}, -1), ({"x": P + 8}, -1), ({"w": P + 4}, -1), ({"y": P + 2}, -1), ({"flags": 2}, -1), ({}, -1)])
+def test_c_entry(change, status):
+    a = {"x": P, "ldx": 64, "sx": P, "w": P, "sw": P, "n": 8, "k": 64, "y": P, "yd": 0, "ldy": 8, "rows": 4, "flags": 0}
+    a.update(change)
+    assert capi.lib().iq_qmm_i8(None, None, *a.values()) == status
+
+
+@pytest.mark.parametrize("change,rotate,status", [
+    ({"w": 0}, 0, -1), ({"biases": 0}, 0, -1), ({"bits": 8}, 0, -2), ({"mode": 1}, 0, -2), ({"experts": 2}, 0, -2), ({"group": 128}, 0, -2), ({"k": 96}, 0, -1), ({"k": 65536}, 0, -1),
+    ({"n": 0}, 0, -1), ({}, 64, -1), ({}, 256, -1), ({}, 32, -1)])
+def test_pack_entry(change, rotate, status):
+    a = {"w": P, "scales": P, "biases": P, "n": 8, "k": 128, "bits": 4, "group": 64, "mode": 0, "experts": 1}
+    a.update(change)
+    q = capi.QLinear(*a.values())
+    assert capi.lib().iq_i8_pack(None, None, C.byref(q), rotate, P, P) == status
