@@ -205,6 +205,14 @@ int32_t iq_qmm_w8a8(iq_ctx* ctx, void* stream, const void* x, int32_t x_dtype, i
  * y may not overlap the operands. */
 int32_t iq_qmm_i8(iq_ctx* ctx, void* stream, const int8_t* x, int64_t ldx, const float* x_scales, const int8_t* w, const float* w_scales,
                   int32_t n, int32_t k, void* y, int32_t y_dtype, int64_t ldy, int32_t rows, uint32_t flags);
+/* How iq_qmm_i8 divides a call among the SMs of a GPU. Needs no GPU and no context. For tests that have to know which path a shape takes. */
+typedef struct iq_qmm_i8_tiling {
+    int32_t tile_rows; /* tokens per tile */
+    int32_t pair;      /* 1: a tile of 256 features on two CTAs; 0: of 128 on a cluster */
+    int32_t parts;     /* CTAs of the cluster, which divide k */
+    int64_t tiles;
+} iq_qmm_i8_tiling;
+int32_t iq_qmm_i8_plan(int32_t rows, int32_t n, int32_t k, int32_t sms, iq_qmm_i8_tiling* out);
 /* A 4-bit affine matrix (group 64 or 32; k a multiple of 64, at most 49,152) as int8 rows [n, k] with a scale per row, rotated in blocks of `rotate`
  * inputs (0, 32 or 256, a divisor of k) as the activations will be; the scales take the transform's factor, so that codes of H x meet
  * codes of H w as they are. Done once, at load time. */

@@ -34,7 +34,7 @@ SYMBOLS = [
     "iq_ctx_set_wait_cycles", "iq_colsplit_create", "iq_colsplit_destroy", "iq_linear_colsplit_workspace_bytes",
     "iq_linear_colsplit", "iq_had_rows", "iq_embed_rows_ternary", "iq_qmm_w8a8_workspace_bytes", "iq_qmm_w8a8",
     "iq_qmm_plan", "iq_qmv_plan", "iq_ep_index", "iq_moe_experts_indexed", "iq_ep_pack_push_tokens", "iq_ep_index_tokens",
-    "iq_add_rmsnorm", "iq_i8_pack", "iq_qmm_i8",
+    "iq_add_rmsnorm", "iq_i8_pack", "iq_qmm_i8", "iq_qmm_i8_plan",
 ]
 
 
@@ -50,6 +50,10 @@ class QmmTiling(C.Structure):
 
 class QmvTiling(C.Structure):
     _fields_ = [("cluster", C.c_int32), ("tiles", C.c_int32), ("slices", C.c_int32)]
+
+
+class QmmI8Tiling(C.Structure):
+    _fields_ = [("tile_rows", C.c_int32), ("pair", C.c_int32), ("parts", C.c_int32), ("tiles", C.c_int64)]
 
 
 class MoeDesc(C.Structure):
@@ -194,7 +198,8 @@ def lib() -> C.CDLL:
                                      vp, i64, vp, i32]
         l.iq_i8_pack.argtypes = [vp, vp, C.POINTER(QLinear), i32, vp, vp]
         l.iq_qmm_i8.argtypes = [vp, vp, vp, i64, vp, vp, vp, i32, i32, vp, i32, i64, i32, u32]
-        for name in ("iq_add_rmsnorm", "iq_i8_pack", "iq_qmm_i8"):
+        l.iq_qmm_i8_plan.argtypes = [i32, i32, i32, i32, C.POINTER(QmmI8Tiling)]
+        for name in ("iq_add_rmsnorm", "iq_i8_pack", "iq_qmm_i8", "iq_qmm_i8_plan"):
             getattr(l, name).restype = i32
         for name in ("iq_ctx_create", "iq_qmv", "iq_qmm_workspace_bytes", "iq_qmm", "iq_dense_ffn_workspace_bytes",
                      "iq_dense_ffn", "iq_moe_create", "iq_moe_workspace_bytes", "iq_moe_forward", "iq_moe_route",
@@ -280,6 +285,15 @@ def qmv_plan(n: int, k: int, bits: int, group: int, rows: int, mode: int = IQ_MO
     """How a decode call of five rows and more is divided where the kernel of clusters takes it (iq_qmv_plan); needs no GPU."""
     out = QmvTiling()
     st = lib().iq_qmv_plan(C.byref(QLinear(0, 0, 0, n, k, bits, group, mode, 1)), rows, sms, (C.c_int32 * 3)(*at_once), C.byref(out))
+    if st != 0:
+        raise IngotError(st, lib().iq_strerror(st).decode())
+    return out
+
+
+def qmm_i8_plan(rows: int, n: int, k: int, sms: int = 148) -> QmmI8Tiling:
+    """How a W8A8 call on packed rows is divided (iq_qmm_i8_plan); needs no GPU."""
+    out = QmmI8Tiling()
+    st = lib().iq_qmm_i8_plan(rows, n, k, sms, C.byref(out))
     if st != 0:
         raise IngotError(st, lib().iq_strerror(st).decode())
     return out

@@ -5,6 +5,7 @@
 #include <string.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "internal.h"
 #include "ptx.cuh"
@@ -30,19 +31,19 @@ struct I8Params {
     const float* sw;
     void* y;
     int64_t ldy;
-    int32_t y_dtype, accumulate;
+    int32_t y_dtype, accumulate, whole;  // whole: four neighbouring elements of y lie on their own size
     int32_t M, N, K;
-    int32_t m_tiles, steps;  // tiles of BN tokens; steps of 128 inputs
+    int32_t m_tiles, steps;  // tiles of tokens; steps of 128 inputs
+    int32_t tile_rows;       // pairs: tokens of a tile
     int32_t* status;
 };
 
 template <int BN>
 struct I8Tile {
     static constexpr int STAGE = 128 * 128 + BN * 128;
-    static constexpr int PER_SM = BN <= 64 ? 2 : 1;
-    static constexpr int FIT = (BN <= 64 ? 110 : 220) * 1024 / STAGE;
-    static constexpr int STAGES = FIT > 8 ? 8 : FIT;
+    static constexpr int STAGES = 4;  // (two or three CTAs per SM; with three stages the next call starts earlier but 37 rows take 5 to 15 % longer)
     static constexpr int SMEM = STAGES * STAGE + 1024 + 256;  // alignment, barriers
+    static constexpr int PER_SM = 227 * 1024 / (SMEM + 1024);
     static constexpr uint32_t COLS = BN < 32 ? 32 : BN;
     static_assert(BN * 512 <= STAGES * STAGE, "the partial sums take the stages' place");
 };
@@ -63,6 +64,72 @@ __device__ __forceinline__ int4 ld_dsmem_s4(uint32_t local, uint32_t cta) {
                  : "r"(local), "r"(cta)
                  : "memory");
     return v;
+}
+
+// C neighbouring tokens of one feature: scaled, added, rounded and stored. sx: the scale of token `lane`; live: how many there are.
+template <int DT, int C>
+__device__ __forceinline__ void i8_store(const I8Params& p, const uint32_t (&r)[C], float sx, float sw, int row, int n, int live) {
+    typedef typename std::conditional<DT == kF32, float, uint16_t>::type E;
+    E* const y = static_cast<E*>(p.y) + (size_t)row * p.ldy + n;
+    float v[C];
+#pragma unroll
+    for (int j = 0; j < C; j++) v[j] = __fmul_rn(__fmul_rn((float)(int)r[j], __shfl_sync(0xffffffffu, sx, j)), sw);
+    if (n >= p.N) live = 0;
+    if (p.accumulate) {  // all loads before the first store
+#pragma unroll
+        for (int j = 0; j < C; j++)
+            if (j < live) v[j] += y_load(y, DT, (size_t)j * p.ldy);
+    }
+    if (live >= C) {
+#pragma unroll
+        for (int j = 0; j < C; j++) y_store(y, DT, (size_t)j * p.ldy, v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < C; j++)
+            if (j < live) y_store(y, DT, (size_t)j * p.ldy, v[j]);
+    }
+}
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
+__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+                   "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr)
+                 : "memory");
+}
+// The lanes' features and C tokens of an accumulator to y
+template <int C>
+__device__ __forceinline__ void i8_results(const I8Params& p, uint32_t taddr, float sx, float sw, int row, int n, int live) {
+    uint32_t r[C];
+    tmem_ld(taddr, r);
+    tmem_ld_wait();
+    if (p.y_dtype == kF32) i8_store<kF32, C>(p, r, sx, sw, row, n, live);
+    else if (p.y_dtype == kBF16) i8_store<kBF16, C>(p, r, sx, sw, row, n, live);
+    else i8_store<kF16, C>(p, r, sx, sw, row, n, live);
+}
+// Sums of a token and four neighbouring features, the first of them n
+template <int DT>
+__device__ __forceinline__ void i8_store4(const I8Params& p, const int4& s, float sx, const float (&sw)[4], int row, int n) {
+    typedef typename std::conditional<DT == kF32, float, uint16_t>::type E;
+    E* const y = static_cast<E*>(p.y) + (size_t)row * p.ldy + n;
+    const int k[4] = {s.x, s.y, s.z, s.w}, live = p.N - n;
+    float f[4];
+#pragma unroll
+    for (int j = 0; j < 4; j++) f[j] = __fmul_rn(__fmul_rn((float)k[j], sx), sw[j]);
+    if (p.accumulate) {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (j < live) f[j] += y_load(y, DT, j);
+    }
+    if (live >= 4 && p.whole) {
+        if (DT == kF32) *reinterpret_cast<float4*>(y) = make_float4(f[0], f[1], f[2], f[3]);
+        else if (DT == kF16) *reinterpret_cast<uint2*>(y) = make_uint2(pack_half2(f[0], f[1]), pack_half2(f[2], f[3]));
+        else *reinterpret_cast<uint2*>(y) = make_uint2(f32_to_bf16_bits(f[0]) | f32_to_bf16_bits(f[1]) << 16, f32_to_bf16_bits(f[2]) | f32_to_bf16_bits(f[3]) << 16);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (j < live) y_store(y, DT, j, f[j]);
+    }
 }
 
 // A tile per cluster; its CTAs divide the steps among them and add their sums through distributed shared memory.
@@ -144,31 +211,21 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
         pdl_wait();
         const int q = warp & 3;  // the quarter of tensor memory that this warp may read
         const uint32_t t0 = tmem + ((uint32_t)(32 * q) << 16);
+        constexpr int C = BN < 32 ? BN : 32;
+        const int n = n0 + 32 * q + lane;
+        const float sw = n < p.N ? p.sw[n] : 0.f, sx0 = lane < rows ? p.sx[row0 + lane] : 0.f, sx1 = 32 + lane < rows ? p.sx[row0 + 32 + lane] : 0.f;
         if (__all_sync(0xffffffffu, mbar_wait(sums, 0, abort_flag))) {
             tc_fence_after();
-            const int n = n0 + 32 * q + lane;
-            const float sw = n < p.N ? p.sw[n] : 0.f;
             int* const park = reinterpret_cast<int*>(smem);  // [token][128 features]
-            for (int c0 = 0; c0 < rows; c0 += 16) {
-                uint32_t r[16];
-                asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                             : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
-                               "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                             : "r"(t0 + c0)
-                             : "memory");
-                tmem_ld_wait();
-                if (parts > 1) {
+            for (int c0 = 0; c0 < rows; c0 += C) {
+                if (parts == 1) {
+                    i8_results<C>(p, t0 + c0, __shfl_sync(0xffffffffu, c0 < 32 ? sx0 : sx1, (lane + c0) & 31), sw, row0 + c0, n, rows - c0);
+                } else {
+                    uint32_t r[C];
+                    tmem_ld(t0 + c0, r);
+                    tmem_ld_wait();
 #pragma unroll
-                    for (int j = 0; j < 16; j++) park[(c0 + j) * 128 + 32 * q + lane] = (int)r[j];
-                } else if (n < p.N) {
-#pragma unroll
-                    for (int j = 0; j < 16; j++)
-                        if (c0 + j < rows) {
-                            const size_t o = (size_t)(row0 + c0 + j) * p.ldy + n;
-                            float v = __fmul_rn(__fmul_rn((float)(int)r[j], p.sx[row0 + c0 + j]), sw);
-                            if (p.accumulate) v += y_load(p.y, p.y_dtype, o);
-                            y_store(p.y, p.y_dtype, o, v);
-                        }
+                    for (int j = 0; j < C; j++) park[(c0 + j) * 128 + 32 * q + lane] = (int)r[j];
                 }
             }
         }
@@ -183,25 +240,25 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
     if (parts > 1) {
         cluster_sync_all();  // every CTA's sums lie in its shared memory
         if (warp >= 2 && !*abort_flag) {
-            // this CTA's share of the tile, four features at a time
+            // this CTA's share of the tile, four features at a time; all loads before the first sum
             const int units = rows * 32, u0 = units * part / parts, u1 = units * (part + 1) / parts;
             for (int u = u0 + (int)threadIdx.x - 64; u < u1; u += 128) {
-                int4 v = make_int4(0, 0, 0, 0);
-                for (int c = 0; c < parts; c++) {
-                    const int4 o = ld_dsmem_s4(smem_u32(smem) + u * 16, c);
-                    v.x += o.x; v.y += o.y; v.z += o.z; v.w += o.w;
-                }
                 const int t = row0 + u / 32, n = n0 + u % 32 * 4;
-                const float sx = p.sx[t];
-                const int k[4] = {v.x, v.y, v.z, v.w};
-                const size_t o = (size_t)t * p.ldy + n;
+                int4 o[8];
 #pragma unroll
-                for (int j = 0; j < 4; j++)
-                    if (n + j < p.N) {
-                        float f = __fmul_rn(__fmul_rn((float)k[j], sx), p.sw[n + j]);
-                        if (p.accumulate) f += y_load(p.y, p.y_dtype, o + j);
-                        y_store(p.y, p.y_dtype, o + j, f);
-                    }
+                for (int c = 0; c < 8; c++)
+                    if (c < parts) o[c] = ld_dsmem_s4(smem_u32(smem) + u * 16, c);
+                const float sx = p.sx[t];
+                float sw[4];
+#pragma unroll
+                for (int j = 0; j < 4; j++) sw[j] = n + j < p.N ? p.sw[n + j] : 0.f;
+                int4 v = make_int4(0, 0, 0, 0);
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+                    if (c < parts) { v.x += o[c].x; v.y += o[c].y; v.z += o[c].z; v.w += o[c].w; }
+                if (p.y_dtype == kF32) i8_store4<kF32>(p, v, sx, sw, t, n);
+                else if (p.y_dtype == kBF16) i8_store4<kBF16>(p, v, sx, sw, t, n);
+                else i8_store4<kF16>(p, v, sx, sw, t, n);
             }
         }
         cluster_sync_all();  // nobody reads this CTA's shared memory any more
@@ -213,15 +270,191 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
     }
 }
 
-typedef void (*I8Kernel)(CUtensorMap, CUtensorMap, I8Params);
+// ---- many rows: tiles of 256 features and up to 256 tokens on pairs of CTAs -----------------------------------------------
+constexpr int kI8PairThreads = 320;  // copies, MMAs, eight warps for the results
+constexpr int kI8PairStage = 2 * 128 * 128;  // of a CTA: its 128 features and its half of the tokens
+constexpr int kI8PairStages = 6;
+constexpr int kI8PairSmem = kI8PairStages * kI8PairStage + 1024 + 256;
+
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n}\n"
+        ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+        : "memory");
+}
+// Tensor copy into this CTA's shared memory whose bytes count on the barrier at this offset of the pair's even CTA
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+    asm volatile(
+        "{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %2, 0;\n"
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [r];\n}\n"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1)
+        : "memory");
+}
+
+// Persistent; two accumulators in tensor memory, so that a tile's results leave beside the next tile's products. The even CTA issues the
+// MMAs for both; each copies its 128 features and its half of the tokens and stores its 128 features' results.
+__global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
+    i8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const I8Params p) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kI8PairStages * kI8PairStage);  // full, empty; accumulators full [2], empty [2]
+    const uint32_t full = smem_u32(bars), empty = full + 8 * kI8PairStages, tfull = empty + 8 * kI8PairStages, tempty = tfull + 16;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kI8PairStages + 4);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kI8PairStages; s++) {
+            mbar_init(full + 8 * s, 1);
+            mbar_init(empty + 8 * s, 1);
+        }
+        for (int a = 0; a < 2; a++) {
+            mbar_init(tfull + 8 * a, 1);
+            mbar_init(tempty + 8 * a, 16);  // both CTAs' eight warps
+        }
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // the other CTA's barriers exist
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();
+    pdl_wait();
+    const int total = p.m_tiles * ((p.N + 255) / 256), first = blockIdx.x / 2, stride = gridDim.x / 2;
+    const uint32_t bytes = 128 * 128 + p.tile_rows * 64;  // of a CTA and stage
+    // tokens of a tile's MMAs: whole groups of 32, half of them in each CTA
+    auto tokens = [&](int row0) { return (min(p.tile_rows, p.M - row0) + 31) & ~31; };
+    if (warp == 0) {
+        if (elect_one()) {
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int i = first; i < total && ok; i += stride) {
+                const int row0 = (i % p.m_tiles) * p.tile_rows, n0 = (i / p.m_tiles) * 256 + 128 * (int)rank;
+                const int xrow = row0 + (int)rank * (tokens(row0) / 2);
+                for (int ks = 0; ks < p.steps; ks++) {
+                    if (!(ok = mbar_wait(empty + 8 * s, ph ^ 1, abort_flag))) break;
+                    const uint32_t st = smem_u32(smem + s * kI8PairStage);
+                    if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, 2 * bytes);
+                    tma_load_2d_pair(st, &map_w, full + 8 * s, ks * 128, n0);
+                    tma_load_2d_pair(st + 128 * 128, &map_x, full + 8 * s, ks * 128, xrow);
+                    if (++s == kI8PairStages) { s = 0; ph ^= 1; }
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (rank == 0 && elect_one()) {
+            int s = 0, a = 0;
+            uint32_t ph = 0, tph = 0;
+            bool ok = true;
+            for (int i = first; i < total && ok; i += stride) {
+                const uint32_t idesc = i8_idesc(tokens((i % p.m_tiles) * p.tile_rows)) + (8u << 24);  // M = 256
+                if (!(ok = mbar_wait(tempty + 8 * a, tph ^ 1, abort_flag))) break;
+                tc_fence_after();
+                const uint32_t acc = tmem + a * 256;
+                for (int ks = 0; ks < p.steps; ks++) {
+                    if (!(ok = mbar_wait(full + 8 * s, ph, abort_flag))) break;
+                    tc_fence_after();
+                    const uint32_t st = smem_u32(smem + s * kI8PairStage);
+                    const uint64_t ad = i8_desc(st), bd = i8_desc(st + 128 * 128);
+#pragma unroll
+                    for (int kk = 0; kk < 4; kk++) umma_i8_pair(acc, ad + 2 * kk, bd + 2 * kk, idesc, (ks | kk) != 0 ? 1u : 0u);
+                    umma_commit_pair(empty + 8 * s);
+                    if (++s == kI8PairStages) { s = 0; ph ^= 1; }
+                }
+                if (ok) umma_commit_pair(tfull + 8 * a);
+                a ^= 1;
+                if (a == 0) tph ^= 1;
+            }
+        }
+    } else {
+        const int q = warp & 3, half = (warp - 2) >> 2;
+        int a = 0;
+        uint32_t tph = 0;
+        for (int i = first; i < total; i += stride) {
+            const int row0 = (i % p.m_tiles) * p.tile_rows, rows = min(p.tile_rows, p.M - row0), n = (i / p.m_tiles) * 256 + 128 * (int)rank + 32 * q + lane;
+            const float sw = n < p.N ? p.sw[n] : 0.f;
+            if (!__all_sync(0xffffffffu, mbar_wait(tfull + 8 * a, tph, abort_flag))) break;
+            tc_fence_after();
+            const uint32_t t0 = tmem + ((uint32_t)(32 * q) << 16) + a * 256;
+            for (int c0 = 32 * half; c0 < rows; c0 += 64) {
+                const int live = rows - c0;
+                const float sx = lane < live ? p.sx[row0 + c0 + lane] : 0.f;
+                i8_results<32>(p, t0 + c0, sx, sw, row0 + c0, n, live);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) {
+                if (rank != 0) mbar_arrive_remote(tempty + 8 * a, 0);
+                else mbar_arrive(tempty + 8 * a);
+            }
+            a ^= 1;
+            if (a == 0) tph ^= 1;
+        }
+    }
+    __syncwarp();
+    if (*abort_flag && warp == 0) {  // copies in flight land before the shared memory is given back
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000) {}
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // (the other CTA's MMAs read this one's memory, its arrivals go to this one's barriers)
+    if (*abort_flag && threadIdx.x == 0 && p.status != nullptr) atomicExch(p.status, kErrTimeout);
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
 struct I8Entry {
     int bn;
     void (*fn)(const CUtensorMap, const CUtensorMap, const I8Params);
-    int smem, per_sm;
+    int smem;
 };
 template <int BN>
-constexpr I8Entry i8_entry() { return I8Entry{BN, i8_cluster_kernel<BN>, I8Tile<BN>::SMEM, I8Tile<BN>::PER_SM}; }
-const I8Entry kI8[] = {i8_entry<16>(), i8_entry<32>(), i8_entry<64>(), i8_entry<128>(), i8_entry<256>()};
+constexpr I8Entry i8_entry() { return I8Entry{BN, i8_cluster_kernel<BN>, I8Tile<BN>::SMEM}; }
+const I8Entry kI8[] = {i8_entry<16>(), i8_entry<32>(), i8_entry<64>()};
+
+// How a call is divided. Up to 128 rows clusters, which hide the weights' way from memory; beyond the cheaper of the two by estimates in ns: a
+// step of a pair on h tokens takes 200 + 0.72 h, of a cluster's CTA on 64 tokens (two per SM) 330, the start and the last tile's results 4000 +
+// 8 h and 5000. Measured / estimated, us: 256 x 4096 x 4096 clusters 12.3 / 10.3, pairs 12.5 / 12.4; 256 x 14336 x 4096 27.7 / 26.1, 22.1 / 18.3; 256 x 4096 x
+// 14336 25.1 / 23.5, 30.7 / 32.1; 512 x 4096 x 4096 clusters 15.6 (estimated), pairs 14.4 / 14.3.
+struct I8Plan {
+    bool pair;
+    int rows;  // tokens of a tile
+    int64_t tiles;
+    int parts;  // pieces of k, the CTAs of a cluster
+};
+I8Plan i8_plan(int rows, int n, int k, int sms) {
+    const int64_t steps = (k + 127) / 128;
+    I8Plan c;
+    c.pair = false;
+    c.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
+    c.tiles = (int64_t)((rows + c.rows - 1) / c.rows) * ((n + 127) / 128);
+    c.parts = 1;
+    // (a division costs about 1 us: 37 x 1024 x 1024, eight steps, 4.2 us whole and 4.8 in four; 23 steps of 37 x 2880 x 2880 8.4 and 6.4)
+    while (steps > 8 && c.parts < 8 && c.tiles * c.parts <= sms && steps >= 4 * c.parts) c.parts *= 2;
+    if (rows <= 128 || sms % 2 != 0) return c;
+    int64_t least = (c.tiles * c.parts + 2 * sms - 1) / (2 * sms) * (steps / c.parts) * 330 + 5000;
+    for (int h = 256; h >= 64; h -= 32) {
+        const int64_t tiles = (int64_t)((rows + h - 1) / h) * ((n + 255) / 256);
+        const int64_t cost = (tiles + sms / 2 - 1) / (sms / 2) * steps * (20000 + 72 * h) / 100 + 4000 + 8 * h;
+        if (cost < least) {
+            least = cost;
+            c = I8Plan{true, h, tiles, 1};
+        }
+    }
+    return c;
+}
 
 }  // namespace
 
@@ -230,12 +463,23 @@ int32_t i8_init(iq_ctx* ctx) {
         const cudaError_t r = cudaFuncSetAttribute(reinterpret_cast<const void*>(e.fn), cudaFuncAttributeMaxDynamicSharedMemorySize, e.smem);
         if (r != cudaSuccess) return check_cuda(ctx, r, "cudaFuncSetAttribute(i8)");
     }
-    return kOk;
+    const cudaError_t r = cudaFuncSetAttribute(reinterpret_cast<const void*>(i8_pair_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kI8PairSmem);
+    return check_cuda(ctx, r, "cudaFuncSetAttribute(i8_pair)");
 }
 
 }  // namespace iq
 
 using namespace iq;
+
+extern "C" int32_t iq_qmm_i8_plan(int32_t rows, int32_t n, int32_t k, int32_t sms, iq_qmm_i8_tiling* out) {
+    if (out == nullptr || rows < 1 || n < 1 || k < 16 || k % 16 != 0 || k > kI8MaxK || sms < 1) return kErrInvalidArg;
+    const I8Plan p = i8_plan(rows, n, k, sms);
+    out->tile_rows = p.rows;
+    out->pair = p.pair ? 1 : 0;
+    out->parts = p.parts;
+    out->tiles = p.tiles;
+    return kOk;
+}
 
 extern "C" int32_t iq_qmm_i8(iq_ctx* ctx, void* stream, const int8_t* x, int64_t ldx, const float* x_scales, const int8_t* w, const float* w_scales,
                              int32_t n, int32_t k, void* y, int32_t y_dtype, int64_t ldy, int32_t rows, uint32_t flags) {
@@ -250,33 +494,38 @@ extern "C" int32_t iq_qmm_i8(iq_ctx* ctx, void* stream, const int8_t* x, int64_t
     if ((flags & ~(uint32_t)IQ_FLAG_ACCUMULATE) != 0) return fail(ctx, kErrInvalidArg, "qmm_i8: flags %u", flags);
     if (ctx == nullptr) return kErrInvalidArg;
     if (rows == 0) return kOk;
-    const I8Entry* e = kI8;
-    while (e->bn < rows && e->bn < 256) e++;
+    const I8Plan plan = i8_plan(rows, n, k, ctx->sms);
+    if (plan.tiles * plan.parts > (1 << 30)) return fail(ctx, kErrUnsupported, "qmm_i8: %lld tiles", (long long)plan.tiles);
     I8Params p;
-    p.sx = x_scales; p.sw = w_scales; p.y = y; p.ldy = ldy; p.y_dtype = y_dtype; p.accumulate = flags & IQ_FLAG_ACCUMULATE ? 1 : 0;
+    p.sx = x_scales; p.sw = w_scales; p.y = y; p.ldy = ldy; p.y_dtype = y_dtype;
+    p.accumulate = flags & IQ_FLAG_ACCUMULATE ? 1 : 0;
+    p.whole = ldy % 4 == 0 && reinterpret_cast<uintptr_t>(y) % (4 * dtype_size(y_dtype)) == 0;
     p.M = rows; p.N = n; p.K = k;
-    p.m_tiles = (rows + e->bn - 1) / e->bn; p.steps = (k + 127) / 128; p.status = ctx->d_status;
-    const int64_t tiles = (int64_t)p.m_tiles * ((n + 127) / 128);
-    if (tiles > (1 << 27)) return fail(ctx, kErrUnsupported, "qmm_i8: %lld tiles", (long long)tiles);
-    int parts = 1;
-    while (parts < 8 && tiles * parts * 2 <= (int64_t)ctx->sms * e->per_sm && p.steps >= 4 * parts) parts *= 2;
+    p.tile_rows = plan.rows; p.m_tiles = (rows + plan.rows - 1) / plan.rows; p.steps = (k + 127) / 128;
+    p.status = ctx->d_status;
     DeviceScope on(ctx);
     if (on.error != cudaSuccess) return check_cuda(ctx, on.error, "qmm_i8 device");
     CUtensorMap mx, mw;
-    int32_t st = make_map_2d(ctx, &mx, x, 0, (uint64_t)k, (uint64_t)rows, (uint64_t)ldx, 128, (uint32_t)e->bn, true);
+    int32_t st = make_map_2d(ctx, &mx, x, 0, (uint64_t)k, (uint64_t)rows, (uint64_t)ldx, 128, (uint32_t)(plan.pair ? plan.rows / 2 : plan.rows), true);
     if (st == kOk) st = cached_rows_map(ctx, w, n, k, 128, &mw);
     if (st != kOk) return st;
+    cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
+    if (plan.pair)
+        return check_cuda(ctx, launch_dependent(i8_pair_kernel, dim3((unsigned)std::min<int64_t>(plan.tiles, ctx->sms / 2) * 2), kI8PairThreads, kI8PairSmem, cs, mx, mw, p),
+                          "qmm_i8 launch");
+    const I8Entry* e = kI8;
+    while (e->bn != plan.rows) e++;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
-    cfg.gridDim = dim3((unsigned)(tiles * parts), 1, 1);
+    cfg.gridDim = dim3((unsigned)(plan.tiles * plan.parts), 1, 1);
     cfg.blockDim = dim3(kI8Threads, 1, 1);
     cfg.dynamicSmemBytes = e->smem;
-    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cfg.stream = cs;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = parts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
+    attr[1].val.clusterDim.x = plan.parts; attr[1].val.clusterDim.y = 1; attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
     return check_cuda(ctx, cudaLaunchKernelEx(&cfg, e->fn, mx, mw, p), "qmm_i8 launch");

@@ -67,6 +67,16 @@ def test_many_tiles(cuda_device, rows, n, k):
     run(torch.Generator().manual_seed(rows), rows, n, k, BF16)
 
 
+@pytest.mark.parametrize("rows,n,k,height", [(221, 1280, 256, 64), (1174, 1280, 1040, 96), (680, 9472, 256, 128), (1954, 2560, 384, 160), (1971, 4730, 1040, 192),
+                                                (2160, 9472, 384, 224), (246, 18944, 1040, 256)])
+@pytest.mark.parametrize("dtype,accumulate", [(F32, True), (F16, False)])
+def test_pairs(cuda_device, rows, n, k, height, dtype, accumulate):
+    """Pairs of CTAs on tiles of every height, the last of them short, more than one tile per pair."""
+    plan = capi.qmm_i8_plan(rows, n, k)
+    assert plan.pair == 1 and plan.tile_rows == height
+    run(torch.Generator().manual_seed(rows), rows, n, k, dtype, accumulate, 1)
+
+
 def test_the_largest_sums(cuda_device):
     """Every code -128 at the most inputs: 131,056 * 2^14 is below 2^31."""
     k = I8Linear.MAX_K
