@@ -327,20 +327,33 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_launch_dependents();
-    pdl_wait();
     const int total = p.m_tiles * ((p.N + 255) / 256), first = blockIdx.x / 2, stride = gridDim.x / 2;
     const uint32_t bytes = 128 * 128 + p.tile_rows * 64;  // of a CTA and stage
     // tokens of a tile's MMAs: whole groups of 32, half of them in each CTA
     auto tokens = [&](int row0) { return (min(p.tile_rows, p.M - row0) + 31) & ~31; };
     if (warp == 0) {
         if (elect_one()) {
-            int s = 0;
-            uint32_t ph = 0;
+            auto corner = [&](int i, int& xrow, int& n0) {
+                const int row0 = (i % p.m_tiles) * p.tile_rows;
+                n0 = (i / p.m_tiles) * 256 + 128 * (int)rank;
+                xrow = row0 + (int)rank * (tokens(row0) / 2);
+            };
+            // the first stages' weights ahead of the wait for the kernel before
+            int xrow, n0;
+            corner(first, xrow, n0);
+            const int ahead = min(kI8PairStages, p.steps);
+            for (int s = 0; s < ahead; s++) {
+                if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, 2 * bytes);
+                tma_load_2d_pair(smem_u32(smem + s * kI8PairStage), &map_w, full + 8 * s, s * 128, n0);
+            }
+            pdl_wait();
+            for (int s = 0; s < ahead; s++) tma_load_2d_pair(smem_u32(smem + s * kI8PairStage) + 128 * 128, &map_x, full + 8 * s, s * 128, xrow);
+            int s = ahead % kI8PairStages;
+            uint32_t ph = ahead / kI8PairStages;
             bool ok = true;
-            for (int i = first; i < total && ok; i += stride) {
-                const int row0 = (i % p.m_tiles) * p.tile_rows, n0 = (i / p.m_tiles) * 256 + 128 * (int)rank;
-                const int xrow = row0 + (int)rank * (tokens(row0) / 2);
-                for (int ks = 0; ks < p.steps; ks++) {
+            for (int i = first, ks = ahead; i < total && ok; i += stride, ks = 0) {
+                corner(i, xrow, n0);
+                for (; ks < p.steps; ks++) {
                     if (!(ok = mbar_wait(empty + 8 * s, ph ^ 1, abort_flag))) break;
                     const uint32_t st = smem_u32(smem + s * kI8PairStage);
                     if (rank == 0) mbar_arrive_expect_tx(full + 8 * s, 2 * bytes);
@@ -376,19 +389,34 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
             }
         }
     } else {
+        pdl_wait();
         const int q = warp & 3, half = (warp - 2) >> 2;
         int a = 0;
         uint32_t tph = 0;
         for (int i = first; i < total; i += stride) {
             const int row0 = (i % p.m_tiles) * p.tile_rows, rows = min(p.tile_rows, p.M - row0), n = (i / p.m_tiles) * 256 + 128 * (int)rank + 32 * q + lane;
             const float sw = n < p.N ? p.sw[n] : 0.f;
+            float sx[4];  // of the warp's (up to) four times 32 tokens
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int t = 64 * c + 32 * half + lane;
+                sx[c] = t < rows ? p.sx[row0 + t] : 0.f;
+            }
             if (!__all_sync(0xffffffffu, mbar_wait(tfull + 8 * a, tph, abort_flag))) break;
             tc_fence_after();
-            const uint32_t t0 = tmem + ((uint32_t)(32 * q) << 16) + a * 256;
-            for (int c0 = 32 * half; c0 < rows; c0 += 64) {
-                const int live = rows - c0;
-                const float sx = lane < live ? p.sx[row0 + c0 + lane] : 0.f;
-                i8_results<32>(p, t0 + c0, sx, sw, row0 + c0, n, live);
+            const uint32_t t0 = tmem + ((uint32_t)(32 * q) << 16) + a * 256 + 32 * half;
+            uint32_t r[2][32];  // the next columns are under way while these are stored
+            if (32 * half < rows) tmem_ld(t0, r[0]);
+#pragma unroll
+            for (int c = 0; c < 4; c++) {
+                const int c0 = 64 * c + 32 * half;
+                if (c0 < rows) {
+                    tmem_ld_wait();
+                    if (c < 3 && c0 + 64 < rows) tmem_ld(t0 + 64 * (c + 1), r[(c + 1) & 1]);
+                    if (p.y_dtype == kF32) i8_store<kF32, 32>(p, r[c & 1], sx[c], sw, row0 + c0, n, rows - c0);
+                    else if (p.y_dtype == kBF16) i8_store<kBF16, 32>(p, r[c & 1], sx[c], sw, row0 + c0, n, rows - c0);
+                    else i8_store<kF16, 32>(p, r[c & 1], sx[c], sw, row0 + c0, n, rows - c0);
+                }
             }
             tc_fence_before();
             __syncwarp();
