@@ -470,6 +470,41 @@ int32_t iq_topk64(iq_ctx* ctx, void* stream, const float* x, int64_t ldx, int32_
                   const float* temperatures, int32_t n_temperatures, uint32_t* idx, float* val, float* z, void* scratch,
                   size_t scratch_bytes);
 
+/* The sampler's rules on rows of logits, between the lm_head and iq_argmax_rows or iq_topk64. For token t of row r:
+ *   c = how often t stands in tokens[r, prompt_lens[r] .. lens[r]), seen = t stands in tokens[r, 0 .. lens[r])
+ *   l = seen ? (x > 0 ? x / repetition[r] : x * repetition[r]) : x
+ *   l = (l - frequency[r] * c) - (c > 0 ? presence[r] : 0)
+ *   l = l + bias_values[j] for every j in bias_offsets[r] .. bias_offsets[r + 1) with bias_tokens[j] == t, in their order
+ *   out = bit t of the row's mask is set, or the row has no mask ? l : -infinity
+ * each operation in fp32. All pointers are device arrays; a null one is a rule that nobody has: tokens (no history), prompt_lens (all of the history
+ * was generated), repetition (1), presence, frequency (0), bias_offsets (no biases), mask (everything allowed), mask_rows (row r has mask
+ * r). What they hold may change between calls and graph replays; lengths beyond max_tokens and offsets beyond biases are cut there, tokens outside
+ * the vocabulary are passed over, and an index in mask_rows that is none of the `masks` masks (-1) means no mask. A row of the mask is words of 32
+ * tokens, the lowest bit first. NaN logits stay NaN where they are allowed; a row whose mask allows nothing is -infinity throughout. Repetition is above 0.
+ * The reference samples from raw logits and has no counterpart. */
+typedef struct iq_logit_rules {
+    const int32_t* tokens;       /* [rows, ld_tokens] */
+    int64_t ld_tokens;
+    const int32_t* lens;         /* [rows], with tokens */
+    const int32_t* prompt_lens;  /* [rows] */
+    const float* repetition;     /* [rows] */
+    const float* presence;       /* [rows] */
+    const float* frequency;      /* [rows] */
+    const int32_t* bias_offsets; /* [rows + 1] */
+    const int32_t* bias_tokens;  /* [biases] */
+    const float* bias_values;    /* [biases] */
+    const uint32_t* mask;        /* [masks, ld_mask] */
+    int64_t ld_mask;
+    const int32_t* mask_rows;    /* [rows] */
+    int32_t max_tokens;
+    int32_t biases;
+    int32_t masks;
+} iq_logit_rules;
+/* x: [rows, ldx] of x_dtype; out: fp32 [rows, ldo], x itself where that is fp32 and ldo = ldx, else without overlap. Up to 262,144 logits per row; rows = 0
+ * does nothing. `rules` is read during the call. */
+int32_t iq_logits_rules(iq_ctx* ctx, void* stream, const void* x, int32_t x_dtype, int64_t ldx, float* out, int64_t ldo, int32_t rows, int32_t vocab,
+                        const iq_logit_rules* rules);
+
 /* ---- weight loader (host only; no GPU needed) -------------------------------------------------------------------------
  * One safetensors file mapped read-only with its header parsed into a tensor table: MappedFile + the per-shard part of
  * SafetensorsStore (Loader/Safetensors.swift:46-148). `data` points into the mapping (it may be unaligned) and stays

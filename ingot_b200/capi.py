@@ -34,7 +34,7 @@ SYMBOLS = [
     "iq_ctx_set_wait_cycles", "iq_colsplit_create", "iq_colsplit_destroy", "iq_linear_colsplit_workspace_bytes",
     "iq_linear_colsplit", "iq_had_rows", "iq_embed_rows_ternary", "iq_qmm_w8a8_workspace_bytes", "iq_qmm_w8a8",
     "iq_qmm_plan", "iq_qmv_plan", "iq_ep_index", "iq_moe_experts_indexed", "iq_ep_pack_push_tokens", "iq_ep_index_tokens",
-    "iq_add_rmsnorm", "iq_i8_pack", "iq_qmm_i8", "iq_qmm_i8_plan",
+    "iq_add_rmsnorm", "iq_i8_pack", "iq_qmm_i8", "iq_qmm_i8_plan", "iq_logits_rules",
 ]
 
 
@@ -54,6 +54,12 @@ class QmvTiling(C.Structure):
 
 class QmmI8Tiling(C.Structure):
     _fields_ = [("tile_rows", C.c_int32), ("pair", C.c_int32), ("parts", C.c_int32), ("tiles", C.c_int64)]
+
+
+class LogitRules(C.Structure):
+    _fields_ = [("tokens", C.c_void_p), ("ld_tokens", C.c_int64), ("lens", C.c_void_p), ("prompt_lens", C.c_void_p), ("repetition", C.c_void_p),
+                ("presence", C.c_void_p), ("frequency", C.c_void_p), ("bias_offsets", C.c_void_p), ("bias_tokens", C.c_void_p), ("bias_values", C.c_void_p),
+                ("mask", C.c_void_p), ("ld_mask", C.c_int64), ("mask_rows", C.c_void_p), ("max_tokens", C.c_int32), ("biases", C.c_int32), ("masks", C.c_int32)]
 
 
 class MoeDesc(C.Structure):
@@ -199,7 +205,8 @@ def lib() -> C.CDLL:
         l.iq_i8_pack.argtypes = [vp, vp, C.POINTER(QLinear), i32, vp, vp]
         l.iq_qmm_i8.argtypes = [vp, vp, vp, i64, vp, vp, vp, i32, i32, vp, i32, i64, i32, u32]
         l.iq_qmm_i8_plan.argtypes = [i32, i32, i32, i32, C.POINTER(QmmI8Tiling)]
-        for name in ("iq_add_rmsnorm", "iq_i8_pack", "iq_qmm_i8", "iq_qmm_i8_plan"):
+        l.iq_logits_rules.argtypes = [vp, vp, vp, i32, i64, vp, i64, i32, i32, C.POINTER(LogitRules)]
+        for name in ("iq_add_rmsnorm", "iq_i8_pack", "iq_qmm_i8", "iq_qmm_i8_plan", "iq_logits_rules"):
             getattr(l, name).restype = i32
         for name in ("iq_ctx_create", "iq_qmv", "iq_qmm_workspace_bytes", "iq_qmm", "iq_dense_ffn_workspace_bytes",
                      "iq_dense_ffn", "iq_moe_create", "iq_moe_workspace_bytes", "iq_moe_forward", "iq_moe_route",
@@ -224,7 +231,7 @@ def call():
         mod = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_iqcall", CALL_PATH, loader=loader))
         loader.exec_module(mod)
         for name in ("iq_qmv", "iq_qmm", "iq_dense_ffn", "iq_moe_forward", "iq_rmsnorm", "iq_had_rows", "iq_embed_rows",
-                     "iq_argmax_rows", "iq_topk64", "iq_add_rmsnorm", "iq_qmm_i8"):
+                     "iq_argmax_rows", "iq_topk64", "iq_add_rmsnorm", "iq_qmm_i8", "iq_logits_rules"):
             mod.bind(name, C.cast(getattr(l, name), C.c_void_p).value)
         _call = mod
     return _call

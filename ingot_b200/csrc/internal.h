@@ -204,6 +204,7 @@ int32_t launch_tern_qmv(iq_ctx* ctx, cudaStream_t st, const void* x, int32_t x_d
 int32_t w8a8_init(iq_ctx* ctx);
 int32_t norm_init(iq_ctx* ctx);
 int32_t i8_init(iq_ctx* ctx);
+int32_t rules_init(iq_ctx* ctx);
 int32_t gqmv_init(iq_ctx* ctx);
 int32_t qmm_init(iq_ctx* ctx);
 int32_t moe_init(iq_ctx* ctx);

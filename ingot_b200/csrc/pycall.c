@@ -20,12 +20,13 @@ static void* fn_argmax_rows;
 static void* fn_topk64;
 static void* fn_add_rmsnorm;
 static void* fn_qmm_i8;
+static void* fn_logits_rules;
 
 static const struct { const char* name; void** slot; } table[] = {
     {"iq_qmv", &fn_qmv},           {"iq_qmm", &fn_qmm},               {"iq_dense_ffn", &fn_dense_ffn},
     {"iq_moe_forward", &fn_moe_forward}, {"iq_rmsnorm", &fn_rmsnorm}, {"iq_had_rows", &fn_had_rows},
     {"iq_embed_rows", &fn_embed_rows},   {"iq_argmax_rows", &fn_argmax_rows}, {"iq_topk64", &fn_topk64},
-    {"iq_add_rmsnorm", &fn_add_rmsnorm}, {"iq_qmm_i8", &fn_qmm_i8},
+    {"iq_add_rmsnorm", &fn_add_rmsnorm}, {"iq_qmm_i8", &fn_qmm_i8}, {"iq_logits_rules", &fn_logits_rules},
 };
 
 static PyObject* py_bind(PyObject* self, PyObject* args) {
@@ -180,9 +181,18 @@ ENTRY(qmm_i8, 14, qmm_i8_t, {
     LAUNCH(f(c, s, x, ldx, sx, w, sw, nn, k, y, yd, ldy, rows, fl));
 })
 
+typedef int32_t (*rules_t)(iq_ctx*, void*, const void*, int32_t, int64_t, float*, int64_t, int32_t, int32_t, const iq_logit_rules*);
+ENTRY(logits_rules, 10, rules_t, {
+    void *c = P(0), *s = P(1), *x = P(2), *o = P(5), *r = P(9);
+    int32_t xd = I32(3), rows = I32(7), vocab = I32(8);
+    int64_t ldx = I64(4), ldo = I64(6);
+    CHECKED;
+    LAUNCH(f(c, s, x, xd, ldx, o, ldo, rows, vocab, r));
+})
+
 #define M(NAME) {#NAME, (PyCFunction)(void (*)(void))py_##NAME, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {
     {"bind", py_bind, METH_VARARGS, NULL}, M(qmv), M(qmm), M(dense_ffn), M(moe_forward), M(rmsnorm), M(had_rows), M(embed_rows),
-    M(argmax_rows), M(topk64), M(add_rmsnorm), M(qmm_i8), {NULL, NULL, 0, NULL}};
+    M(argmax_rows), M(topk64), M(add_rmsnorm), M(qmm_i8), M(logits_rules), {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_iqcall", NULL, -1, methods, NULL, NULL, NULL, NULL};
 PyMODINIT_FUNC PyInit__iqcall(void) { return PyModule_Create(&module); }

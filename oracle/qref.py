@@ -462,3 +462,35 @@ def hadamard(n: int) -> np.ndarray:
     while h.shape[0] < n:
         h = np.block([[h, h], [h, -h]])
     return h
+
+
+def logit_rules(x, dtype, tokens=None, lens=None, prompt_lens=None, repetition=None, presence=None, frequency=None, bias_offsets=None, bias_tokens=None, bias_values=None,
+                mask=None, mask_rows=None):
+    """Penalties, biases and masks on rows of logits (iq_logits_rules), every operation in `dtype`: float32 gives the kernel's bits, float64 the value."""
+    x = np.array(x, dtype=dtype, copy=True)
+    rows, V = x.shape
+    with np.errstate(invalid="ignore", over="ignore"):
+        for r in range(rows):
+            v = x[r]
+            if tokens is not None:
+                n = min(max(int(lens[r]), 0), tokens.shape[1])
+                p = 0 if prompt_lens is None else min(max(int(prompt_lens[r]), 0), n)
+                history = tokens[r, :n]
+                inside = lambda t: t[(t >= 0) & (t < V)]
+                said = np.bincount(inside(history[p:]), minlength=V)
+                seen = np.bincount(inside(history), minlength=V) > 0
+                rep, pres, freq = (dtype(d if a is None else a[r]) for a, d in ((repetition, 1), (presence, 0), (frequency, 0)))
+                v = np.where(seen, np.where(v > 0, v / rep, v * rep), v)
+                v = np.where(seen, v - freq * said.astype(dtype), v)
+                v = np.where(said > 0, v - pres, v)
+            if bias_offsets is not None:
+                for j in range(max(int(bias_offsets[r]), 0), min(int(bias_offsets[r + 1]), len(bias_tokens))):
+                    if 0 <= bias_tokens[j] < V:
+                        v[bias_tokens[j]] += dtype(bias_values[j])
+            if mask is not None:
+                m = r if mask_rows is None else int(mask_rows[r])
+                if 0 <= m < mask.shape[0]:
+                    t = np.arange(V)
+                    v = np.where((mask[m].view(np.uint32)[t >> 5] >> (t & 31).astype(np.uint32)) & 1, v, dtype(-np.inf))
+            x[r] = v
+    return x
