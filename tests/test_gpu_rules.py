@@ -73,7 +73,7 @@ def check(rng, rows, V, a, dtype=F32, pad=0, in_place=False, x=None):
     if "bias_values" in a and len(a["bias_values"]):
         size, ops = size + np.abs(a["bias_values"]).sum(), ops + len(a["bias_values"])
     fine = np.isfinite(ref)
-    assert np.array_equal(fine, np.isfinite(got)) and (np.abs(got - ref)[fine] <= ops * 2.0**-24 * size[fine]).all()
+    assert np.array_equal(fine, np.isfinite(got)) and (np.abs(got[fine] - ref[fine]) <= ops * 2.0**-24 * size[fine]).all()
 
 
 @pytest.mark.parametrize("V", [1, 2, 31, 33, 127, 1000, 1024, 1025, 4096, 32768, 50257, 128000, 262144])
