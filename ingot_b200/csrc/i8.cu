@@ -133,6 +133,12 @@ __device__ __forceinline__ void i8_store4(const I8Params& p, const int4& s, floa
 }
 
 // A tile per cluster; its CTAs divide the steps among them and add their sums through distributed shared memory.
+//
+// Bound: the weights' way from memory, and per call some 4 us of start (1 us from the kernel before to the first activations), sums of the cluster (2) and
+// end. Four stages per CTA of the next call are loaded meanwhile. One row: 14336 x 4096 12.9 us (floor 9.0), 28672 x 4096 19.2 (18.0), 128,000 x 2048
+// 40.7 (40.2). Asking for further weights into L2 ahead of the wait made it slower (12.9 -> 13.4 us with four more steps, 15.6 with all: the copies queue up
+// before the activations'), and so did L2 promotion by 256 bytes (no effect) and tiles of 128 and 256 tokens (64 rows 8.7 us, 128 on one tile 11.1 and
+// on two 9.2).
 template <int BN>
 __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
     i8_cluster_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const I8Params p) {
@@ -167,6 +173,15 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     pdl_launch_dependents();
+    // a divided tile: this CTA's share of it, in units of a token and four features, and the scales of a thread's unit (the first: ahead of the sums)
+    const int units = rows * 32, u0 = units * part / parts, u1 = units * (part + 1) / parts;
+    float unit_sx = 0.f, unit_sw[4];
+    auto unit_scales = [&](int u) {
+        const int n = n0 + u % 32 * 4;
+        unit_sx = p.sx[row0 + u / 32];
+#pragma unroll
+        for (int j = 0; j < 4; j++) unit_sw[j] = n + j < p.N ? p.sw[n + j] : 0.f;
+    };
     if (warp == 0) {
         // ---- copies: the first stages' weights ahead of the wait for the kernel before (nothing of this library's that runs beside its
         // successor writes weights)
@@ -212,6 +227,7 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
         const int q = warp & 3;  // the quarter of tensor memory that this warp may read
         const uint32_t t0 = tmem + ((uint32_t)(32 * q) << 16);
         constexpr int C = BN < 32 ? BN : 32;
+        if (parts > 1 && u0 + (int)threadIdx.x - 64 < u1) unit_scales(u0 + (int)threadIdx.x - 64);
         const int n = n0 + 32 * q + lane;
         const float sw = n < p.N ? p.sw[n] : 0.f, sx0 = lane < rows ? p.sx[row0 + lane] : 0.f, sx1 = 32 + lane < rows ? p.sx[row0 + 32 + lane] : 0.f;
         if (__all_sync(0xffffffffu, mbar_wait(sums, 0, abort_flag))) {
@@ -241,24 +257,20 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
         cluster_sync_all();  // every CTA's sums lie in its shared memory
         if (warp >= 2 && !*abort_flag) {
             // this CTA's share of the tile, four features at a time; all loads before the first sum
-            const int units = rows * 32, u0 = units * part / parts, u1 = units * (part + 1) / parts;
             for (int u = u0 + (int)threadIdx.x - 64; u < u1; u += 128) {
                 const int t = row0 + u / 32, n = n0 + u % 32 * 4;
+                if (u >= u0 + 128) unit_scales(u);
                 int4 o[8];
 #pragma unroll
                 for (int c = 0; c < 8; c++)
                     if (c < parts) o[c] = ld_dsmem_s4(smem_u32(smem) + u * 16, c);
-                const float sx = p.sx[t];
-                float sw[4];
-#pragma unroll
-                for (int j = 0; j < 4; j++) sw[j] = n + j < p.N ? p.sw[n + j] : 0.f;
                 int4 v = make_int4(0, 0, 0, 0);
 #pragma unroll
                 for (int c = 0; c < 8; c++)
                     if (c < parts) { v.x += o[c].x; v.y += o[c].y; v.z += o[c].z; v.w += o[c].w; }
-                if (p.y_dtype == kF32) i8_store4<kF32>(p, v, sx, sw, t, n);
-                else if (p.y_dtype == kBF16) i8_store4<kBF16>(p, v, sx, sw, t, n);
-                else i8_store4<kF16>(p, v, sx, sw, t, n);
+                if (p.y_dtype == kF32) i8_store4<kF32>(p, v, unit_sx, unit_sw, t, n);
+                else if (p.y_dtype == kBF16) i8_store4<kBF16>(p, v, unit_sx, unit_sw, t, n);
+                else i8_store4<kF16>(p, v, unit_sx, unit_sw, t, n);
             }
         }
         cluster_sync_all();  // nobody reads this CTA's shared memory any more

@@ -38,7 +38,7 @@ struct NormParams {
 };
 
 // Eight values as they lie in memory, and as floats. A dtype is the same for a whole launch; HT is the 16-bit type where all 16-bit tensors
-// of the call have the same one, else kF32: chosen at run time, where both conversions are made (2048 rows of 4096 in fp16: 15.5 us for 12.4).
+// of the call have the same one, else kF32: chosen at run time, where both conversions are made.
 template <int HT>
 __device__ __forceinline__ int32_t known_type(int32_t dtype) { return HT == kF32 || dtype == kF32 ? dtype : HT; }
 
@@ -101,7 +101,7 @@ __device__ __forceinline__ Raw8 pack8(int32_t dtype, const float (&v)[8]) {
 }
 __device__ __forceinline__ void store8(void* p, int32_t dtype, size_t i, const Raw8& r) {
     if (dtype == kF32) {
-        // (whole sectors: two stores of 16 bytes, 32 apart between lanes, are 30 % of the kernel's time)
+        // (whole sectors: with two stores of 16 bytes, 32 apart between lanes, 4096 rows of 7680 took 2 us longer)
         asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(static_cast<float*>(p) + i), "r"(r.a.x), "r"(r.a.y), "r"(r.a.z), "r"(r.a.w),
                      "r"(r.b.x), "r"(r.b.y), "r"(r.b.z), "r"(r.b.w)
                      : "memory");
@@ -123,11 +123,16 @@ __device__ __forceinline__ void store1(void* p, int32_t dtype, size_t i, float v
     if (dtype == kF32) static_cast<float*>(p)[i] = v;
     else static_cast<uint16_t*>(p)[i] = dtype == kBF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
-// max(a, |b|), NaN if one of them is
-__device__ __forceinline__ float max_abs(float a, float b) {
+// Largest magnitude of three, NaN if one of them is
+__device__ __forceinline__ float max_abs(float a, float b, float c) {
     float r;
-    asm("{\n.reg .f32 t;\nabs.f32 t, %2;\nmax.NaN.f32 %0, %1, t;\n}\n" : "=f"(r) : "f"(a), "f"(b));
+    asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+__device__ __forceinline__ float max_abs8(float m, const float (&u)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) m = max_abs(m, u[j], u[j + 1]);
+    return m;
 }
 
 // Butterflies of spans FROM, 2 FROM, ... below TO inside a thread, and between lanes h apart: a + b in the lower one, a - b in the upper one,
@@ -164,14 +169,14 @@ __device__ __forceinline__ void rotate8(float (&u)[8], int lane) {
 __device__ __forceinline__ uint2 codes8(const float (&u)[8], float s, float inv) {
     constexpr float kMagic = 12582912.f, kFar = 0.49998f;
     uint32_t m[8];
-    bool far = true;
+    float off[8];
 #pragma unroll
     for (int j = 0; j < 8; j++) {
         const float v = fmaf(u[j], inv, kMagic), n = v - kMagic;
         m[j] = __float_as_uint(v);
-        far = far && fabsf(fmaf(u[j], inv, -n)) <= kFar;
+        off[j] = fmaf(u[j], inv, -n);
     }
-    if (!far) {
+    if (!(max_abs8(0.f, off) <= kFar)) {
 #pragma unroll
         for (int j = 0; j < 8; j++)
             if (!(fabsf(fmaf(u[j], inv, kMagic - __uint_as_float(m[j]))) <= kFar)) m[j] = (uint32_t)max(-127, min(127, __float2int_rn(__fdiv_rn(u[j], s))));
@@ -278,11 +283,13 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
 #pragma unroll
             for (int j = 0; j < 8; j++) u[c][j] = __fmul_rn(v[c][j], w[j]);
             rotate8<ROT>(u[c], lane);
-#pragma unroll
-            for (int j = 0; j < 8; j++) most = max_abs(most, u[c][j]);
+            most = max_abs8(most, u[c]);
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) most = max_abs(most, __shfl_xor_sync(0xffffffffu, most, o));
+        for (int o = 16; o > 0; o >>= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, most, o);
+            most = max_abs(most, other, other);
+        }
         if (lane == 0) wmax[warp] = most;
     }
 #pragma unroll
@@ -318,7 +325,10 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
     if (CODES) {
         float most = lane < warps ? wmax[lane] : 0.f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) most = max_abs(most, __shfl_xor_sync(0xffffffffu, most, o));
+        for (int o = 16; o > 0; o >>= 1) {
+            const float other = __shfl_xor_sync(0xffffffffu, most, o);
+            most = max_abs(most, other, other);
+        }
         const bool finite = most < INFINITY;  // (not with a NaN either)
         const float s = __fdiv_rn(most, 127.f), inv = __fdiv_rn(1.f, s);
         if (tid == 0) p.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : most == 0.f ? 0.f : __fmul_rn(s, q);
@@ -341,116 +351,123 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
 // groups of eight, 128 apart, so that spans 8 to 64 of a rotation go from lane to lane. The next row is under way into shared memory
 // meanwhile, copied by the warp that uses it, so that no barrier stands between copy and use. One barrier per row, the sums of two rows in turn.
 //
-// Bound: issue slots where codes are wanted (a lane's reductions, quotients and addresses are some 120 instructions per row, a rotated value some 25), else the
-// memory. 4096 rows of 4096, bf16 added to bf16, us, the kernel of a row per block / this one: out 28.1 / 23.3 (floor 20.5), codes
-// 32.4 / 29.3, rotated 44.7 / 34.0 (18.0); 7680 wide 70 / 44, 81 / 55, 95 / 65. With one group per lane 26.2, 33.0, 37.4; with four 27.9, 30.5, 35.3; a third
-// stage 25.4, 29.5, 34.3.
+// Bound: issue slots where codes are wanted (some 100 instructions per row and lane, 25 per rotated value), else the memory. 4096 rows of 4096,
+// bf16 added to bf16, us, the kernel of a row per block / this one: out 27.8 / 23.4 (floor 20.5), codes 32.3 / 21.9, rotated 44.3 / 28.0 (18.0); 7680 wide
+// 70 / 43.8, 80 / 39.7, 94 / 51.2. On the way: types chosen at run time 24.3, 27.6, 33.5, and addresses made per row 23.3, 29.3, 34.0; with one group
+// per lane then 26.2, 33.0, 37.4, with four 27.9, 30.5, 35.3, with a third stage 25.4, 29.5, 34.3.
 constexpr int kNormStages = 2;
 constexpr int kNormRowsSmem = 200 * 1024;  // of an SM's blocks
-template <bool OUT, bool CODES, int ROT, int HT>
+// TYPES: kSum32 and kSum16 have a 16-bit x and out and a residual of fp32 or the same type; kAnyTypes asks at run time, which makes both of every
+// conversion.
+enum { kAnyTypes, kSum32, kSum16 };
+template <int TYPES, bool OUT, bool CODES, int ROT, int HT>
 __global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const __grid_constant__ NormParams p) {
-    extern __shared__ uint4 ring[];  // r, then x: [stage][group of the lane][warp][lane]
+    constexpr int K = 2, LB = 32 / K, APART = 256 / K;  // groups of a lane, lanes of 256 values, values between a lane's groups
+    extern __shared__ uint4 ring[];                     // r, then x: [stage][group of the lane][warp][lane]
     __shared__ float wsum[2][64], wmax[2][32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
-    constexpr int K = 2, LB = 32 / K, APART = 256 / K;  // groups of a lane, lanes of 256 values, values between a lane's groups
-    const int first = warp * 256 * K + (lane / LB) * 256 + (lane % LB) * 8;  // the lane's first value
+    const int block = warp * 256 * K + (lane / LB) * 256, first = block + (lane % LB) * 8;  // the lanes' 256 values, the lane's first one
+    const bool live[K] = {first < p.d, first + APART < p.d};
     pdl_launch_dependents();
-    Raw8 rw[K];
-    if (p.w != nullptr) {  // (weights may be read ahead of the wait)
+    float w[K][8];
 #pragma unroll
-        for (int k = 0; k < K; k++)
-            if (first + APART * k < p.d) rw[k] = load8(p.w, p.w_dtype, first + APART * k);
+    for (int k = 0; k < K; k++) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) w[k][j] = 1.f;
+        if (p.w != nullptr && live[k]) {  // (weights may be read ahead of the wait)
+            unpack8<HT>(load8(p.w, p.w_dtype, first + APART * k), p.w_dtype, w[k]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[k][j] = __fadd_rn(w[k][j], p.offset);
+        }
     }
-    const uint32_t r_size = p.r_dtype == kF32 ? 4 : 2, x_size = p.x == nullptr ? 0 : p.x_dtype == kF32 ? 4 : 2;
-    const uint32_t r_stage = warps * 256 * K * r_size, x_stage = warps * 256 * K * x_size;
-    const uint32_t base = smem_u32(ring), x_base = base + kNormStages * r_stage;
-    // the warp's values of a row; fp32: 32 LB bytes per LB lanes and group, each copy half of them
-    auto copy = [&](uint32_t to, const char* row, uint32_t size) {
-        const int at = size == 4 ? warp * 256 * K + (lane / LB) * 256 + (lane % LB) * 4 : first;
-        to += (warp * 32 * 8) * size + (size == 4 ? (lane / LB) * (LB * 32) + (lane % LB) * 16 : lane * 16);
-        const char* src = row + at * size;
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            if (at + APART * k < p.d) cp_async_cg16(to + k * warps * 256 * size, src + APART * k * size);
-            if (size == 4 && at + APART * k + LB * 4 < p.d) cp_async_cg16(to + k * warps * 256 * size + LB * 16, src + APART * k * size + LB * 16);
-        }
+    // Everything that a row's addresses are made of, once
+    const int32_t r_dtype = TYPES == kAnyTypes ? p.r_dtype : TYPES == kSum32 ? kF32 : HT, x_dtype = TYPES == kAnyTypes ? p.x_dtype : HT;
+    const int32_t out_dtype = TYPES == kAnyTypes ? p.out_dtype : HT;
+    const bool wide_r = r_dtype == kF32, wide_x = x_dtype == kF32, add = TYPES != kAnyTypes || p.x != nullptr;
+    const uint32_t r_size = wide_r ? 4 : 2, x_size = wide_x ? 4 : 2, o_size = out_dtype == kF32 ? 4 : 2;
+    // a copy is 16 bytes: a group of 16-bit values; of fp32 ones LB lanes copy 16 LB neighbouring bytes twice
+    struct Source {
+        const char* row;
+        int64_t step;         // to the block's next row
+        uint32_t to, stage, group_to, group_from;
+        bool first, second;   // whether the copies of the lane's first and second group lie in the row
+        bool first2, second2;  // fp32: and 16 LB bytes further
     };
-    auto fetch = [&](int s, int64_t row) {
-        if (row < p.rows) {
-            copy(base + s * r_stage, static_cast<const char*>(p.r) + row * p.ldr * r_size, r_size);
-            if (x_size != 0) copy(x_base + s * x_stage, static_cast<const char*>(p.x) + row * p.ldx * x_size, x_size);
-        }
-        asm volatile("cp.async.commit_group;" ::: "memory");
+    auto source = [&](const void* t, int64_t ld, uint32_t size, uint32_t ring_at) {
+        Source s;
+        const int at = size == 4 ? block + (lane % LB) * 4 : first;
+        s.row = static_cast<const char*>(t) + ((int64_t)blockIdx.x * ld + at) * size;
+        s.step = (int64_t)gridDim.x * ld * size;
+        s.stage = warps * 256 * K * size;
+        s.group_to = warps * 256 * size;
+        s.group_from = APART * size;
+        s.to = ring_at + warp * 256 * size + (size == 4 ? (lane / LB) * (LB * 32) + (lane % LB) * 16 : lane * 16);
+        s.first = at < p.d;
+        s.second = at + APART < p.d;
+        s.first2 = at + LB * 4 < p.d;
+        s.second2 = at + APART + LB * 4 < p.d;
+        return s;
     };
-    auto take = [&](uint32_t from, uint32_t size, int k) {
-        from += ((k * warps + warp) * 32 + lane) * 8 * size;
+    const uint32_t base = smem_u32(ring), x_base = base + kNormStages * warps * 256 * K * r_size;
+    Source r = source(p.r, p.ldr, r_size, base), x = source(p.x, p.ldx, x_size, x_base);
+    uint32_t r_from = base + (warp * 32 + lane) * 8 * r_size, x_from = x_base + (warp * 32 + lane) * 8 * x_size;
+    char* r_out = static_cast<char*>(p.r_out) + ((int64_t)blockIdx.x * p.ldro + first) * r_size;
+    char* out = static_cast<char*>(p.out) + ((int64_t)blockIdx.x * p.ldo + first) * o_size;
+    int8_t* codes = p.codes + (int64_t)blockIdx.x * p.ldc + first;
+    const int64_t r_out_step = (int64_t)gridDim.x * p.ldro * r_size, out_step = (int64_t)gridDim.x * p.ldo * o_size, codes_step = (int64_t)gridDim.x * p.ldc;
+    auto copy = [&](Source& s, bool wide, uint32_t to) {
+        if (s.first) cp_async_cg16(to, s.row);
+        if (s.second) cp_async_cg16(to + s.group_to, s.row + s.group_from);
+        if (wide) {
+            if (s.first2) cp_async_cg16(to + LB * 16, s.row + LB * 16);
+            if (s.second2) cp_async_cg16(to + s.group_to + LB * 16, s.row + s.group_from + LB * 16);
+        }
+        s.row += s.step;
+    };
+    auto take = [&](uint32_t from, bool wide) {
         Raw8 v;
         v.a = lds128(from);
-        v.b = size == 4 ? lds128(from + 16) : make_uint4(0, 0, 0, 0);
+        v.b = wide ? lds128(from + 16) : make_uint4(0, 0, 0, 0);
         return v;
     };
-    auto weights = [&](int k, float (&w)[8]) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) w[j] = 1.f;
-        if (p.w == nullptr) return;
-        if (first + APART * k < p.d) unpack8<HT>(rw[k], p.w_dtype, w);
-        if (p.offset != 0.f) {
-#pragma unroll
-            for (int j = 0; j < 8; j++) w[j] = __fadd_rn(w[j], p.offset);
-        }
-    };
-    auto turned = [&](float (&u)[K][8]) {  // the rotation
-        if (ROT == 1) return;
-#pragma unroll
-        for (int k = 0; k < K; k++) {
-            rotate_spans<1, 8>(u[k]);
-#pragma unroll
-            for (int h = 1; h < (ROT < APART ? ROT / 8 : LB); h <<= 1) rotate_lanes(u[k], lane, h);
-        }
-#pragma unroll
-        for (int h = 1; h < ROT / APART; h <<= 1)
-#pragma unroll
-            for (int k = 0; k < K; k++)
-                if ((k & h) == 0) {
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float a = u[k][j], b = u[k + h][j];
-                        u[k][j] = __fadd_rn(a, b);
-                        u[k + h][j] = __fsub_rn(a, b);
-                    }
-                }
-    };
     pdl_wait();
-#pragma unroll
-    for (int s = 0; s < kNormStages - 1; s++) fetch(s, blockIdx.x + (int64_t)s * gridDim.x);
-    int s = 0, turn = 0;
-    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
-        // (into the stage of the row before: a barrier has passed since it was read)
-        fetch(s == 0 ? kNormStages - 1 : s - 1, row + (int64_t)(kNormStages - 1) * gridDim.x);
-        asm volatile("cp.async.wait_group %0;" ::"n"(kNormStages - 1) : "memory");
+    static_assert(kNormStages == 2, "a stage for the row under work and one for the next");
+    copy(r, wide_r, r.to);  // (there are no more blocks than rows)
+    if (add) copy(x, wide_x, x.to);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
+        // the next row, into the stage of the row before: a barrier has passed since it was read
+        const uint32_t r_at = turn ? r.stage : 0, x_at = turn ? x.stage : 0;
+        if (row + gridDim.x < p.rows) {
+            copy(r, wide_r, r.to + (r.stage - r_at));
+            if (add) copy(x, wide_x, x.to + (x.stage - x_at));
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncwarp();
         float v[K][8], sums[K];
 #pragma unroll
         for (int k = 0; k < K; k++) {
+            sums[k] = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; j++) v[k][j] = 0.f;
-            if (first + APART * k < p.d) {
-                unpack8<HT>(take(base + s * r_stage, r_size, k), p.r_dtype, v[k]);
-                if (x_size != 0) {
+            if (live[k]) {
+                unpack8<HT>(take(r_from + r_at + k * r.group_to, wide_r), r_dtype, v[k]);
+                if (add) {
                     float xv[8];
-                    unpack8<HT>(take(x_base + s * x_stage, x_size, k), p.x_dtype, xv);
+                    unpack8<HT>(take(x_from + x_at + k * x.group_to, wide_x), x_dtype, xv);
 #pragma unroll
                     for (int j = 0; j < 8; j++) v[k][j] += xv[j];
-                    const Raw8 stored = pack8<HT>(p.r_dtype, v[k]);
-                    store8(p.r_out, p.r_dtype, row * p.ldro + first + APART * k, stored);
-                    unpack8<HT>(stored, p.r_dtype, v[k]);
+                    const Raw8 stored = pack8<HT>(r_dtype, v[k]);
+                    store8(r_out + k * r.group_from, r_dtype, 0, stored);
+                    if (!wide_r) unpack8<HT>(stored, r_dtype, v[k]);
                 }
             }
-            sums[k] = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; j++) sums[k] = fmaf(v[k][j], v[k][j], sums[k]);
         }
-        s = s == kNormStages - 1 ? 0 : s + 1;
+        r_out += r_out_step;
         // (the order of the other kernel's lanes: 16, 8, 4, 2 and 1 groups apart)
         float sum = sums[0] + sums[1];
 #pragma unroll
@@ -460,20 +477,31 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const __grid_con
         float kept[OUT && CODES ? K : 1][8];  // r', where both outputs are wanted; v is u from here on
         if (CODES) {
 #pragma unroll
-            for (int k = 0; k < K; k++) {
-                float w[8];
-                weights(k, w);
+            for (int k = 0; k < K; k++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     if (OUT) kept[OUT ? k : 0][j] = v[k][j];
-                    v[k][j] = __fmul_rn(v[k][j], w[j]);
+                    v[k][j] = __fmul_rn(v[k][j], w[k][j]);
+                }
+            if (ROT > 1) {
+#pragma unroll
+                for (int k = 0; k < K; k++) {
+                    rotate_spans<1, 8>(v[k]);
+#pragma unroll
+                    for (int h = 1; h < (ROT < APART ? ROT / 8 : LB); h <<= 1) rotate_lanes(v[k], lane, h);
+                }
+                if (ROT > APART) {
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const float a = v[0][j], b = v[1][j];
+                        v[0][j] = __fadd_rn(a, b);
+                        v[1][j] = __fsub_rn(a, b);
+                    }
                 }
             }
-            turned(v);
 #pragma unroll
             for (int k = 0; k < K; k++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) most = max_abs(most, v[k][j]);
+                most = max_abs8(most, v[k]);
             const uint32_t m = __reduce_max_sync(0xffffffffu, __float_as_uint(most));  // (bits order as the values do, NaN last)
             if (lane == 0) wmax[turn][warp] = __uint_as_float(m);
         }
@@ -486,13 +514,13 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const __grid_con
         if (OUT) {
 #pragma unroll
             for (int k = 0; k < K; k++)
-                if (first + APART * k < p.d) {
-                    float w[8], o[8];
-                    weights(k, w);
+                if (live[k]) {
+                    float o[8];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) o[j] = ((CODES ? kept[CODES ? k : 0][j] : v[k][j]) * q) * w[j];
-                    store8(p.out, p.out_dtype, row * p.ldo + first + APART * k, pack8<HT>(p.out_dtype, o));
+                    for (int j = 0; j < 8; j++) o[j] = ((CODES ? kept[CODES ? k : 0][j] : v[k][j]) * q) * w[k][j];
+                    store8(out + k * APART * o_size, out_dtype, 0, pack8<HT>(out_dtype, o));
                 }
+            out += out_step;
         }
         if (CODES) {
             most = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < warps ? __float_as_uint(wmax[turn][lane]) : 0u));
@@ -502,23 +530,31 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const __grid_con
             if (tid == 0) p.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : most == 0.f ? 0.f : __fmul_rn(step, q);
 #pragma unroll
             for (int k = 0; k < K; k++)
-                if (first + APART * k < p.d) {
-                    const uint2 c = none ? make_uint2(0, 0) : codes8(v[k], step, inv);
-                    *reinterpret_cast<uint2*>(p.codes + row * p.ldc + first + APART * k) = c;
-                }
+                if (live[k]) *reinterpret_cast<uint2*>(codes + k * APART) = none ? make_uint2(0, 0) : codes8(v[k], step, inv);
+            codes += codes_step;
         }
+        turn ^= 1;
     }
 }
 
 typedef void (*NormKernel)(NormParams);
-template <int HT>
+template <int TYPES, int HT>
 NormKernel norm_pick_rows(bool out, bool codes, int rotate) {
-    if (!codes) return add_rmsnorm_rows_kernel<true, false, 1, HT>;
-    if (out) return rotate == 256 ? add_rmsnorm_rows_kernel<true, true, 256, HT> : rotate == 32 ? add_rmsnorm_rows_kernel<true, true, 32, HT> : add_rmsnorm_rows_kernel<true, true, 1, HT>;
-    return rotate == 256 ? add_rmsnorm_rows_kernel<false, true, 256, HT> : rotate == 32 ? add_rmsnorm_rows_kernel<false, true, 32, HT> : add_rmsnorm_rows_kernel<false, true, 1, HT>;
+    if (!codes) return add_rmsnorm_rows_kernel<TYPES, true, false, 1, HT>;
+    if (out)
+        return rotate == 256 ? add_rmsnorm_rows_kernel<TYPES, true, true, 256, HT> : rotate == 32 ? add_rmsnorm_rows_kernel<TYPES, true, true, 32, HT>
+                                                                                               : add_rmsnorm_rows_kernel<TYPES, true, true, 1, HT>;
+    return rotate == 256 ? add_rmsnorm_rows_kernel<TYPES, false, true, 256, HT> : rotate == 32 ? add_rmsnorm_rows_kernel<TYPES, false, true, 32, HT>
+                                                                                            : add_rmsnorm_rows_kernel<TYPES, false, true, 1, HT>;
 }
-NormKernel norm_pick_rows(int half, bool out, bool codes, int rotate) {
-    return half == kF16 ? norm_pick_rows<kF16>(out, codes, rotate) : half == kBF16 ? norm_pick_rows<kBF16>(out, codes, rotate) : norm_pick_rows<kF32>(out, codes, rotate);
+template <int HT>
+NormKernel norm_pick_rows(int types, bool out, bool codes, int rotate) {
+    return types == kSum32 ? norm_pick_rows<kSum32, HT>(out, codes, rotate) : types == kSum16 ? norm_pick_rows<kSum16, HT>(out, codes, rotate)
+                                                                                             : norm_pick_rows<kAnyTypes, HT>(out, codes, rotate);
+}
+NormKernel norm_pick_rows(int half, int types, bool out, bool codes, int rotate) {
+    return half == kF16 ? norm_pick_rows<kF16>(types, out, codes, rotate) : half == kBF16 ? norm_pick_rows<kBF16>(types, out, codes, rotate)
+                                                                                         : norm_pick_rows<kAnyTypes, kF32>(out, codes, rotate);
 }
 template <int NCH, int MAXT, bool VEC, int HT>
 NormKernel norm_pick(bool codes, int rotate) {
@@ -543,8 +579,9 @@ bool aligned(const void* p, int64_t ld, int esz) {
 
 int32_t norm_init(iq_ctx* ctx) {
     for (int half = 0; half < 3; half++)
-        for (int mode = 0; mode < 7; mode++) {  // out; out and codes of three rotations; codes of three
-            const NormKernel k = norm_pick_rows(half, mode < 4, mode != 0, mode % 3 == 2 ? 32 : mode % 3 == 0 ? 256 : 0);
+        for (int mode = 0; mode < 21; mode++) {  // of three types: out; out and codes of three rotations; codes of three
+            const int m = mode % 7;
+            const NormKernel k = norm_pick_rows(half, mode / 7, m < 4, m != 0, m % 3 == 2 ? 32 : m % 3 == 0 ? 256 : 0);
             const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributeMaxDynamicSharedMemorySize, kNormRowsSmem);
             if (e != cudaSuccess) return check_cuda(ctx, e, "cudaFuncSetAttribute(add_rmsnorm_rows)");
         }
@@ -596,12 +633,13 @@ extern "C" int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int3
     NormKernel kernel = nch == 1 ? norm_pick<1, 1024>(vec, half, c8, rotate) : threads <= 512 ? norm_pick<4, 512>(vec, half, c8, rotate)
                                                                                               : norm_pick<4, 1024>(vec, half, c8, rotate);
     // Many rows: more than the blocks that run at once (of 64 registers a thread, the stages in shared memory). The norm alone of an fp32 sum is at the memory's
-    // rate up to some 5000 values with a row per block as well, and faster (4096 rows of 4096: 31.9 against 37.0 us; of 7680: 75 against 69).
+    // rate with a row per block as well up to some 5000 values (4096 rows of 4096: 31.9 us, floor 30.8; of 7680 75 us, here 64).
     const int row_threads = (d + 511) / 512 * 32;
     const size_t row_smem = (size_t)kNormStages * row_threads * 16 * (dtype_size(r_dtype) + (x == nullptr ? 0 : dtype_size(x_dtype)));
     const int at_once = row_threads > 1024 ? 0 : ctx->sms * (int)std::min<size_t>({(size_t)(1024 / row_threads), kNormRowsSmem / row_smem, 16});
     if (vec && at_once > 0 && rows > at_once && (c8 || r_dtype != kF32 || d > 5120)) {
-        kernel = norm_pick_rows(half, out != nullptr, c8, rotate);
+        const bool x16 = x != nullptr && x_dtype != kF32 && (out == nullptr || out_dtype != kF32);
+        kernel = norm_pick_rows(half, !x16 ? kAnyTypes : r_dtype == kF32 ? kSum32 : kSum16, out != nullptr, c8, rotate);
         threads = row_threads;
         blocks = at_once;
         smem = row_smem;

@@ -300,7 +300,8 @@ class I8Linear:
         if rotate is None:
             rotate = 256 if m.K % 256 == 0 else 32
         dev = m.w.device
-        w, s = torch.empty(m.N, m.K, dtype=torch.int8, device=dev), torch.empty(m.N, dtype=torch.float32, device=dev)
+        with torch.cuda.stream(stream):  # (None: the current one) the memory's stream is the kernel's
+            w, s = torch.empty(m.N, m.K, dtype=torch.int8, device=dev), torch.empty(m.N, dtype=torch.float32, device=dev)
         ctx, q = capi.context(m.device_index), m.qlinear()
         ctx.check(capi.lib().iq_i8_pack(ctx.handle, stream.cuda_stream if stream is not None else _raw_stream(m.device_index), C.byref(q), rotate, w.data_ptr(), s.data_ptr()))
         return cls(w, s, rotate)
@@ -322,15 +323,17 @@ class I8Linear:
                stream: Optional[torch.cuda.Stream] = None):
         """y[rows, N] (+)= (x codes · wᵀ codes) · x_scales · scales for int8 rows x [rows, K], any number of them."""
         dev = self.w.get_device()
-        if not (dev >= 0 and x.get_device() == dev and x_scales.get_device() == dev and y.get_device() == dev and x.dim() == 2 and y.dim() == 2 and x_scales.dim() == 1):
+        try:
+            (xr, xk), (ldx, xs), (yr, yn), (ldy, ys), (sr,), (ss,) = x.shape, x.stride(), y.shape, y.stride(), x_scales.shape, x_scales.stride()
+            yt = _DT.get(y.dtype, -1)
+            ok = (dev >= 0 and x.get_device() == dev and x_scales.get_device() == dev and y.get_device() == dev and 0 <= rows <= xr and rows <= yr and xk == self.K
+                  and yn == self.N and xs == 1 and (ys == 1 or yn == 1) and yt >= 0 and x.dtype == torch.int8 and x_scales.dtype == torch.float32 and sr >= rows
+                  and (rows <= 1 or ss == 1))
+        except (ValueError, AttributeError):  # another number of dimensions, no tensor
+            ok = False
+        if not ok:
             self._check(x, x_scales, y, rows)
             _need_cuda(x)
-            raise ValueError("I8Linear does not take these tensors")
-        (xr, xk), (ldx, xs), (yr, yn), (ldy, ys) = x.shape, x.stride(), y.shape, y.stride()
-        yt = _DT.get(y.dtype, -1)
-        if not (0 <= rows <= xr and rows <= yr and xk == self.K and yn == self.N and xs == 1 and (ys == 1 or yn == 1) and yt >= 0 and x.dtype == torch.int8
-                and x_scales.dtype == torch.float32 and x_scales.shape[0] >= rows and (rows <= 1 or x_scales.stride(0) == 1)):
-            self._check(x, x_scales, y, rows)
             raise ValueError("I8Linear does not take these tensors")
         if rows <= 1:  # (one row has no stride)
             ldx, ldy = xk, yn

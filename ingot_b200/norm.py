@@ -65,55 +65,45 @@ def add_rmsnorm(x: Optional[torch.Tensor], residual: torch.Tensor, weight: Optio
     [rows, d] with any row stride; x None: the norm of residual alone; weight None: weights of one.
     residual_out may be residual, out may be x (same stride and element size); nothing else may overlap."""
     # (each condition once, in few steps: a call of one row is bound by the host. What fails one is described by _check)
-    ok = residual.dim() == 2 and (out is not None or codes is not None) and rotate in ROTATIONS
-    if ok:
-        have, d = residual.shape
-        ldr, step = residual.stride()
+    dev, ok = -1, (out is not None or codes is not None) and rotate in ROTATIONS and (x is not None or residual_out is None)
+    xp = xt = ldx = rop = ldro = wp = wt = op = ot = ldo = cp = ldc = sp = 0
+    try:
+        (have, d), (ldr, step) = residual.shape, residual.stride()
         rt, dev = _DT.get(residual.dtype, -1), residual.get_device()
-        ok = 0 <= rows <= have and (step == 1 or d == 1) and 1 <= d <= MAX_WIDTH and rt >= 0 and eps >= 0 and (codes is None) == (scales is None)
-        xp = xt = ldx = rop = ldro = wp = wt = op = ot = ldo = cp = ldc = sp = 0
-        wide = rows > 1  # (one row has no stride)
+        ok = ok and 0 <= rows <= have and (step == 1 or d == 1) and 1 <= d <= MAX_WIDTH and rt >= 0 and eps >= 0
         if x is not None:
-            ok = ok and x.dim() == 2 and x.get_device() == dev
-            if ok:
-                (n, k), (ldx, step) = x.shape, x.stride()
-                xp, xt = x.data_ptr(), _DT.get(x.dtype, -1)
-                ok = n >= rows and k == d and (step == 1 or d == 1) and xt >= 0
+            (n, k), (ldx, step) = x.shape, x.stride()
+            xp, xt = x.data_ptr(), _DT.get(x.dtype, -1)
+            ok = ok and n >= rows and k == d and (step == 1 or d == 1) and xt >= 0 and x.get_device() == dev
             if residual_out is None:
                 rop, ldro = residual.data_ptr(), ldr
             else:
-                ok = ok and residual_out.dim() == 2 and residual_out.get_device() == dev and residual_out.dtype == residual.dtype
-                if ok:
-                    (n, k), (ldro, step) = residual_out.shape, residual_out.stride()
-                    rop = residual_out.data_ptr()
-                    ok = n >= rows and k == d and (step == 1 or d == 1)
-        elif residual_out is not None:
-            ok = False
-        if ok and weight is not None:
+                (n, k), (ldro, step) = residual_out.shape, residual_out.stride()
+                rop = residual_out.data_ptr()
+                ok = ok and n >= rows and k == d and (step == 1 or d == 1) and residual_out.get_device() == dev and residual_out.dtype == residual.dtype
+        if weight is not None:
             wp, wt = weight.data_ptr(), _DT.get(weight.dtype, -1)
-            ok = wt >= 0 and weight.get_device() == dev and weight.numel() == d and weight.is_contiguous()
-        if ok and out is not None:
-            ok = out.dim() == 2 and out.get_device() == dev
-            if ok:
-                (n, k), (ldo, step) = out.shape, out.stride()
-                op, ot = out.data_ptr(), _DT.get(out.dtype, -1)
-                ok = n >= rows and k == d and (step == 1 or d == 1) and ot >= 0
-        if ok and codes is not None:
-            ok = codes.dim() == 2 and codes.get_device() == dev and scales.get_device() == dev and scales.dim() == 1
-            if ok:
-                (n, k), (ldc, step) = codes.shape, codes.stride()
-                cp, sp = codes.data_ptr(), scales.data_ptr()
-                ok = (n >= rows and k == d and (step == 1 or d == 1) and codes.dtype == torch.int8 and scales.dtype == torch.float32
-                      and scales.shape[0] >= rows and (not wide or scales.stride(0) == 1) and (not rotate or d % rotate == 0))
-        elif rotate:
+            ok = ok and wt >= 0 and weight.get_device() == dev and weight.numel() == d and weight.is_contiguous()
+        if out is not None:
+            (n, k), (ldo, step) = out.shape, out.stride()
+            op, ot = out.data_ptr(), _DT.get(out.dtype, -1)
+            ok = ok and n >= rows and k == d and (step == 1 or d == 1) and ot >= 0 and out.get_device() == dev
+        if codes is not None:
+            (n, k), (ldc, step), (m,), (one,) = codes.shape, codes.stride(), scales.shape, scales.stride()
+            cp, sp = codes.data_ptr(), scales.data_ptr()
+            ok = (ok and n >= rows and k == d and (step == 1 or d == 1) and codes.dtype == torch.int8 and scales.dtype == torch.float32 and m >= rows and (one == 1 or rows <= 1)
+                  and codes.get_device() == dev and scales.get_device() == dev and (not rotate or d % rotate == 0))
+        elif rotate or scales is not None:
             ok = False
+    except (ValueError, AttributeError):  # another number of dimensions, no tensor
+        ok = False
     if not ok or dev < 0:
         _check(x, residual, weight, rows, eps, residual_out, out, codes, scales, rotate)
         if residual.device.type != "cuda":
             _no_cpu()
         raise ValueError("add_rmsnorm does not take these tensors")
     ctx = capi.context(dev)
-    if not wide:
+    if rows <= 1:  # (one row has no stride)
         ldx = ldr = ldro = ldo = ldc = d
     st = capi.call().add_rmsnorm(ctx.address, stream.cuda_stream if stream is not None else _raw_stream(dev), xp, xt, ldx, residual.data_ptr(), rt, ldr,
                                  rop, ldro, wp, wt, weight_offset, eps, rows, d, op, ot, ldo, cp, ldc, sp, rotate)

@@ -98,6 +98,7 @@ class LogitRules:
         self.device = self._kept[0].device if self._kept else None
         if self.device is not None and self.device.type != "cuda":
             _no_cpu()
+        self._index = None if self.device is None else self.device.index
         at = lambda t: 0 if t is None else t.data_ptr()
         wide = lambda t: 0 if t is None else t.stride(0) if t.shape[0] > 1 else t.shape[1]
         self._c = capi.LogitRules(at(tokens), wide(tokens), at(lens), at(prompt_lens), at(repetition), at(presence), at(frequency), at(bias_offsets), at(bias_tokens),
@@ -124,13 +125,16 @@ class LogitRules:
         """The first `rows` rows of logits x [*, vocab] under the rules, as float32 into out (x itself where that is float32; None: a new tensor)."""
         dev = x.get_device()
         if out is None and dev >= 0:
-            out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
-        ok = out is not None and out.get_device() == dev and x.dim() == 2 and out.dim() == 2 and (self.device is None or self.device.index == dev)
-        if ok:
+            with torch.cuda.stream(stream):  # (None: the current one) the memory's stream is the kernel's
+                out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
+        try:
             (xr, xv), (ldx, xs), (outr, ov), (ldo, os) = x.shape, x.stride(), out.shape, out.stride()
             xt = _DT.get(x.dtype, -1)
-            ok = 0 <= rows <= self.rows and rows <= xr and rows <= outr and xv == self.vocab and ov == xv and (xv == 1 or xs == os == 1) and xt >= 0 and out.dtype == torch.float32
-        if not ok:
+            ok = (out.get_device() == dev and (self._index is None or self._index == dev) and 0 <= rows <= self.rows and rows <= xr and rows <= outr and xv == self.vocab and ov == xv
+                  and (xv == 1 or xs == os == 1) and xt >= 0 and out.dtype == torch.float32)
+        except (ValueError, AttributeError):  # another number of dimensions, no tensor
+            ok = False
+        if not ok or dev < 0:
             self._check(x, rows, out)
             if not x.is_cuda:
                 _no_cpu()
