@@ -109,11 +109,13 @@ __device__ __forceinline__ void store8(void* p, int32_t dtype, size_t i, const R
         *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = r.a;
     }
 }
-// One value at a time, for rows that are not aligned
-__device__ __forceinline__ float load1(const void* p, int32_t dtype, size_t i) {
-    if (dtype == kF32) return static_cast<const float*>(p)[i];
-    const uint16_t h = static_cast<const uint16_t*>(p)[i];
-    return dtype == kBF16 ? bf16_bits_to_f32(h) : __half2float(__ushort_as_half(h));
+// One value at a time, for rows that are not aligned: as it lies in memory, and as a float
+__device__ __forceinline__ uint32_t load1(const void* p, int32_t dtype, size_t i) {
+    return dtype == kF32 ? static_cast<const uint32_t*>(p)[i] : (uint32_t)static_cast<const uint16_t*>(p)[i];
+}
+__device__ __forceinline__ float unpack1(uint32_t v, int32_t dtype) {
+    const float h = __half2float(__ushort_as_half((unsigned short)v)), b = bf16_bits_to_f32(v);
+    return dtype == kF32 ? __uint_as_float(v) : dtype == kBF16 ? b : h;
 }
 __device__ __forceinline__ float round1(float v, int32_t dtype) {
     if (dtype == kF32) return v;
@@ -186,8 +188,8 @@ __device__ __forceinline__ uint2 codes8(const float (&u)[8], float s, float inv)
 }
 
 // A row per block, NCH times eight values per thread.
-// VEC: rows of whole, 16-byte aligned groups of eight (codes: 8-byte aligned). Else value by value: neighbouring threads take
-// neighbouring values, except where the rotation wants a thread to have eight in a row.
+// VEC: rows of whole groups of eight that lie on their own size. Else value by value: neighbouring threads take
+// neighbouring values, and where the rotation wants a thread to have eight in a row, they pass through shared memory.
 // CODES, ROT: int8 codes, rotated in blocks of ROT inputs (1: not).
 template <int NCH, int MAXT, bool VEC, bool CODES, int ROT, int HT>
 __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant__ NormParams p) {
@@ -196,8 +198,8 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
     const size_t row = blockIdx.x;
     pdl_launch_dependents();
-    constexpr bool RUNS = VEC || ROT > 1;  // a thread's eight values lie in a row
-    auto at = [&](int c, int j) { return RUNS ? (c * (int)blockDim.x + tid) * 8 + j : (c * 8 + j) * (int)blockDim.x + tid; };
+    __shared__ __align__(16) float turn[VEC || ROT == 1 ? 1 : MAXT * 8];  // a warp's 256 values on their way to eight in a row per thread, and back
+    auto at = [&](int c, int j) { return (c * (int)blockDim.x + warp * 32) * 8 + (VEC ? lane * 8 + j : j * 32 + lane); };
     Raw8 rw[VEC ? NCH : 1];
     if (VEC && p.w != nullptr) {  // (weights may be read ahead of the wait)
 #pragma unroll
@@ -232,16 +234,23 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
             }
         }
     } else {
+        // (sixteen loads under way: the indexes are cut at the row's end, no guard stands between them)
 #pragma unroll
-        for (int c = 0; c < NCH; c++)
+        for (int c = 0; c < NCH; c++) {
+            uint32_t rr[8], xx[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) rr[j] = load1(p.r, p.r_dtype, row * p.ldr + min(at(c, j), p.d - 1));
+            if (p.x != nullptr) {
+#pragma unroll
+                for (int j = 0; j < 8; j++) xx[j] = load1(p.x, p.x_dtype, row * p.ldx + min(at(c, j), p.d - 1));
+            }
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                v[c][j] = 0.f;
-                if (at(c, j) < p.d) {
-                    v[c][j] = load1(p.r, p.r_dtype, row * p.ldr + at(c, j));
-                    if (p.x != nullptr) v[c][j] = round1(v[c][j] + load1(p.x, p.x_dtype, row * p.ldx + at(c, j)), p.r_dtype);
-                }
+                v[c][j] = unpack1(rr[j], p.r_dtype);
+                if (p.x != nullptr) v[c][j] = round1(v[c][j] + unpack1(xx[j], p.x_dtype), p.r_dtype);
+                if (at(c, j) >= p.d) v[c][j] = 0.f;
             }
+        }
         if (p.x != nullptr) {  // (behind all loads: r_out may be r)
 #pragma unroll
             for (int c = 0; c < NCH; c++)
@@ -266,9 +275,11 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
         if (VEC) {
             if (at(c, 0) < p.d) unpack8<HT>(rw[VEC ? c : 0], p.w_dtype, w);
         } else {
+            uint32_t ww[8];
 #pragma unroll
-            for (int j = 0; j < 8; j++)
-                if (at(c, j) < p.d) w[j] = load1(p.w, p.w_dtype, at(c, j));
+            for (int j = 0; j < 8; j++) ww[j] = load1(p.w, p.w_dtype, min(at(c, j), p.d - 1));
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = unpack1(ww[j], p.w_dtype);
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) w[j] = __fadd_rn(w[j], p.offset);
@@ -282,6 +293,16 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
             weights(c, w);
 #pragma unroll
             for (int j = 0; j < 8; j++) u[c][j] = __fmul_rn(v[c][j], w[j]);
+            if (!VEC && ROT > 1) {
+                float* const mine = turn + warp * 256;
+#pragma unroll
+                for (int j = 0; j < 8; j++) mine[j * 32 + lane] = u[c][j];
+                __syncwarp();
+                const float4 a = *reinterpret_cast<const float4*>(mine + lane * 8), b = *reinterpret_cast<const float4*>(mine + lane * 8 + 4);
+                u[c][0] = a.x; u[c][1] = a.y; u[c][2] = a.z; u[c][3] = a.w;
+                u[c][4] = b.x; u[c][5] = b.y; u[c][6] = b.z; u[c][7] = b.w;
+                __syncwarp();
+            }
             rotate8<ROT>(u[c], lane);
             most = max_abs8(most, u[c]);
         }
@@ -338,6 +359,14 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
             const uint2 k = none ? make_uint2(0, 0) : codes8(u[c], s, inv);
             if (VEC) {
                 if (at(c, 0) < p.d) *reinterpret_cast<uint2*>(p.codes + row * p.ldc + at(c, 0)) = k;
+            } else if (ROT > 1) {  // codes of eight values in a row per thread, stored neighbour by neighbour
+                uint2* const mine = reinterpret_cast<uint2*>(turn + warp * 256);
+                mine[lane] = k;
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 8; j++)
+                    if (at(c, j) < p.d) p.codes[row * p.ldc + at(c, j)] = reinterpret_cast<const int8_t*>(mine)[j * 32 + lane];
+                __syncwarp();
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; j++)
@@ -619,7 +648,7 @@ extern "C" int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int3
     p.rows = rows; p.d = d; p.offset = weight_offset; p.eps = eps;
     const bool vec = d % 8 == 0 && aligned(x, ldx, dtype_size(x_dtype)) && aligned(residual, ldr, dtype_size(r_dtype)) && aligned(residual_out, ldro, dtype_size(r_dtype)) &&
                      aligned(weight, 0, dtype_size(w_dtype)) && aligned(out, ldo, dtype_size(out_dtype)) && aligned(codes, ldc, 1);
-    const int groups = (d + 7) / 8, nch = groups <= 1024 ? 1 : 4;
+    const int groups = (d + 7) / 8, nch = groups <= 1024 ? 1 : groups <= 2048 ? 2 : 4;
     int threads = round_up((groups + nch - 1) / nch, 32), blocks = rows;
     size_t smem = 0;
     // the one 16-bit type of the call (bf16 where it has none), kF32 where it has both
@@ -630,8 +659,8 @@ extern "C" int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int3
     meet(x, x_dtype); meet(residual, r_dtype); meet(weight, w_dtype); meet(out, out_dtype);
     if (half == -1) half = kBF16;
     const bool c8 = codes != nullptr;
-    NormKernel kernel = nch == 1 ? norm_pick<1, 1024>(vec, half, c8, rotate) : threads <= 512 ? norm_pick<4, 512>(vec, half, c8, rotate)
-                                                                                              : norm_pick<4, 1024>(vec, half, c8, rotate);
+    NormKernel kernel = nch == 1 ? norm_pick<1, 1024>(vec, half, c8, rotate) : nch == 2 ? norm_pick<2, 1024>(vec, half, c8, rotate)
+                                                                                       : norm_pick<4, 1024>(vec, half, c8, rotate);
     // Many rows: more than the blocks that run at once (of 64 registers a thread, the stages in shared memory). The norm alone of an fp32 sum is at the memory's
     // rate with a row per block as well up to some 5000 values (4096 rows of 4096: 31.9 us, floor 30.8; of 7680 75 us, here 64).
     const int row_threads = (d + 511) / 512 * 32;

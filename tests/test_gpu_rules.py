@@ -110,7 +110,7 @@ def test_one_token_many_times(cuda_device):
     check(rng, 2, 1000, a)
 
 
-@pytest.mark.parametrize("V", [1000, 40000])
+@pytest.mark.parametrize("V", [1000, 1001, 2047, 40000, 40003])
 def test_what_lies_outside_is_passed_over(cuda_device, V):
     rng = np.random.default_rng(V)
     for _ in range(4):
@@ -146,6 +146,26 @@ def test_infinities_nan_and_empty_masks(cuda_device):
     assert (argmax_rows(torch.from_numpy(got).cuda(), rows).cpu().numpy()[1]) == 0
     idx, val, z = TopK64(rows, V, torch.device("cuda", 0)).encode(torch.from_numpy(got).cuda(), rows, [1.0])
     assert (idx[1] == -1).all() and (val[1] == torch.finfo(F32).min).all()
+
+
+@pytest.mark.parametrize("V", [2045, 2046, 2047, 2048, 20477, 20478, 20480, 20481, 40957])
+def test_the_ends_of_the_blocks_parts(cuda_device, V):
+    """Rows that begin anywhere within a group of four, vocabularies next to whole parts."""
+    rng = np.random.default_rng(V)
+    for rows, pad in ((4, 0), (900, 1)):
+        check(rng, rows, V, some(rng, rows, V, history=60, bias=8, masks=3), pad=pad)
+
+
+def test_results_that_begin_elsewhere(cuda_device):
+    """x and out at different places within a group of four: one logit at a time."""
+    rng = np.random.default_rng(11)
+    rows, V = 3, 4999
+    a = some(rng, rows, V, history=100, bias=20, masks=2)
+    x = torch.from_numpy(rng.normal(size=(rows, V)).astype(np.float32)).cuda()
+    out = torch.full((rows * V + 9,), 7.0, device="cuda")
+    for at in (0, 1, 2, 3):
+        got = LogitRules(rows, V, **device(a)).encode(x, rows, out=out[at:at + rows * V].view(rows, V))
+        assert np.array_equal(got.cpu().numpy(), qref.logit_rules(x.cpu().numpy(), np.float32, **a))
 
 
 @pytest.mark.parametrize("V,pad", [(9000, 0), (9001, 0), (9000, 6)])
