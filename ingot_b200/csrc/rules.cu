@@ -21,7 +21,7 @@ namespace {
 constexpr int kRuleThreads = 512;
 constexpr int kRuleMaxVocab = 262144;
 constexpr int kRulePerSm = 3;     // blocks of an SM
-constexpr int kRuleSpan = 20480;  // most logits of a block
+constexpr int kRuleSpan = 24576;  // most logits of a block
 constexpr int kRuleBatch = 2;     // times four logits of a thread that are under way at once
 constexpr int kRuleLook = 4;      // tokens of the history likewise, before its length is known
 
@@ -47,6 +47,13 @@ struct Counter {
         else atomicAdd(w, 1u << up);
     }
     static __device__ __forceinline__ uint32_t one(const uint32_t* c, uint32_t t) { return WIDE ? c[t] : reinterpret_cast<const uint16_t*>(c)[t]; }
+    // the same without a branch, where t is one of n tokens
+    template <bool ASKED>
+    static __device__ __forceinline__ void note_if(uint32_t c, uint32_t t, uint32_t n) {
+        const uint32_t at = c + (WIDE ? t * 4 : (t >> 1) * 4), v = (ASKED ? PROMPT : 1u) << (WIDE ? 0 : 16 * (t & 1));
+        if (ASKED) asm volatile("{\n.reg .pred p;\nsetp.lt.u32 p, %0, %1;\n@p red.shared.or.b32 [%2], %3;\n}\n" ::"r"(t), "r"(n), "r"(at), "r"(v) : "memory");
+        else asm volatile("{\n.reg .pred p;\nsetp.lt.u32 p, %0, %1;\n@p red.shared.add.u32 [%2], %3;\n}\n" ::"r"(t), "r"(n), "r"(at), "r"(v) : "memory");
+    }
     // of four tokens, i a multiple of four
     static __device__ __forceinline__ uint4 four(const uint32_t* c, int i) {
         if (WIDE) return *reinterpret_cast<const uint4*>(c + i);
@@ -182,14 +189,23 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
         };
 #pragma unroll
         for (int k = 0; k < kRuleLook; k++) note(k * kRuleThreads + tid, look[k]);
+        // Long histories by 4096 tokens that are all of the prompt or all generated (a load of 32 costs some ten instructions then, else thirty: the blocks of a
+        // row all look at all of them)
         const bool whole = (reinterpret_cast<uintptr_t>(tokens) & 15) == 0;
+        const uint32_t counters = smem_u32(count);
         for (int i0 = kRuleLook * kRuleThreads; i0 < len; i0 += 8 * kRuleThreads) {
-            if (whole && i0 + 8 * kRuleThreads <= len) {
+            const int i1 = i0 + 8 * kRuleThreads;
+            if (whole && i1 <= len && (i0 >= prompt || i1 <= prompt)) {
                 const int4* const q = reinterpret_cast<const int4*>(tokens + i0) + tid;
                 const int4 a = q[0], b = q[kRuleThreads];
-                const int ia = i0 + 4 * tid, ib = ia + 4 * kRuleThreads;
-                note(ia, a.x); note(ia + 1, a.y); note(ia + 2, a.z); note(ia + 3, a.w);
-                note(ib, b.x); note(ib + 1, b.y); note(ib + 2, b.z); note(ib + 3, b.w);
+                const uint32_t t[8] = {(uint32_t)a.x, (uint32_t)a.y, (uint32_t)a.z, (uint32_t)a.w, (uint32_t)b.x, (uint32_t)b.y, (uint32_t)b.z, (uint32_t)b.w};
+                if (i0 >= prompt) {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) Count::template note_if<false>(counters, t[k] - (uint32_t)lo, (uint32_t)n);
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 8; k++) Count::template note_if<true>(counters, t[k] - (uint32_t)lo, (uint32_t)n);
+                }
                 continue;
             }
             uint32_t t[8];
@@ -301,7 +317,8 @@ void (*rules_pick(bool vec))(RuleParams) { return vec ? logit_rules_kernel<HIST,
 
 int32_t rules_init(iq_ctx* ctx) {
     for (int vec = 0; vec < 2; vec++) {
-        const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(rules_pick<true, true>(vec != 0)), cudaFuncAttributeMaxDynamicSharedMemorySize, kRuleSpan * 4);
+        cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(rules_pick<true, true>(vec != 0)), cudaFuncAttributeMaxDynamicSharedMemorySize, kRuleSpan * 4);
+        if (e == cudaSuccess) e = cudaFuncSetAttribute(reinterpret_cast<const void*>(rules_pick<true, false>(vec != 0)), cudaFuncAttributeMaxDynamicSharedMemorySize, kRuleSpan * 2);
         if (e != cudaSuccess) return check_cuda(ctx, e, "cudaFuncSetAttribute(logit_rules)");
     }
     return kOk;
