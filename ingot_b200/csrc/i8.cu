@@ -227,7 +227,7 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
         const int q = warp & 3;  // the quarter of tensor memory that this warp may read
         const uint32_t t0 = tmem + ((uint32_t)(32 * q) << 16);
         constexpr int C = BN < 32 ? BN : 32;
-        if (parts > 1 && u0 + (int)threadIdx.x - 64 < u1) unit_scales(u0 + (int)threadIdx.x - 64);
+        if (parts > 1 && u0 + (int)threadIdx.x < u1) unit_scales(u0 + (int)threadIdx.x);
         const int n = n0 + 32 * q + lane;
         const float sw = n < p.N ? p.sw[n] : 0.f, sx0 = lane < rows ? p.sx[row0 + lane] : 0.f, sx1 = 32 + lane < rows ? p.sx[row0 + 32 + lane] : 0.f;
         if (__all_sync(0xffffffffu, mbar_wait(sums, 0, abort_flag))) {
@@ -247,6 +247,10 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
         }
     }
     __syncwarp();
+    if (parts > 1 && warp < 2) {
+        pdl_wait();
+        if (u0 + (int)threadIdx.x < u1) unit_scales(u0 + (int)threadIdx.x);
+    }
     if (*abort_flag && warp == 0) {  // copies in flight land before the shared memory is given back
         const long long t0 = clock64();
         while (clock64() - t0 < 2000000) {}
@@ -255,11 +259,11 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
     __syncthreads();
     if (parts > 1) {
         cluster_sync_all();  // every CTA's sums lie in its shared memory
-        if (warp >= 2 && !*abort_flag) {
+        if (!*abort_flag) {
             // this CTA's share of the tile, four features at a time; all loads before the first sum
-            for (int u = u0 + (int)threadIdx.x - 64; u < u1; u += 128) {
+            for (int u = u0 + (int)threadIdx.x; u < u1; u += kI8Threads) {
                 const int t = row0 + u / 32, n = n0 + u % 32 * 4;
-                if (u >= u0 + 128) unit_scales(u);
+                if (u >= u0 + kI8Threads) unit_scales(u);
                 int4 o[8];
 #pragma unroll
                 for (int c = 0; c < 8; c++)
@@ -273,7 +277,9 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
                 else i8_store4<kF16>(p, v, unit_sx, unit_sw, t, n);
             }
         }
-        cluster_sync_all();  // nobody reads this CTA's shared memory any more
+        // nobody reads this CTA's shared memory any more (what was read has gone into the sums: no ordering of memory to wait for)
+        __syncwarp();
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
     }
     if (*abort_flag && threadIdx.x == 0 && p.status != nullptr) atomicExch(p.status, kErrTimeout);
     if (warp == 1) {
