@@ -17,6 +17,7 @@
 // additions of few lanes each), lanes with the same token found by match (16.8), tokens queued until there are 32 (14.4).
 #include <math.h>
 #include <algorithm>
+#include <type_traits>
 
 #include "internal.h"
 #include "ptx.cuh"
@@ -51,6 +52,14 @@ struct Counter {
         const uint32_t up = WIDE ? 0 : 16 * (t & 1);
         if (prompt) atomicOr(w, PROMPT << up);
         else atomicAdd(w, 1u << up);
+    }
+    static __device__ __forceinline__ bool any(const uint32_t* c, int i) {
+        if (WIDE) {
+            const uint4 w = *reinterpret_cast<const uint4*>(c + i);
+            return (w.x | w.y | w.z | w.w) != 0;
+        }
+        const uint2 w = *reinterpret_cast<const uint2*>(c + i / 2);
+        return (w.x | w.y) != 0;
     }
     static __device__ __forceinline__ uint32_t one(const uint32_t* c, uint32_t t) { return WIDE ? c[t] : reinterpret_cast<const uint16_t*>(c)[t]; }
     // the same without a branch, where t is one of n tokens
@@ -91,12 +100,13 @@ struct BiasList {
     }
 };
 
-// HIST: with counters. VEC: a row of x and the same one of out begin at the same place within groups of four (0 to 3 elements into one); the
-// blocks' parts begin on such groups, the first one's `shift` before the row. Rows of an odd vocabulary are taken four logits at a time like this
+// DT: x's type. HIST: with counters. VEC: a row of x and the same one of out begin at the same place within groups of four (0 to 3 elements into one);
+// the blocks' parts begin on such groups, the first one's `shift` before the row. Rows of an odd vocabulary are taken four logits at a time like this
 // (eight rows of 151,665 4.0 us on one logit at a time, of 151,936 2.5).
-template <bool HIST, bool WIDE, bool VEC>
+template <int DT, bool HIST, bool WIDE, bool VEC>
 __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(const __grid_constant__ RuleParams p) {
     typedef Counter<WIDE> Count;
+    typedef typename std::conditional<DT == kF32, float, uint16_t>::type E;
     extern __shared__ uint4 smem[];
     __shared__ BiasList list;
     uint32_t* const count = reinterpret_cast<uint32_t*>(smem);
@@ -109,43 +119,43 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
         for (int i = tid; i < p.span / (WIDE ? 4 : 8); i += kRuleThreads) smem[i] = make_uint4(0, 0, 0, 0);
     if (tid == 0) list.n = 0;
     pdl_wait();
-    const char* const xr = static_cast<const char*>(p.x) + (size_t)row * p.ldx * (p.x_dtype == kF32 ? 4 : 2);
-    float* const out = p.out + (size_t)row * p.ldo;
-    // four logits as they lie in memory
-    auto load = [&](int i) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (i >= n) return v;
-        const int t = lo + i;
-        if (VEC && i + 4 <= n && t >= 0) {
-            if (p.x_dtype == kF32) {
-                v = *reinterpret_cast<const uint4*>(xr + (size_t)t * 4);
-            } else {
-                const uint2 h = *reinterpret_cast<const uint2*>(xr + (size_t)t * 2);
-                v.x = h.x;
-                v.y = h.y;
-            }
-        } else if (p.x_dtype == kF32) {
-            const uint32_t* q = reinterpret_cast<const uint32_t*>(xr) + t;
-            if (t >= 0) v.x = q[0];
-            if (i + 1 < n && t + 1 >= 0) v.y = q[1];
-            if (i + 2 < n && t + 2 >= 0) v.z = q[2];
-            if (i + 3 < n && t + 3 >= 0) v.w = q[3];
-        } else {
-            const uint16_t* q = reinterpret_cast<const uint16_t*>(xr) + t;
-            v.x = (t >= 0 ? q[0] : 0u) | (i + 1 < n && t + 1 >= 0 ? (uint32_t)q[1] << 16 : 0u);
-            v.y = (i + 2 < n && t + 2 >= 0 ? q[2] : 0u) | (i + 3 < n && t + 3 >= 0 ? (uint32_t)q[3] << 16 : 0u);
-        }
-        return v;
+    const E* const x = static_cast<const E*>(p.x) + (size_t)row * p.ldx + lo;  // (of the block's logits)
+    float* const out = p.out + (size_t)row * p.ldo + lo;
+    auto load1 = [&](int i) {
+        if (DT == kF32) return reinterpret_cast<const float*>(x)[i];
+        const uint16_t h = reinterpret_cast<const uint16_t*>(x)[i];
+        return DT == kBF16 ? bf16_bits_to_f32(h) : __half2float(__ushort_as_half(h));
     };
-    auto load1 = [&](uint32_t i) {
-        if (p.x_dtype == kF32) return reinterpret_cast<const float*>(xr)[lo + i];
-        const uint16_t h = reinterpret_cast<const uint16_t*>(xr)[lo + i];
-        return p.x_dtype == kBF16 ? bf16_bits_to_f32(h) : __half2float(__ushort_as_half(h));
+    // A thread has the groups of four tid, tid + kRuleThreads, ... of the part: those that lie in the row as a whole are turns first_ .. last_, one at
+    // either end may not (the row's first and last logits).
+    constexpr int kStep = 4 * kRuleThreads;
+    const int first_ = lo + 4 * tid < 0 ? 1 : 0, last_ = n >= 4 * tid + 4 ? (n - 4 * tid - 4) / kStep + 1 : 0;
+    struct Four {
+        uint32_t v[DT == kF32 ? 4 : 2];
+    };
+    auto load = [&](int turn) {
+        const E* const q = x + 4 * tid + turn * kStep;
+        Four f;
+        if (VEC && DT == kF32) {
+            const uint4 w = *reinterpret_cast<const uint4*>(q);
+            f.v[0] = w.x; f.v[1] = w.y; f.v[DT == kF32 ? 2 : 0] = w.z; f.v[DT == kF32 ? 3 : 0] = w.w;
+        } else if (VEC) {
+            const uint2 w = *reinterpret_cast<const uint2*>(q);
+            f.v[0] = w.x; f.v[1] = w.y;
+        } else if (DT == kF32) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) f.v[DT == kF32 ? j : 0] = reinterpret_cast<const uint32_t*>(q)[j];
+        } else {
+            f.v[0] = (uint32_t)q[0] | (uint32_t)q[1] << 16;
+            f.v[1] = (uint32_t)q[2] | (uint32_t)q[3] << 16;
+        }
+        return f;
     };
     // Everything that does not wait for something else first: the first logits, the row's numbers, the first tokens of its history
-    uint4 ahead[kRuleBatch];
+    Four ahead[kRuleBatch] = {};
 #pragma unroll
-    for (int k = 0; k < kRuleBatch; k++) ahead[k] = load((k * kRuleThreads + tid) * 4);
+    for (int k = 0; k < kRuleBatch; k++)
+        if (first_ + k < last_) ahead[k] = load(first_ + k);
     const int32_t* const tokens = HIST ? p.r.tokens + (size_t)row * p.r.ld_tokens : nullptr;
     uint32_t look[kRuleLook];
     if (HIST) {
@@ -175,17 +185,21 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
     const uint32_t my_token = mine >= 0 ? list.key[mine] & 0xFFFFu : 0;
     const float my_logit = mine >= 0 ? load1(my_token) : 0.f;
     const uint32_t* const mask = m >= 0 && m < p.r.masks ? p.r.mask + (size_t)m * p.r.ld_mask : nullptr;
-    uint32_t bits[kRuleBatch];
-    auto allowed = [&](int i) {
-        if (mask == nullptr || i >= n) return 15u;
-        const int t = lo + i, at = t & 31;
-        if (t < 0) return mask[0] << -t & 15u;
-        uint32_t four = mask[t >> 5] >> at;
-        if (VEC && at > 28 && (t | 31) + 1 < p.vocab) four |= mask[(t >> 5) + 1] << (32 - at);
-        return four & 15u;
+    // the bits of a whole group: a turn is 64 words on, and the place in a word stays
+    const int mask_at = (lo + 4 * tid) & 31;
+    const uint32_t* const mask_word = mask + ((lo + 4 * tid) >> 5);
+    auto allowed = [&](int turn) {
+        const uint32_t* const q = mask_word + turn * (kStep / 32);
+        uint32_t four = q[0] >> mask_at;
+        if (VEC && mask_at > 28) four |= q[1] << (32 - mask_at);
+        return four;
     };
+    uint32_t bits[kRuleBatch] = {};
+    if (mask != nullptr) {
 #pragma unroll
-    for (int k = 0; k < kRuleBatch; k++) bits[k] = allowed((k * kRuleThreads + tid) * 4);
+        for (int k = 0; k < kRuleBatch; k++)
+            if (first_ + k < last_) bits[k] = allowed(first_ + k);
+    }
     const bool counts = HIST && len > 0 && (rep != 1.f || pres != 0.f || freq != 0.f);
     if (counts) {
         const int prompt = min(max(said, 0), len);
@@ -230,37 +244,6 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
         l = __fsub_rn(l, __fmul_rn(freq, (float)times));
         return times != 0 ? __fsub_rn(l, pres) : l;
     };
-    auto finish = [&](int i, const uint4& f, uint32_t may) {
-        if (i >= n) return;
-        float v[4];
-        if (p.x_dtype == kF32) {
-            v[0] = __uint_as_float(f.x); v[1] = __uint_as_float(f.y); v[2] = __uint_as_float(f.z); v[3] = __uint_as_float(f.w);
-        } else if (p.x_dtype == kBF16) {
-            v[0] = __uint_as_float(f.x << 16); v[1] = __uint_as_float(f.x & 0xFFFF0000u); v[2] = __uint_as_float(f.y << 16); v[3] = __uint_as_float(f.y & 0xFFFF0000u);
-        } else {
-            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&f.x)), b = __half22float2(*reinterpret_cast<const __half2*>(&f.y));
-            v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
-        }
-        if (HIST && counts) {
-            const uint4 c = Count::four(count, i);
-            if ((c.x | c.y | c.z | c.w) != 0) {
-                v[0] = one(v[0], c.x);
-                v[1] = one(v[1], c.y);
-                v[2] = one(v[2], c.z);
-                v[3] = one(v[3], c.w);
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (!(may >> j & 1)) v[j] = -INFINITY;
-        if (VEC && i + 4 <= n && lo + i >= 0) {
-            *reinterpret_cast<float4*>(out + lo + i) = make_float4(v[0], v[1], v[2], v[3]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-                if (i + j < n && lo + i + j >= 0) out[lo + i + j] = v[j];
-        }
-    };
     // a list's entry: whether no earlier one is of its token, and whether it is the only one
     auto first = [&](int at, bool& only) {
         const uint32_t key = list.key[at];
@@ -273,7 +256,7 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
         }
         return yes;
     };
-    auto may1 = [&](uint32_t t) { return mask == nullptr || (mask[(lo + t) >> 5] >> ((lo + t) & 31) & 1); };
+    auto may1 = [&](uint32_t t) { return mask == nullptr || (mask[(lo + (int)t) >> 5] >> ((lo + (int)t) & 31) & 1); };
     float my_result = 0.f;
     bool store = false;
     if (mine >= 0) {
@@ -285,21 +268,65 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
             if (!may1(my_token)) my_result = -INFINITY;
         }
     }
-    constexpr int kTurn = 4 * kRuleThreads * kRuleBatch;
-    for (int i0 = tid * 4; i0 < n; i0 += kTurn) {
+    auto finish = [&](int turn, const Four& f, uint32_t may) {
+        const int i = 4 * tid + turn * kStep;
+        float v[4];
+        if (DT == kF32) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[j] = __uint_as_float(f.v[DT == kF32 ? j : 0]);
+        } else if (DT == kBF16) {
+            v[0] = __uint_as_float(f.v[0] << 16); v[1] = __uint_as_float(f.v[0] & 0xFFFF0000u); v[2] = __uint_as_float(f.v[1] << 16); v[3] = __uint_as_float(f.v[1] & 0xFFFF0000u);
+        } else {
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&f.v[0])), b = __half22float2(*reinterpret_cast<const __half2*>(&f.v[1]));
+            v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+        }
+        if (HIST && counts) {
+            if (Count::any(count, i)) {
+                const uint4 c = Count::four(count, i);
+                v[0] = one(v[0], c.x);
+                v[1] = one(v[1], c.y);
+                v[2] = one(v[2], c.z);
+                v[3] = one(v[3], c.w);
+            }
+        }
+        if (mask != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                if (!(may >> j & 1)) v[j] = -INFINITY;
+        }
+        if (VEC) {
+            *reinterpret_cast<float4*>(out + i) = make_float4(v[0], v[1], v[2], v[3]);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) out[i + j] = v[j];
+        }
+    };
+    for (int turn = first_; turn < last_; turn += kRuleBatch) {
 #pragma unroll
         for (int k = 0; k < kRuleBatch; k++) {
-            const int i = i0 + k * kRuleThreads * 4;
-            const uint4 f = ahead[k];
+            const Four f = ahead[k];
             const uint32_t may = bits[k];
-            ahead[k] = load(i + kTurn);
-            bits[k] = allowed(i + kTurn);
-            finish(i, f, may);
+            if (turn + k + kRuleBatch < last_) {
+                ahead[k] = load(turn + k + kRuleBatch);
+                if (mask != nullptr) bits[k] = allowed(turn + k + kRuleBatch);
+            }
+            if (turn + k < last_) finish(turn + k, f, may);
         }
     }
+    auto single = [&](int i) {
+        if (i >= n || lo + i < 0) return;
+        float v = load1(i);
+        if (HIST && counts) v = one(v, Count::one(count, i));
+        out[i] = may1(i) ? v : -INFINITY;
+    };
+    if (first_ == 1)
+        for (int j = 0; j < 4; j++) single(4 * tid + j);
+    const int end = 4 * tid + last_ * kStep;
+    if (last_ >= first_ && end < n)
+        for (int j = 0; j < 4; j++) single(end + j);
     if (b0 < b1) {
         __syncthreads();
-        if (store) out[lo + my_token] = my_result;
+        if (store) out[my_token] = my_result;
     }
     // more biases than the list takes at once: by rounds
     for (int j0 = b0 + kRuleThreads; j0 < b1; j0 += kRuleThreads) {
@@ -311,22 +338,31 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
         bool only;
         if (at >= 0 && first(at, only)) {
             const uint32_t t = list.key[at] & 0xFFFFu;
-            if (may1(t)) out[lo + t] = list.add(out[lo + t], t);
+            if (may1(t)) out[t] = list.add(out[t], t);
         }
     }
 }
 
-template <bool HIST, bool WIDE>
-void (*rules_pick(bool vec))(RuleParams) { return vec ? logit_rules_kernel<HIST, WIDE, true> : logit_rules_kernel<HIST, WIDE, false>; }
+typedef void (*RulesKernel)(RuleParams);
+template <int DT>
+RulesKernel rules_pick(bool hist, bool wide, bool vec) {
+    if (!hist) return vec ? logit_rules_kernel<DT, false, false, true> : logit_rules_kernel<DT, false, false, false>;
+    if (wide) return vec ? logit_rules_kernel<DT, true, true, true> : logit_rules_kernel<DT, true, true, false>;
+    return vec ? logit_rules_kernel<DT, true, false, true> : logit_rules_kernel<DT, true, false, false>;
+}
+RulesKernel rules_pick(int dtype, bool hist, bool wide, bool vec) {
+    return dtype == kF32 ? rules_pick<kF32>(hist, wide, vec) : dtype == kF16 ? rules_pick<kF16>(hist, wide, vec) : rules_pick<kBF16>(hist, wide, vec);
+}
 
 }  // namespace
 
 int32_t rules_init(iq_ctx* ctx) {
-    for (int vec = 0; vec < 2; vec++) {
-        cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(rules_pick<true, true>(vec != 0)), cudaFuncAttributeMaxDynamicSharedMemorySize, kRuleSpan * 4);
-        if (e == cudaSuccess) e = cudaFuncSetAttribute(reinterpret_cast<const void*>(rules_pick<true, false>(vec != 0)), cudaFuncAttributeMaxDynamicSharedMemorySize, kRuleSpan * 2);
-        if (e != cudaSuccess) return check_cuda(ctx, e, "cudaFuncSetAttribute(logit_rules)");
-    }
+    for (int dtype = 0; dtype < 3; dtype++)
+        for (int kind = 0; kind < 4; kind++) {
+            const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(rules_pick(dtype, true, (kind & 1) != 0, (kind & 2) != 0)),
+                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kRuleSpan * (kind & 1 ? 4 : 2));
+            if (e != cudaSuccess) return check_cuda(ctx, e, "cudaFuncSetAttribute(logit_rules)");
+        }
     return kOk;
 }
 
@@ -364,7 +400,7 @@ extern "C" int32_t iq_logits_rules(iq_ctx* ctx, void* stream, const void* x, int
     p.misplaced = (uint32_t)(reinterpret_cast<uintptr_t>(out) / 4 & 3);
     const bool vec = reinterpret_cast<uintptr_t>(x) % esz == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0 &&
                      (reinterpret_cast<uintptr_t>(x) / esz & 3) == p.misplaced && ((ldx ^ ldo) & 3) == 0;
-    auto kernel = !hist ? rules_pick<false, false>(vec) : wide ? rules_pick<true, true>(vec) : rules_pick<true, false>(vec);
+    const RulesKernel kernel = rules_pick(x_dtype, hist, wide, vec);
     DeviceScope on(ctx);
     if (on.error != cudaSuccess) return check_cuda(ctx, on.error, "logits_rules device");
     return check_cuda(ctx, launch_dependent(kernel, dim3((unsigned)rows * p.parts), kRuleThreads, hist ? (size_t)p.span * (wide ? 4 : 2) : 0, reinterpret_cast<cudaStream_t>(stream), p),
