@@ -207,7 +207,9 @@ int32_t iq_qmm_i8(iq_ctx* ctx, void* stream, const int8_t* x, int64_t ldx, const
                   int32_t n, int32_t k, void* y, int32_t y_dtype, int64_t ldy, int32_t rows, uint32_t flags);
 /* How iq_qmm_i8 divides a call among the SMs of a GPU. Needs no GPU and no context. For tests that have to know which path a shape takes. */
 typedef struct iq_qmm_i8_tiling {
-    int32_t tile_rows; /* tokens per tile */
+    int32_t tile_rows; /* tokens per tile, */
+    int32_t tall;      /* of the first `tall` of the */
+    int32_t row_tiles; /* tiles over the rows; with pairs the others have 32 fewer */
     int32_t pair;      /* 1: a tile of 256 features on two CTAs; 0: of 128 on a cluster */
     int32_t parts;     /* CTAs of the cluster, which divide k */
     int64_t tiles;

@@ -53,7 +53,7 @@ class QmvTiling(C.Structure):
 
 
 class QmmI8Tiling(C.Structure):
-    _fields_ = [("tile_rows", C.c_int32), ("pair", C.c_int32), ("parts", C.c_int32), ("tiles", C.c_int64)]
+    _fields_ = [("tile_rows", C.c_int32), ("tall", C.c_int32), ("row_tiles", C.c_int32), ("pair", C.c_int32), ("parts", C.c_int32), ("tiles", C.c_int64)]
 
 
 class LogitRules(C.Structure):

@@ -34,7 +34,7 @@ struct I8Params {
     int32_t y_dtype, accumulate, whole;  // whole: four neighbouring elements of y lie on their own size
     int32_t M, N, K;
     int32_t m_tiles, steps;  // tiles of tokens; steps of 128 inputs
-    int32_t tile_rows;       // pairs: tokens of a tile
+    int32_t tile_rows, tall;  // pairs: tokens of the first `tall` of the tiles over the rows; the others have 32 fewer
     int32_t* status;
 };
 
@@ -347,14 +347,16 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
     pdl_launch_dependents();
     const int total = p.m_tiles * ((p.N + 255) / 256), first = blockIdx.x / 2, stride = gridDim.x / 2;
     const uint32_t bytes = 128 * 128 + p.tile_rows * 64;  // of a CTA and stage
-    // tokens of a tile's MMAs: whole groups of 32, half of them in each CTA
-    auto tokens = [&](int row0) { return (min(p.tile_rows, p.M - row0) + 31) & ~31; };
+    // tile m over the rows: its first row, its rows, and the tokens of its MMAs: whole groups of 32, half of them in each CTA
+    auto first_row = [&](int m) { return m * p.tile_rows - 32 * max(m - p.tall, 0); };
+    auto tile_rows = [&](int m) { return min(p.tile_rows - (m < p.tall ? 0 : 32), p.M - first_row(m)); };
+    auto tokens = [&](int m) { return (tile_rows(m) + 31) & ~31; };
     if (warp == 0) {
         if (elect_one()) {
             auto corner = [&](int i, int& xrow, int& n0) {
-                const int row0 = (i % p.m_tiles) * p.tile_rows;
+                const int m = i % p.m_tiles;
                 n0 = (i / p.m_tiles) * 256 + 128 * (int)rank;
-                xrow = row0 + (int)rank * (tokens(row0) / 2);
+                xrow = first_row(m) + (int)rank * (tokens(m) / 2);
             };
             // the first stages' weights ahead of the wait for the kernel before
             int xrow, n0;
@@ -387,7 +389,7 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
             uint32_t ph = 0, tph = 0;
             bool ok = true;
             for (int i = first; i < total && ok; i += stride) {
-                const uint32_t idesc = i8_idesc(tokens((i % p.m_tiles) * p.tile_rows)) + (8u << 24);  // M = 256
+                const uint32_t idesc = i8_idesc(tokens(i % p.m_tiles)) + (8u << 24);  // M = 256
                 if (!(ok = mbar_wait(tempty + 8 * a, tph ^ 1, abort_flag))) break;
                 tc_fence_after();
                 const uint32_t acc = tmem + a * 256;
@@ -412,7 +414,7 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
         int a = 0;
         uint32_t tph = 0;
         for (int i = first; i < total; i += stride) {
-            const int row0 = (i % p.m_tiles) * p.tile_rows, rows = min(p.tile_rows, p.M - row0), n = (i / p.m_tiles) * 256 + 128 * (int)rank + 32 * q + lane;
+            const int row0 = first_row(i % p.m_tiles), rows = tile_rows(i % p.m_tiles), n = (i / p.m_tiles) * 256 + 128 * (int)rank + 32 * q + lane;
             const float sw = n < p.N ? p.sw[n] : 0.f;
             float sx[4];  // of the warp's (up to) four times 32 tokens
 #pragma unroll
@@ -473,10 +475,12 @@ const I8Entry kI8[] = {i8_entry<16>(), i8_entry<32>(), i8_entry<64>()};
 // How a call is divided. Up to 128 rows clusters, which hide the weights' way from memory; beyond the cheaper of the two by estimates in ns: a
 // step of a pair on h tokens takes 200 + 0.72 h, of a cluster's CTA on 64 tokens (two per SM) 330, the start and the last tile's results 4000 +
 // 8 h and 5000. Measured / estimated, us: 256 x 4096 x 4096 clusters 12.3 / 10.3, pairs 12.5 / 12.4; 256 x 14336 x 4096 27.7 / 26.1, 22.1 / 18.3; 256 x 4096 x
-// 14336 25.1 / 23.5, 30.7 / 32.1; 512 x 4096 x 4096 clusters 15.6 (estimated), pairs 14.4 / 14.3.
+// 14336 25.1 / 23.5, 30.7 / 32.1; 512 x 4096 x 4096 clusters 15.6 (estimated), pairs 14.4 / 14.3. The pairs' tiles over the rows are of two heights, 32
+// apart, so that any number of them can be had: sixteen times nine fill 74 pairs twice, sixteen times eight (of 256 tokens) did so to 86 %.
 struct I8Plan {
     bool pair;
-    int rows;  // tokens of a tile
+    int rows, tall;  // tokens of a tile; pairs: of the first `tall` over the rows, the others have 32 fewer
+    int m_tiles;
     int64_t tiles;
     int parts;  // pieces of k, the CTAs of a cluster
 };
@@ -485,19 +489,24 @@ I8Plan i8_plan(int rows, int n, int k, int sms) {
     I8Plan c;
     c.pair = false;
     c.rows = rows <= 16 ? 16 : rows <= 32 ? 32 : 64;
-    c.tiles = (int64_t)((rows + c.rows - 1) / c.rows) * ((n + 127) / 128);
+    c.m_tiles = (rows + c.rows - 1) / c.rows;
+    c.tall = c.m_tiles;
+    c.tiles = (int64_t)c.m_tiles * ((n + 127) / 128);
     c.parts = 1;
     // (a division costs about 1 us: 37 x 1024 x 1024, eight steps, 4.2 us whole and 4.8 in four; 23 steps of 37 x 2880 x 2880 8.4 and 6.4)
     while (steps > 8 && c.parts < 8 && c.tiles * c.parts <= sms && steps >= 4 * c.parts) c.parts *= 2;
     if (rows <= 128 || sms % 2 != 0) return c;
     int64_t least = (c.tiles * c.parts + 2 * sms - 1) / (2 * sms) * (steps / c.parts) * 330 + 5000;
-    for (int h = 256; h >= 64; h -= 32) {
-        const int64_t tiles = (int64_t)((rows + h - 1) / h) * ((n + 255) / 256);
-        const int64_t cost = (tiles + sms / 2 - 1) / (sms / 2) * steps * (20000 + 72 * h) / 100 + 4000 + 8 * h;
+    const int n_tiles = (n + 255) / 256, groups = (rows + 31) / 32;
+    for (int m = (groups + 7) / 8; m <= (groups + 1) / 2; m++) {
+        const int high = (groups + m - 1) / m;  // groups of 32 tokens
+        const int64_t rounds = ((int64_t)m * n_tiles + sms / 2 - 1) / (sms / 2), h = rows / m;
+        const int64_t cost = rounds * steps * (20000 + 72 * h) / 100 + 4000 + 8 * h;
         if (cost < least) {
             least = cost;
-            c = I8Plan{true, h, tiles, 1};
+            c = I8Plan{true, 32 * high, groups - m * (high - 1), m, (int64_t)m * n_tiles, 1};
         }
+        if (rounds > 64) break;  // (finer tiles only cost)
     }
     return c;
 }
@@ -521,6 +530,8 @@ extern "C" int32_t iq_qmm_i8_plan(int32_t rows, int32_t n, int32_t k, int32_t sm
     if (out == nullptr || rows < 1 || n < 1 || k < 16 || k % 16 != 0 || k > kI8MaxK || sms < 1) return kErrInvalidArg;
     const I8Plan p = i8_plan(rows, n, k, sms);
     out->tile_rows = p.rows;
+    out->tall = p.tall;
+    out->row_tiles = p.m_tiles;
     out->pair = p.pair ? 1 : 0;
     out->parts = p.parts;
     out->tiles = p.tiles;
@@ -547,7 +558,7 @@ extern "C" int32_t iq_qmm_i8(iq_ctx* ctx, void* stream, const int8_t* x, int64_t
     p.accumulate = flags & IQ_FLAG_ACCUMULATE ? 1 : 0;
     p.whole = ldy % 4 == 0 && reinterpret_cast<uintptr_t>(y) % (4 * dtype_size(y_dtype)) == 0;
     p.M = rows; p.N = n; p.K = k;
-    p.tile_rows = plan.rows; p.m_tiles = (rows + plan.rows - 1) / plan.rows; p.steps = (k + 127) / 128;
+    p.tile_rows = plan.rows; p.tall = plan.tall; p.m_tiles = plan.m_tiles; p.steps = (k + 127) / 128;
     p.status = ctx->d_status;
     DeviceScope on(ctx);
     if (on.error != cudaSuccess) return check_cuda(ctx, on.error, "qmm_i8 device");

@@ -67,13 +67,14 @@ def test_many_tiles(cuda_device, rows, n, k):
     run(torch.Generator().manual_seed(rows), rows, n, k, BF16)
 
 
-@pytest.mark.parametrize("rows,n,k,height", [(221, 1280, 256, 64), (1174, 1280, 1040, 96), (680, 9472, 256, 128), (1954, 2560, 384, 160), (1971, 4730, 1040, 192),
-                                                (2160, 9472, 384, 224), (246, 18944, 1040, 256)])
+@pytest.mark.parametrize("rows,n,k,height,tall", [(429, 4730, 384, 64, 7), (221, 1280, 256, 64, 3), (180, 18944, 384, 96, 2), (1174, 1280, 1040, 96, 9), (625, 14336, 528, 128, 5),
+                                                  (680, 9472, 256, 128, 4), (470, 18944, 256, 160, 3), (1954, 2560, 384, 160, 6), (173, 18944, 528, 192, 1), (1971, 4730, 1040, 192, 7),
+                                                  (870, 18944, 256, 224, 4), (2160, 9472, 384, 224, 8), (246, 18944, 1040, 256, 1), (1902, 9472, 256, 256, 4)])
 @pytest.mark.parametrize("dtype,accumulate", [(F32, True), (F16, False)])
-def test_pairs(cuda_device, rows, n, k, height, dtype, accumulate):
-    """Pairs of CTAs on tiles of every height, the last of them short, more than one tile per pair."""
+def test_pairs(cuda_device, rows, n, k, height, tall, dtype, accumulate):
+    """Pairs of CTAs on tiles of every height, of one and of two heights, the last of them short, more than one tile per pair."""
     plan = capi.qmm_i8_plan(rows, n, k)
-    assert plan.pair == 1 and plan.tile_rows == height
+    assert plan.pair == 1 and plan.tile_rows == height and plan.tall == tall
     run(torch.Generator().manual_seed(rows), rows, n, k, dtype, accumulate, 1)
 
 
