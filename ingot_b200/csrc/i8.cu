@@ -312,6 +312,10 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
 
 // Persistent; two accumulators in tensor memory, so that a tile's results leave beside the next tile's products. The even CTA issues the
 // MMAs for both; each copies its 128 features and its half of the tokens and stores its 128 features' results.
+//
+// Bound: operands on their way from L2 (a step of 128 inputs moves 16 KB + 64 bytes per token and SM, at some 46 bytes per cycle: 0.36 us on 256 tokens,
+// the MMAs alone 0.27) and power. 2048 x 4096 x 14336 79 to 98 us, 2048 x 14336 x 4096 82, 4096 x 14336 x 4096 156 (3080 TOP/s). Measured and taken
+// back: 512 tokens per pair as two MMAs on the same features (the step 11 % shorter per token, but no room for a second accumulator: 84 us against 79).
 __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
     i8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const I8Params p) {
     extern __shared__ unsigned char smem_raw[];
@@ -410,32 +414,35 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
         }
     } else {
         pdl_wait();
+        // Two times four warps take sixteen tokens in turn. (Thirty-two at once spill: 2048 x 4096 x 4096 30.7 us against 27.7, 2048 x 1024 x 1024 8.8 against 7.1.)
+        constexpr int C = 16;
         const int q = warp & 3, half = (warp - 2) >> 2;
         int a = 0;
         uint32_t tph = 0;
         for (int i = first; i < total; i += stride) {
-            const int row0 = first_row(i % p.m_tiles), rows = tile_rows(i % p.m_tiles), n = (i / p.m_tiles) * 256 + 128 * (int)rank + 32 * q + lane;
+            const int row0 = first_row(i % p.m_tiles) + C * half, rows = tile_rows(i % p.m_tiles) - C * half;  // from the warp's first token on
+            const int n = (i / p.m_tiles) * 256 + 128 * (int)rank + 32 * q + lane;
             const float sw = n < p.N ? p.sw[n] : 0.f;
-            float sx[4];  // of the warp's (up to) four times 32 tokens
-#pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int t = 64 * c + 32 * half + lane;
-                sx[c] = t < rows ? p.sx[row0 + t] : 0.f;
-            }
+            auto scale = [&](int c0) { return lane < C && c0 + lane < rows ? p.sx[row0 + c0 + lane] : 0.f; };
+            float sx = scale(0);
             if (!__all_sync(0xffffffffu, mbar_wait(tfull + 8 * a, tph, abort_flag))) break;
             tc_fence_after();
-            const uint32_t t0 = tmem + ((uint32_t)(32 * q) << 16) + a * 256 + 32 * half;
-            uint32_t r[2][32];  // the next columns are under way while these are stored
-            if (32 * half < rows) tmem_ld(t0, r[0]);
+            const uint32_t t0 = tmem + ((uint32_t)(32 * q) << 16) + a * 256 + C * half;
+            uint32_t r[2][C];  // the next columns are under way while these are stored
+            if (rows > 0) tmem_ld(t0, r[0]);
+#pragma unroll 1
+            for (int c2 = 0; c2 < rows; c2 += 4 * C) {
 #pragma unroll
-            for (int c = 0; c < 4; c++) {
-                const int c0 = 64 * c + 32 * half;
-                if (c0 < rows) {
+                for (int c1 = 0; c1 < 2; c1++) {
+                    const int c0 = c2 + 2 * C * c1;
+                    if (c0 >= rows) break;
+                    const float next = scale(c0 + 2 * C);
                     tmem_ld_wait();
-                    if (c < 3 && c0 + 64 < rows) tmem_ld(t0 + 64 * (c + 1), r[(c + 1) & 1]);
-                    if (p.y_dtype == kF32) i8_store<kF32, 32>(p, r[c & 1], sx[c], sw, row0 + c0, n, rows - c0);
-                    else if (p.y_dtype == kBF16) i8_store<kBF16, 32>(p, r[c & 1], sx[c], sw, row0 + c0, n, rows - c0);
-                    else i8_store<kF16, 32>(p, r[c & 1], sx[c], sw, row0 + c0, n, rows - c0);
+                    if (c0 + 2 * C < rows) tmem_ld(t0 + c0 + 2 * C, r[c1 ^ 1]);
+                    if (p.y_dtype == kF32) i8_store<kF32, C>(p, r[c1], sx, sw, row0 + c0, n, rows - c0);
+                    else if (p.y_dtype == kBF16) i8_store<kBF16, C>(p, r[c1], sx, sw, row0 + c0, n, rows - c0);
+                    else i8_store<kF16, C>(p, r[c1], sx, sw, row0 + c0, n, rows - c0);
+                    sx = next;
                 }
             }
             tc_fence_before();
