@@ -89,7 +89,6 @@ __device__ __forceinline__ void i8_store(const I8Params& p, const uint32_t (&r)[
             if (j < live) y_store(y, DT, (size_t)j * p.ldy, v[j]);
     }
 }
-__device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[32]) { tmem_ld32(taddr, r); }
 __device__ __forceinline__ void tmem_ld(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
                  : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
@@ -226,7 +225,7 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
         pdl_wait();
         const int q = warp & 3;  // the quarter of tensor memory that this warp may read
         const uint32_t t0 = tmem + ((uint32_t)(32 * q) << 16);
-        constexpr int C = BN < 32 ? BN : 32;
+        constexpr int C = 16;
         if (parts > 1 && u0 + (int)threadIdx.x < u1) unit_scales(u0 + (int)threadIdx.x);
         const int n = n0 + 32 * q + lane;
         const float sw = n < p.N ? p.sw[n] : 0.f, sx0 = lane < rows ? p.sx[row0 + lane] : 0.f, sx1 = 32 + lane < rows ? p.sx[row0 + 32 + lane] : 0.f;
