@@ -200,13 +200,8 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
     pdl_launch_dependents();
     __shared__ __align__(16) float turn[VEC || ROT == 1 ? 1 : MAXT * 8];  // a warp's 256 values on their way to eight in a row per thread, and back
     auto at = [&](int c, int j) { return (c * (int)blockDim.x + warp * 32) * 8 + (VEC ? lane * 8 + j : j * 32 + lane); };
+    pdl_wait();  // (the weight, too, may be what the kernel before has written: a norm's may depend on the input)
     Raw8 rw[VEC ? NCH : 1];
-    if (VEC && p.w != nullptr) {  // (weights may be read ahead of the wait)
-#pragma unroll
-        for (int c = 0; c < NCH; c++)
-            if (at(c, 0) < p.d) rw[VEC ? c : 0] = load8(p.w, p.w_dtype, at(c, 0));
-    }
-    pdl_wait();
     float v[NCH][8];  // r'
     if (VEC) {
         Raw8 rr[NCH], xx[NCH];
@@ -215,6 +210,7 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
             if (at(c, 0) < p.d) {
                 rr[c] = load8(p.r, p.r_dtype, row * p.ldr + at(c, 0));
                 if (p.x != nullptr) xx[c] = load8(p.x, p.x_dtype, row * p.ldx + at(c, 0));
+                if (p.w != nullptr) rw[VEC ? c : 0] = load8(p.w, p.w_dtype, at(c, 0));
             }
 #pragma unroll
         for (int c = 0; c < NCH; c++) {
@@ -398,17 +394,6 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const __grid_con
     const int block = warp * 256 * K + (lane / LB) * 256, first = block + (lane % LB) * 8;  // the lanes' 256 values, the lane's first one
     const bool live[K] = {first < p.d, first + APART < p.d};
     pdl_launch_dependents();
-    float w[K][8];
-#pragma unroll
-    for (int k = 0; k < K; k++) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) w[k][j] = 1.f;
-        if (p.w != nullptr && live[k]) {  // (weights may be read ahead of the wait)
-            unpack8<HT>(load8(p.w, p.w_dtype, first + APART * k), p.w_dtype, w[k]);
-#pragma unroll
-            for (int j = 0; j < 8; j++) w[k][j] = __fadd_rn(w[k][j], p.offset);
-        }
-    }
     // Everything that a row's addresses are made of, once
     const int32_t r_dtype = TYPES == kAnyTypes ? p.r_dtype : TYPES == kSum32 ? kF32 : HT, x_dtype = TYPES == kAnyTypes ? p.x_dtype : HT;
     const int32_t out_dtype = TYPES == kAnyTypes ? p.out_dtype : HT;
@@ -464,6 +449,17 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const __grid_con
     copy(r, wide_r, r.to);  // (there are no more blocks than rows)
     if (add) copy(x, wide_x, x.to);
     asm volatile("cp.async.commit_group;" ::: "memory");
+    float w[K][8];
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+#pragma unroll
+        for (int j = 0; j < 8; j++) w[k][j] = 1.f;
+        if (p.w != nullptr && live[k]) {
+            unpack8<HT>(load8(p.w, p.w_dtype, first + APART * k), p.w_dtype, w[k]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[k][j] = __fadd_rn(w[k][j], p.offset);
+        }
+    }
     int turn = 0;
     for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x) {
         // the next row, into the stage of the row before: a barrier has passed since it was read
@@ -598,6 +594,7 @@ NormKernel norm_pick(bool vec, int half, bool codes, int rotate) {
                                                                                           : norm_pick<NCH, MAXT, true, kF32>(codes, rotate);
 }
 
+bool misplaced(const void* p, int esz) { return reinterpret_cast<uintptr_t>(p) % esz != 0; }
 bool known(int32_t dtype) { return dtype >= 0 && dtype <= 2; }
 // whether every group of eight of the rows lies on its own size
 bool aligned(const void* p, int64_t ld, int esz) {
@@ -636,6 +633,9 @@ extern "C" int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int3
     if (out != nullptr && (!known(out_dtype) || ldo < d)) return fail(ctx, kErrInvalidArg, "add_rmsnorm: out of fp32, fp16 or bf16, rows at least d apart");
     if (codes != nullptr ? scales == nullptr || ldc < d : scales != nullptr)
         return fail(ctx, kErrInvalidArg, "add_rmsnorm: codes come with scales, rows at least d apart");
+    if (misplaced(residual, dtype_size(r_dtype)) || misplaced(residual_out, dtype_size(r_dtype)) || (x != nullptr && misplaced(x, dtype_size(x_dtype))) ||
+        (weight != nullptr && misplaced(weight, dtype_size(w_dtype))) || (out != nullptr && misplaced(out, dtype_size(out_dtype))) || misplaced(scales, 4))
+        return fail(ctx, kErrInvalidArg, "add_rmsnorm: a tensor does not begin on an element");
     if (rotate != 0 && rotate != 32 && rotate != 256) return fail(ctx, kErrUnsupported, "add_rmsnorm: rotation in blocks of %d (0, 32 or 256)", rotate);
     if (rotate != 0 && (codes == nullptr || d % rotate != 0))
         return fail(ctx, kErrInvalidArg, "add_rmsnorm: the rotation is the codes', d = %d a multiple of its blocks of %d", d, rotate);

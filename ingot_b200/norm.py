@@ -102,6 +102,8 @@ def add_rmsnorm(x: Optional[torch.Tensor], residual: torch.Tensor, weight: Optio
         if residual.device.type != "cuda":
             _no_cpu()
         raise ValueError("add_rmsnorm does not take these tensors")
+    if rows == 0:  # (tensors of no rows have no address)
+        return
     ctx = capi.context(dev)
     if rows <= 1:  # (one row has no stride)
         ldx = ldr = ldro = ldo = ldc = d

@@ -266,3 +266,45 @@ def test_many_rows_in_place_and_poisoned(cuda_device):
     keep = [t for t in range(rows) if t not in (700, 701)]
     want, _ = qref.norm_codes(total[keep].float().numpy(), np.ones(d, np.float32), 256)
     assert np.array_equal(codes[keep].cpu().numpy(), want)
+
+
+def test_a_weight_that_the_launch_before_wrote(cuda_device):
+    """Launches start before their predecessors have ended; what those write is waited for, the weight too. Both kernels."""
+    gen = torch.Generator().manual_seed(11)
+    for rows, d in ((1, 2048), (1500, 2048)):
+        r = torch.randn(rows, d, generator=gen).to(BF16).cuda()
+        parts = [torch.randn(1, d, generator=gen).to(BF16).cuda() for _ in range(20)]
+        w, out = torch.zeros(1, d, dtype=BF16, device="cuda"), torch.empty(20, rows, d, dtype=BF16, device="cuda")
+        for i, part in enumerate(parts):
+            add_rmsnorm(None, part, None, 1, out=w)
+            add_rmsnorm(None, r, w[0], rows, out=out[i])
+        for i, part in enumerate(parts):
+            add_rmsnorm(None, part, None, 1, out=w)
+            torch.cuda.synchronize()
+            want = torch.empty_like(r)
+            add_rmsnorm(None, r, w[0].clone(), rows, out=want)
+            assert torch.equal(out[i], want)
+
+
+def test_two_streams_at_once(cuda_device):
+    gen = torch.Generator().manual_seed(12)
+    r = torch.randn(700, 2880, generator=gen).to(BF16).cuda()
+    def call(stream=None):
+        out, codes, scales = torch.empty_like(r), torch.empty(700, 2880, dtype=torch.int8, device="cuda"), torch.empty(700, device="cuda")
+        return (out, codes, scales), lambda: add_rmsnorm(None, r, None, 700, out=out, codes=codes, scales=scales, rotate=32, stream=stream)
+    want, go = call()
+    go()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    calls = [call(s) for s in streams]
+    for _ in range(10):
+        for _, go in calls:
+            go()
+    torch.cuda.synchronize()
+    for got, _ in calls:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_tensors_of_no_rows(cuda_device):
+    none = torch.empty(0, 64, device="cuda")
+    add_rmsnorm(none, none, None, 0, out=none, codes=torch.empty(0, 64, dtype=torch.int8, device="cuda"), scales=torch.empty(0, device="cuda"))

@@ -56,3 +56,21 @@ def test_c_entry_refuses(change, status):
          "ldo": 64, "codes": 0, "ldc": 0, "scales": 0, "rot": 0}
     a.update(change)
     assert capi.lib().iq_add_rmsnorm(None, None, *a.values()) == status  # (with nothing wrong: there is no context)
+
+
+@pytest.mark.parametrize("change", [{"x": P + 2}, {"r": P + 1, "rd": 1}, {"ro": P + 2}, {"w": P + 2}, {"w": P + 1, "wd": 2}, {"out": P + 3}, {"codes": P, "scales": P + 2, "ldc": 64}])
+def test_tensors_begin_on_an_element(change):
+    a = {"x": P, "xd": 0, "ldx": 64, "r": P, "rd": 0, "ldr": 64, "ro": P, "ldro": 64, "w": P, "wd": 0, "off": 0.0, "eps": 1e-6, "rows": 4, "d": 64, "out": P, "od": 0,
+         "ldo": 64, "codes": 0, "ldc": 0, "scales": 0, "rot": 0}
+    a.update(change)
+    call = lambda: capi.lib().iq_add_rmsnorm(None, None, *a.values())
+    a["rot"] = 64  # (refused with another status, and later)
+    assert call() == -1
+    a.update({k: v & ~3 for k, v in a.items() if k in change and k not in ("rd", "wd", "ldc")})
+    assert call() == -2
+
+
+def test_no_rows_are_no_addresses():
+    none = torch.zeros(0, 64)
+    with pytest.raises(ValueError, match="CUDA"):  # (nothing but the device is wrong)
+        add_rmsnorm(none, none, None, 0, out=none)
