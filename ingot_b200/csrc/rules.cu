@@ -375,8 +375,14 @@ extern "C" int32_t iq_logits_rules(iq_ctx* ctx, void* stream, const void* x, int
     // (the checks come before the context is looked at: they are the same without a GPU)
     if (x == nullptr || out == nullptr || rules == nullptr || x_dtype < 0 || x_dtype > 2) return fail(ctx, kErrInvalidArg, "logits_rules: null pointer, or x is not of fp32, fp16 or bf16");
     if (rows < 0 || vocab < 1 || ldx < vocab || ldo < vocab) return fail(ctx, kErrInvalidArg, "logits_rules: rows = %d, vocab = %d, rows at least vocab apart", rows, vocab);
-    if (vocab > kRuleMaxVocab || rows > (1 << 24)) return fail(ctx, kErrUnsupported, "logits_rules: up to %d logits per row", kRuleMaxVocab);
     const iq_logit_rules& r = *rules;
+    const int esz = dtype_size(x_dtype);
+    uintptr_t words = reinterpret_cast<uintptr_t>(out);
+    for (const void* t : {(const void*)r.tokens, (const void*)r.lens, (const void*)r.prompt_lens, (const void*)r.repetition, (const void*)r.presence, (const void*)r.frequency,
+                          (const void*)r.bias_offsets, (const void*)r.bias_tokens, (const void*)r.bias_values, (const void*)r.mask, (const void*)r.mask_rows})
+        words |= reinterpret_cast<uintptr_t>(t);
+    if (words % 4 != 0 || reinterpret_cast<uintptr_t>(x) % esz != 0) return fail(ctx, kErrInvalidArg, "logits_rules: a tensor does not begin on an element");
+    if (vocab > kRuleMaxVocab || rows > (1 << 24)) return fail(ctx, kErrUnsupported, "logits_rules: up to %d logits per row", kRuleMaxVocab);
     if (r.tokens != nullptr && (r.lens == nullptr || r.max_tokens < 0 || r.ld_tokens < r.max_tokens))
         return fail(ctx, kErrInvalidArg, "logits_rules: a history has lengths, its rows at least max_tokens apart");
     if (r.bias_offsets != nullptr && (r.biases < 0 || (r.biases > 0 && (r.bias_tokens == nullptr || r.bias_values == nullptr))))
@@ -396,10 +402,8 @@ extern "C" int32_t iq_logits_rules(iq_ctx* ctx, void* stream, const void* x, int
     p.parts = (vocab + 3 + p.span - 1) / p.span;  // (a row may begin three elements into the first one's)
     const bool hist = r.tokens != nullptr && r.max_tokens > 0 && (r.repetition != nullptr || r.presence != nullptr || r.frequency != nullptr);
     const bool wide = hist && r.max_tokens > 0x7FFF;
-    const int esz = dtype_size(x_dtype);
     p.misplaced = (uint32_t)(reinterpret_cast<uintptr_t>(out) / 4 & 3);
-    const bool vec = reinterpret_cast<uintptr_t>(x) % esz == 0 && reinterpret_cast<uintptr_t>(out) % 4 == 0 &&
-                     (reinterpret_cast<uintptr_t>(x) / esz & 3) == p.misplaced && ((ldx ^ ldo) & 3) == 0;
+    const bool vec = (reinterpret_cast<uintptr_t>(x) / esz & 3) == p.misplaced && ((ldx ^ ldo) & 3) == 0;
     const RulesKernel kernel = rules_pick(x_dtype, hist, wide, vec);
     DeviceScope on(ctx);
     if (on.error != cudaSuccess) return check_cuda(ctx, on.error, "logits_rules device");

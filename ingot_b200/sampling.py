@@ -139,6 +139,8 @@ class LogitRules:
             if not x.is_cuda:
                 _no_cpu()
             raise ValueError("LogitRules does not take these tensors")
+        if rows == 0:  # (tensors of no rows have no address)
+            return out
         if rows <= 1:  # (one row has no stride)
             ldx = ldo = xv
         ctx = capi.context(dev)

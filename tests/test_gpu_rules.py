@@ -249,3 +249,22 @@ def test_the_end_of_a_decode_step(cuda_device):
         assert np.array_equal(idx[t, :len(order)].cpu().numpy(), order) and best[t].item() == order[0]
     ref = qref.add_rmsnorm((x.to(BF16).float() + r).numpy(), w.numpy(), 1e-6)[0]
     assert np.abs(h.double().cpu().numpy() - ref).max() <= np.abs(ref).max() * (2.0**-8 + 2.0**-18)
+
+
+def test_tensors_of_no_rows(cuda_device):
+    assert LogitRules(2, 100).encode(torch.empty(0, 100, device="cuda"), 0).shape == (0, 100)
+
+
+def test_two_streams_at_once(cuda_device):
+    rng = np.random.default_rng(21)
+    rows, V = 5, 30001
+    rules = LogitRules(rows, V, **device(some(rng, rows, V, history=3000, bias=40, masks=3)))
+    x = torch.from_numpy(rng.normal(size=(rows, V)).astype(np.float32)).cuda()
+    want = rules.encode(x, rows)
+    torch.cuda.synchronize()
+    streams, outs = [torch.cuda.Stream(), torch.cuda.Stream()], [torch.empty_like(x) for _ in range(2)]
+    for _ in range(10):
+        for s, o in zip(streams, outs):
+            rules.encode(x, rows, out=o, stream=s)
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)

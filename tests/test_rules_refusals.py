@@ -61,3 +61,15 @@ def test_the_struct_is_the_headers():
     for name, struct in (("iq_logit_rules", capi.LogitRules), ("iq_qmm_i8_tiling", capi.QmmI8Tiling)):
         body = re.sub(r"/\*.*?\*/", "", text[text.index(f"typedef struct {name} {{"):text.index(f"}} {name};")], flags=re.S)
         assert re.findall(r"(\w+);", body) == [f[0] for f in struct._fields_]
+
+
+@pytest.mark.parametrize("call,rules", [({"x": P + 2}, {}), ({"x": P + 1, "xd": 2}, {}), ({"out": P + 2}, {})] + [({}, {name: P + 1}) for name in (
+    "tokens", "lens", "prompt_lens", "repetition", "presence", "frequency", "bias_offsets", "bias_tokens", "bias_values", "mask", "mask_rows")])
+def test_tensors_begin_on_an_element(call, rules):
+    a = {"x": P, "xd": 0, "ldx": 262145, "out": P, "ldo": 262145, "rows": 4, "vocab": 262145}  # (refused with another status, and later)
+    given = lambda: capi.lib().iq_logits_rules(None, None, *a.values(), C.byref(capi.LogitRules(**rules)))
+    a.update(call)
+    assert given() == -1
+    a.update({"x": P, "out": P})
+    rules = {name: P for name in rules}
+    assert given() == -2
