@@ -202,7 +202,8 @@ int32_t iq_qmm_w8a8(iq_ctx* ctx, void* stream, const void* x, int32_t x_dtype, i
  * 131,056, where the sums are exact in 32 bits for all codes (-128 too): the result does not depend on the other rows, nor on how a
  * call is divided. y of fp32, fp16 or bf16: fp32(fp32(sum) * x_scale) * w_scale, rounded once more for 16 bits; with
  * IQ_FLAG_ACCUMULATE added to y in fp32. Rows and columns of y beyond rows and n stay as they are. rows = 0 does nothing.
- * y may not overlap the operands. */
+ * y may not overlap the operands. w is read as weights are: it may be read while the launch before on the stream still runs, so it is
+ * complete before that launch begins (after iq_i8_pack it is). x, x_scales, w_scales and y may come from that launch. */
 int32_t iq_qmm_i8(iq_ctx* ctx, void* stream, const int8_t* x, int64_t ldx, const float* x_scales, const int8_t* w, const float* w_scales,
                   int32_t n, int32_t k, void* y, int32_t y_dtype, int64_t ldy, int32_t rows, uint32_t flags);
 /* How iq_qmm_i8 divides a call among the SMs of a GPU. Needs no GPU and no context. For tests that have to know which path a shape takes. */
@@ -551,7 +552,8 @@ int32_t iq_rmsnorm(iq_ctx* ctx, void* stream, const float* x, int64_t ldx, void*
  * u holds an infinity or NaN has codes 0 and scale NaN. The sum of squares is fp32: rows beyond 1e19 overflow it.
  * x null (with residual_out null): no addition, r' = residual. weight null: weights of 1, the offset unused. out null or codes (with scales) null: not
  * wanted. weight_offset: 1 where the checkpoint stores w - 1 (Gemma), else 0. residual_out may be residual and out may be x,
- * where row stride and element size are the same; other overlaps are not allowed. Any alignment and strides of at least d; where groups of eight lie on their own size (fp32: 32 bytes, 16 bits: 16, codes: 8) it is faster. d up to 32768; rows = 0 does nothing.
+ * where row stride and element size are the same; other overlaps are not allowed. Tensors begin on an element, strides are at least d; where groups of
+ * eight lie on their own size (fp32: 32 bytes, 16 bits: 16, codes: 8) it is faster. d up to 32768; rows = 0 does nothing.
  * The reference has norm and addition as kernels of their own (Shaders/verify.metal:503-523) and converts activations inside its W8A8
  * GEMM (Layers/Dense.swift:99-172). */
 int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int32_t x_dtype, int64_t ldx, const void* residual, int32_t r_dtype,

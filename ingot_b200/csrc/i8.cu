@@ -19,6 +19,7 @@ int32_t make_map_2d(iq_ctx* ctx, CUtensorMap* map, const void* base, int elem, u
 namespace {
 
 constexpr int kI8MaxK = 131056;  // 131,056 * 128 * 128 < 2^31
+constexpr int kI8Most = 1 << 30;  // rows, features and CTAs
 // kind::i8: s32 sums, signed 8-bit operands, both K-major, M = 128, N = n
 __device__ __forceinline__ uint32_t i8_idesc(int n) { return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(n >> 3) << 17) | (8u << 24); }
 // K-major rows of 128 bytes with the 128-byte swizzle
@@ -256,6 +257,10 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
     }
     tc_fence_before();
     __syncthreads();
+    if (warp == 1) {  // (ahead of the cluster's meeting: a CTA that waits for others holds no tensor memory that theirs, or another kernel's, may be waiting for)
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(T::COLS) : "memory");
+    }
     if (parts > 1) {
         cluster_sync_all();  // every CTA's sums lie in its shared memory
         if (!*abort_flag) {
@@ -281,10 +286,6 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
         asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
     }
     if (*abort_flag && threadIdx.x == 0 && p.status != nullptr) atomicExch(p.status, kErrTimeout);
-    if (warp == 1) {
-        tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(T::COLS) : "memory");
-    }
 }
 
 // ---- many rows: tiles of 256 features and up to 256 tokens on pairs of CTAs -----------------------------------------------
@@ -501,7 +502,7 @@ I8Plan i8_plan(int rows, int n, int k, int sms) {
     c.parts = 1;
     // (a division costs about 1 us: 37 x 1024 x 1024, eight steps, 4.2 us whole and 4.8 in four; 23 steps of 37 x 2880 x 2880 8.4 and 6.4)
     while (steps > 8 && c.parts < 8 && c.tiles * c.parts <= sms && steps >= 4 * c.parts) c.parts *= 2;
-    if (rows <= 128 || sms % 2 != 0) return c;
+    if (rows <= 128 || sms % 2 != 0 || c.tiles > kI8Most) return c;
     int64_t least = (c.tiles * c.parts + 2 * sms - 1) / (2 * sms) * (steps / c.parts) * 330 + 5000;
     const int n_tiles = (n + 255) / 256, groups = (rows + 31) / 32;
     for (int m = (groups + 7) / 8; m <= (groups + 1) / 2; m++) {
@@ -534,6 +535,7 @@ using namespace iq;
 
 extern "C" int32_t iq_qmm_i8_plan(int32_t rows, int32_t n, int32_t k, int32_t sms, iq_qmm_i8_tiling* out) {
     if (out == nullptr || rows < 1 || n < 1 || k < 16 || k % 16 != 0 || k > kI8MaxK || sms < 1) return kErrInvalidArg;
+    if (rows > kI8Most || n > kI8Most) return kErrUnsupported;
     const I8Plan p = i8_plan(rows, n, k, sms);
     out->tile_rows = p.rows;
     out->tall = p.tall;
@@ -552,13 +554,14 @@ extern "C" int32_t iq_qmm_i8(iq_ctx* ctx, void* stream, const int8_t* x, int64_t
     if (rows < 0 || n < 1 || k < 16 || k % 16 != 0) return fail(ctx, kErrInvalidArg, "qmm_i8: rows = %d, n = %d, k = %d (a multiple of 16)", rows, n, k);
     if (k > kI8MaxK) return fail(ctx, kErrUnsupported, "qmm_i8: k = %d (up to %d: sums in 32 bits)", k, kI8MaxK);
     if (ldx < k || ldx % 16 != 0 || ldy < n || reinterpret_cast<uintptr_t>(x) % 16 != 0 || reinterpret_cast<uintptr_t>(w) % 16 != 0 ||
-        reinterpret_cast<uintptr_t>(y) % dtype_size(y_dtype) != 0)
-        return fail(ctx, kErrInvalidArg, "qmm_i8: x and w 16-byte aligned, ldx >= k a multiple of 16, ldy >= n");
+        reinterpret_cast<uintptr_t>(y) % dtype_size(y_dtype) != 0 || (reinterpret_cast<uintptr_t>(x_scales) | reinterpret_cast<uintptr_t>(w_scales)) % 4 != 0)
+        return fail(ctx, kErrInvalidArg, "qmm_i8: x and w 16-byte aligned, y and scales on their elements, ldx >= k a multiple of 16, ldy >= n");
+    if (rows > kI8Most || n > kI8Most) return fail(ctx, kErrUnsupported, "qmm_i8: rows = %d, n = %d (up to %d)", rows, n, kI8Most);
     if ((flags & ~(uint32_t)IQ_FLAG_ACCUMULATE) != 0) return fail(ctx, kErrInvalidArg, "qmm_i8: flags %u", flags);
     if (ctx == nullptr) return kErrInvalidArg;
     if (rows == 0) return kOk;
     const I8Plan plan = i8_plan(rows, n, k, ctx->sms);
-    if (plan.tiles * plan.parts > (1 << 30)) return fail(ctx, kErrUnsupported, "qmm_i8: %lld tiles", (long long)plan.tiles);
+    if (plan.tiles * plan.parts > kI8Most) return fail(ctx, kErrUnsupported, "qmm_i8: %lld tiles", (long long)plan.tiles);
     I8Params p;
     p.sx = x_scales; p.sw = w_scales; p.y = y; p.ldy = ldy; p.y_dtype = y_dtype;
     p.accumulate = flags & IQ_FLAG_ACCUMULATE ? 1 : 0;
@@ -570,7 +573,7 @@ extern "C" int32_t iq_qmm_i8(iq_ctx* ctx, void* stream, const int8_t* x, int64_t
     if (on.error != cudaSuccess) return check_cuda(ctx, on.error, "qmm_i8 device");
     CUtensorMap mx, mw;
     int32_t st = make_map_2d(ctx, &mx, x, 0, (uint64_t)k, (uint64_t)rows, (uint64_t)ldx, 128, (uint32_t)(plan.pair ? plan.rows / 2 : plan.rows), true);
-    if (st == kOk) st = cached_rows_map(ctx, w, n, k, 128, &mw);
+    if (st == kOk) st = make_map_2d(ctx, &mw, w, 0, (uint64_t)k, (uint64_t)n, (uint64_t)k, 128, 128, true);
     if (st != kOk) return st;
     cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
     if (plan.pair)

@@ -210,10 +210,16 @@ extern "C" int32_t iq_qmm_w8a8(iq_ctx* ctx, void* stream, const void* x, int32_t
     return launch_qmm(ctx, cs, c);
 }
 
+// iq_qmm_i8 may read weights while the launch before it still runs. This one, in plain stream order, is between: it starts when the rows are in memory.
+__global__ void i8_packed_kernel() {}
+
 extern "C" int32_t iq_i8_pack(iq_ctx* ctx, void* stream, const iq_qlinear* m, int32_t rotate, int8_t* w, float* scales) {
     // (the checks come before the context is looked at: they are the same without a GPU)
     if (m == nullptr || m->w == nullptr || m->scales == nullptr || m->biases == nullptr || w == nullptr || scales == nullptr || reinterpret_cast<uintptr_t>(w) % 16 != 0)
         return fail(ctx, kErrInvalidArg, "i8_pack: null pointer, or w is not 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(m->w) % 4 != 0 || (reinterpret_cast<uintptr_t>(m->scales) | reinterpret_cast<uintptr_t>(m->biases)) % 2 != 0 ||
+        reinterpret_cast<uintptr_t>(scales) % 4 != 0)
+        return fail(ctx, kErrInvalidArg, "i8_pack: a tensor does not begin on an element");
     if (m->mode != IQ_MODE_AFFINE || m->experts > 1 || m->bits != 4 || (m->group != 64 && m->group != 32))
         return fail(ctx, kErrUnsupported, "i8_pack: %d-bit group %d mode %d (4-bit affine with group 64 or 32)", m->bits, m->group, m->mode);
     if (m->n < 1 || m->k < 64 || m->k % 64 != 0 || m->k > 49152) return fail(ctx, kErrInvalidArg, "i8_pack: n = %d, k = %d (a multiple of 64, at most 49152)", m->n, m->k);
@@ -226,5 +232,6 @@ extern "C" int32_t iq_i8_pack(iq_ctx* ctx, void* stream, const iq_qlinear* m, in
     // (H x) . (H w) = n x . w: the weights' scales take the 1 / n
     rot_quant_rows_kernel<0><<<m->n, 256, (size_t)m->k * sizeof(float), reinterpret_cast<cudaStream_t>(stream)>>>(
         m->w, static_cast<const uint16_t*>(m->scales), static_cast<const uint16_t*>(m->biases), m->group, 0, 0, m->k, n, w, scales, 1.0f / (float)n);
+    i8_packed_kernel<<<1, 1, 0, reinterpret_cast<cudaStream_t>(stream)>>>();
     return check_cuda(ctx, cudaGetLastError(), "i8_pack launch");
 }

@@ -275,7 +275,8 @@ class VQMV:
 
 class I8Linear:
     """A W8A8 linear on weights packed once: int8 rows [N, K] and a float32 scale per row (iq_qmm_i8). `rotate`: the block of the Hadamard transform
-    that its inputs have gone through as well (0: none), for add_rmsnorm(rotate=)."""
+    that its inputs have gone through as well (0: none), for add_rmsnorm(rotate=). `w` may be read while the
+    launch before on the stream still runs: it is complete before that launch begins (after `pack` it is)."""
 
     MAX_K = 131056
 
@@ -335,6 +336,8 @@ class I8Linear:
             self._check(x, x_scales, y, rows)
             _need_cuda(x)
             raise ValueError("I8Linear does not take these tensors")
+        if rows == 0:  # (tensors of no rows have no address)
+            return
         if rows <= 1:  # (one row has no stride)
             ldx, ldy = xk, yn
         ctx = capi.context(dev)

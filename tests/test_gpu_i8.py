@@ -1,11 +1,13 @@
 """W8A8 linears on packed int8 rows (iq_qmm_i8 through linear.I8Linear): bit for bit, since the sums are exact integers and what follows is
 a fixed order of fp32 operations. And the packing of 4-bit matrices."""
+import ctypes as C
+
 import numpy as np
 import pytest
 import torch
 
 from ingot_b200 import capi
-from ingot_b200.linear import I8Linear
+from ingot_b200.linear import VQMV, I8Linear
 from ingot_b200.norm import add_rmsnorm
 from oracle import qref
 from gpu_util import affine_case, deq
@@ -165,3 +167,68 @@ def test_codes_into_linear(cuda_device, rows, K, rotate):
     # and exactly, from the codes
     want = reference(xq.cpu(), sx.cpu(), lin.w.cpu(), lin.scales.cpu())
     assert torch.equal(y.cpu(), want)
+
+
+@pytest.mark.parametrize("rows", [5, 300])
+def test_weights_packed_by_the_launch_before(cuda_device, rows):
+    """The linear reads weights ahead of the launch before it; packing leaves them complete, a buffer that is packed again too, eagerly and in a graph."""
+    rng, gen = np.random.default_rng(rows), torch.Generator().manual_seed(rows)
+    N, K = 640, 1024
+    matrices = [affine_case(rng, N, K, 4, cuda_device)[0] for _ in range(2)]
+    w, s = torch.zeros(N, K, dtype=torch.int8, device="cuda"), torch.zeros(N, device="cuda")
+    lin = I8Linear(w, s)
+    x, sx = codes(gen, rows, K).cuda(), torch.rand(rows, generator=gen).cuda()
+    want = [torch.empty(rows, N, device="cuda") for _ in matrices]
+    for m, y in zip(matrices, want):
+        packed = I8Linear.pack(m, 0)
+        torch.cuda.synchronize()
+        packed.encode(x, sx, y, rows)
+    y = torch.empty(8, rows, N, device="cuda")
+    def again():
+        for i in range(8):
+            q = matrices[i % 2].qlinear()
+            st = capi.lib().iq_i8_pack(capi.context(0).handle, torch.cuda.current_stream().cuda_stream, C.byref(q), 0, w.data_ptr(), s.data_ptr())
+            assert st == 0
+            lin.encode(x, sx, y[i], rows)
+    again()
+    torch.cuda.synchronize()
+    for i in range(8):
+        assert torch.equal(y[i], want[i % 2])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        again()
+    for _ in range(3):
+        y.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y[i], want[i % 2]) for i in range(8))
+
+
+def test_streams_at_once(cuda_device):
+    """Clusters, pairs and the decode linears' own clusters beside one another: a CTA that waits for the others of its cluster holds no tensor memory."""
+    rng, gen = np.random.default_rng(3), torch.Generator().manual_seed(3)
+    dense, _ = affine_case(rng, 1024, 4096, 4, cuda_device)
+    dx, dy = torch.randn(8, 4096, generator=gen).half().cuda(), torch.empty(8, 1024, device="cuda")
+    VQMV.encode(dx, dense, dy, 8)
+    dense_want = dy.clone()
+    jobs = []
+    for rows, n, k in ((1, 1024, 4096), (40, 512, 4096), (300, 1024, 1024), (64, 1000, 2048)):
+        x, sx = codes(gen, rows, k).cuda(), torch.rand(rows, generator=gen).cuda()
+        m = I8Linear(codes(gen, n, k).cuda(), torch.rand(n, generator=gen).cuda())
+        want = torch.empty(rows, n, device="cuda")
+        m.encode(x, sx, want, rows)
+        jobs.append((m, x, sx, torch.empty_like(want), want, rows, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    for _ in range(20):
+        for m, x, sx, y, _, rows, stream in jobs:
+            m.encode(x, sx, y, rows, stream=stream)
+        VQMV.encode(dx, dense, dy, 8, stream=side)
+    torch.cuda.synchronize()
+    assert capi.context(0).device_status() == 0
+    assert all(torch.equal(j[3], j[4]) for j in jobs) and torch.equal(dy, dense_want)
+
+
+def test_tensors_of_no_rows(cuda_device):
+    m = I8Linear(torch.zeros(8, 64, dtype=torch.int8, device="cuda"), torch.zeros(8, device="cuda"))
+    m.encode(torch.empty(0, 64, dtype=torch.int8, device="cuda"), torch.empty(0, device="cuda"), torch.empty(0, 8, device="cuda"), 0)

@@ -73,3 +73,31 @@ def test_the_plan():
     for bad in ((0, 1, 16), (1, 0, 16), (1, 1, 24), (1, 1, 131072)):
         with pytest.raises(capi.IngotError):
             capi.qmm_i8_plan(*bad)
+
+
+@pytest.mark.parametrize("change", [{"sx": P + 2}, {"sw": P + 1}, {"y": P + 2}, {"y": P + 1, "yd": 2}])
+def test_tensors_begin_on_an_element(change):
+    a = {"x": P, "ldx": 64, "sx": P, "w": P, "sw": P, "n": 8, "k": 64, "y": P, "yd": 0, "ldy": 8, "rows": (1 << 30) + 1, "flags": 0}  # (too many rows: later, with another status)
+    a.update(change)
+    call = lambda: capi.lib().iq_qmm_i8(None, None, *a.values())
+    assert call() == -1
+    a.update({"sx": P, "sw": P, "y": P})
+    assert call() == -2
+
+
+@pytest.mark.parametrize("change,scales", [({"w": P + 2}, P), ({"scales": P + 1}, P), ({"biases": P + 1}, P), ({}, P + 2)])
+def test_packed_tensors_begin_on_an_element(change, scales):
+    a = {"w": P, "scales": P, "biases": P, "n": 8, "k": 128, "bits": 8, "group": 64, "mode": 0, "experts": 1}  # (8 bits: later, with another status)
+    assert capi.lib().iq_i8_pack(None, None, C.byref(capi.QLinear(*a.values())), 0, P, P) == -2
+    a.update(change)
+    assert capi.lib().iq_i8_pack(None, None, C.byref(capi.QLinear(*a.values())), 0, P, scales) == -1
+
+
+@pytest.mark.parametrize("rows,n,k", [((1 << 30) + 1, 8, 64), (8, (1 << 30) + 1, 64), (2**31 - 1, 2**31 - 1, 131056), (1 << 30, 1 << 30, 131056)])
+def test_more_than_a_grid_holds(rows, n, k):
+    assert capi.lib().iq_qmm_i8(None, None, P, k, P, P, P, n, k, P, 0, max(n, 1), rows, 0) in (-1, -2)
+    if max(rows, n) > 1 << 30:
+        with pytest.raises(capi.IngotError):
+            capi.qmm_i8_plan(rows, n, k)
+    else:
+        assert capi.qmm_i8_plan(rows, n, k).tiles > 1 << 30  # (refused with a context)
