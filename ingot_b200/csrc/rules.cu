@@ -10,11 +10,11 @@
 // The history is the row's list of tokens as the conversation has it: nothing is kept between calls. A block has a part of a row and a
 // counter for each of its tokens in shared memory, and looks through the row's list for them.
 //
-// Bound: start and latencies for few rows (one of 128,000 with 2048 tokens, biases and a grammar 3.5 us), the memory for many (64 of 262,144 without history
-// 23.0 us, floor 20.6), additions in shared memory for long histories (16,384 tokens: eight rows of 151,936 2.7 -> 10.1 us, most of it in the block that has the
-// frequent tokens). Measured and taken back: a cluster per row whose blocks share the list and count into each other's memory (11.3 us for the one row, 102 for
-// 64 with 16,384 tokens against 40), parts of every so many-th run of 128 tokens instead of neighbouring ones (10.1 -> 14.6: more instructions and more
-// additions of few lanes each), lanes with the same token found by match (16.8), tokens queued until there are 32 (14.4).
+// Bound: start and latencies for few rows (one of 128,000 with 2048 tokens, biases and a grammar 3.3 us), the memory for many (64 of 262,144 without history
+// 22.6 us, floor 20.6), looking at long histories (16,384 tokens: eight rows of 151,665 2.2 -> 6.6 us; each of a row's blocks looks at all of them, 13 instructions
+// for 32). Measured and taken back: a cluster per row whose blocks share the list and count into each other's memory (11.3 us for the one row, 102 for 64 with
+// 16,384 tokens against 40), parts of every so many-th run of 128 tokens instead of neighbouring ones (10.1 -> 14.6), lanes with the same token found by match
+// (16.8), tokens queued until there are 32 (14.4), the next tokens loaded ahead (6.6 -> 6.9), four groups of logits under way instead of two (7.2).
 #include <math.h>
 #include <algorithm>
 #include <type_traits>
@@ -25,10 +25,11 @@
 namespace iq {
 namespace {
 
-constexpr int kRuleThreads = 512;
 constexpr int kRuleMaxVocab = 262144;
-constexpr int kRulePerSm = 3;     // blocks of an SM
-constexpr int kRuleSpan = 24576;  // most logits of a block
+constexpr int kRulePerSm = 3;     // blocks of an SM, of 512 threads each; one of 1024 where that is all
+constexpr int kRuleSpan = 24576;  // most logits of a block,
+constexpr int kRuleWhole = 32768;  // of one with an SM to itself,
+constexpr int kRuleLeast = 2048;   // and least
 constexpr int kRuleBatch = 2;     // times four logits of a thread that are under way at once
 constexpr int kRuleLook = 4;      // tokens of the history likewise, before its length is known
 
@@ -37,7 +38,7 @@ struct RuleParams {
     int64_t ldx;
     float* out;
     int64_t ldo;
-    int32_t x_dtype, vocab, span, parts;  // span: logits of a block, a multiple of 2048; parts: blocks of a row
+    int32_t x_dtype, vocab, span, parts;  // span: logits of a block, a multiple of 128; parts: blocks of a row
     uint32_t misplaced;  // elements by which out lies behind a group of four
     iq_logit_rules r;
 };
@@ -77,10 +78,11 @@ struct Counter {
     }
 };
 
-// The biases of a block's tokens among up to kRuleThreads entries of a row's list, in any order: the place in the list and the token in one word.
+// The biases of a block's tokens among up to T entries of a row's list, in any order: the place in the list and the token in one word.
+template <int T>
 struct BiasList {
-    uint32_t key[kRuleThreads];  // place << 16 | token, from the block's first on
-    float value[kRuleThreads];
+    uint32_t key[T];  // place << 16 | token, from the block's first on
+    float value[T];
     int n;
     // v with the token's biases, in their order
     __device__ __forceinline__ float add(float v, uint32_t t) const {
@@ -103,12 +105,12 @@ struct BiasList {
 // DT: x's type. HIST: with counters. VEC: a row of x and the same one of out begin at the same place within groups of four (0 to 3 elements into one);
 // the blocks' parts begin on such groups, the first one's `shift` before the row. Rows of an odd vocabulary are taken four logits at a time like this
 // (eight rows of 151,665 4.0 us on one logit at a time, of 151,936 2.5).
-template <int DT, bool HIST, bool WIDE, bool VEC>
-__global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(const __grid_constant__ RuleParams p) {
+template <int T, int DT, bool HIST, bool WIDE, bool VEC>
+__global__ void __launch_bounds__(T, T == 512 ? kRulePerSm : 1) logit_rules_kernel(const __grid_constant__ RuleParams p) {
     typedef Counter<WIDE> Count;
     typedef typename std::conditional<DT == kF32, float, uint16_t>::type E;
     extern __shared__ uint4 smem[];
-    __shared__ BiasList list;
+    __shared__ BiasList<T> list;
     uint32_t* const count = reinterpret_cast<uint32_t*>(smem);
     const int tid = threadIdx.x;
     const int row = blockIdx.x / p.parts, part = blockIdx.x % p.parts;
@@ -116,7 +118,7 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
     const int lo = part * p.span - shift, n = max(min(p.span, p.vocab - lo), 0);  // this block's logits are lo .. lo + n, from 0 on
     pdl_launch_dependents();
     if (HIST)
-        for (int i = tid; i < p.span / (WIDE ? 4 : 8); i += kRuleThreads) smem[i] = make_uint4(0, 0, 0, 0);
+        for (int i = tid; i < p.span / (WIDE ? 4 : 8); i += T) smem[i] = make_uint4(0, 0, 0, 0);
     if (tid == 0) list.n = 0;
     pdl_wait();
     const E* const x = static_cast<const E*>(p.x) + (size_t)row * p.ldx + lo;  // (of the block's logits)
@@ -126,9 +128,9 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
         const uint16_t h = reinterpret_cast<const uint16_t*>(x)[i];
         return DT == kBF16 ? bf16_bits_to_f32(h) : __half2float(__ushort_as_half(h));
     };
-    // A thread has the groups of four tid, tid + kRuleThreads, ... of the part: those that lie in the row as a whole are turns first_ .. last_, one at
+    // A thread has the groups of four tid, tid + T, ... of the part: those that lie in the row as a whole are turns first_ .. last_, one at
     // either end may not (the row's first and last logits).
-    constexpr int kStep = 4 * kRuleThreads;
+    constexpr int kStep = 4 * T;
     const int first_ = lo + 4 * tid < 0 ? 1 : 0, last_ = n >= 4 * tid + 4 ? (n - 4 * tid - 4) / kStep + 1 : 0;
     struct Four {
         uint32_t v[DT == kF32 ? 4 : 2];
@@ -160,7 +162,7 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
     uint32_t look[kRuleLook];
     if (HIST) {
 #pragma unroll
-        for (int k = 0; k < kRuleLook; k++) look[k] = k * kRuleThreads + tid < p.r.max_tokens ? (uint32_t)tokens[k * kRuleThreads + tid] : 0xFFFFFFFFu;
+        for (int k = 0; k < kRuleLook; k++) look[k] = k * T + tid < p.r.max_tokens ? (uint32_t)tokens[k * T + tid] : 0xFFFFFFFFu;
     }
     const float rep = p.r.repetition != nullptr ? p.r.repetition[row] : 1.f, pres = p.r.presence != nullptr ? p.r.presence[row] : 0.f;
     const float freq = p.r.frequency != nullptr ? p.r.frequency[row] : 0.f;
@@ -208,16 +210,16 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
             if (i < len && t < (uint32_t)n) Count::note(count, t, i < prompt);
         };
 #pragma unroll
-        for (int k = 0; k < kRuleLook; k++) note(k * kRuleThreads + tid, look[k]);
+        for (int k = 0; k < kRuleLook; k++) note(k * T + tid, look[k]);
         // Long histories by 4096 tokens that are all of the prompt or all generated (a load of 32 costs some ten instructions then, else thirty: the blocks of a
         // row all look at all of them)
         const bool whole = (reinterpret_cast<uintptr_t>(tokens) & 15) == 0;
         const uint32_t counters = smem_u32(count);
-        for (int i0 = kRuleLook * kRuleThreads; i0 < len; i0 += 8 * kRuleThreads) {
-            const int i1 = i0 + 8 * kRuleThreads;
+        for (int i0 = kRuleLook * T; i0 < len; i0 += 8 * T) {
+            const int i1 = i0 + 8 * T;
             if (whole && i1 <= len && (i0 >= prompt || i1 <= prompt)) {
                 const int4* const q = reinterpret_cast<const int4*>(tokens + i0) + tid;
-                const int4 a = q[0], b = q[kRuleThreads];
+                const int4 a = q[0], b = q[T];
                 const uint32_t t[8] = {(uint32_t)a.x, (uint32_t)a.y, (uint32_t)a.z, (uint32_t)a.w, (uint32_t)b.x, (uint32_t)b.y, (uint32_t)b.z, (uint32_t)b.w};
                 if (i0 >= prompt) {
 #pragma unroll
@@ -230,9 +232,9 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
             }
             uint32_t t[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++) t[k] = i0 + k * kRuleThreads + tid < len ? (uint32_t)tokens[i0 + k * kRuleThreads + tid] : 0xFFFFFFFFu;
+            for (int k = 0; k < 8; k++) t[k] = i0 + k * T + tid < len ? (uint32_t)tokens[i0 + k * T + tid] : 0xFFFFFFFFu;
 #pragma unroll
-            for (int k = 0; k < 8; k++) note(i0 + k * kRuleThreads + tid, t[k]);
+            for (int k = 0; k < 8; k++) note(i0 + k * T + tid, t[k]);
         }
     }
     __syncthreads();  // every token is counted, every bias in the list
@@ -329,7 +331,7 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
         if (store) out[my_token] = my_result;
     }
     // more biases than the list takes at once: by rounds
-    for (int j0 = b0 + kRuleThreads; j0 < b1; j0 += kRuleThreads) {
+    for (int j0 = b0 + T; j0 < b1; j0 += T) {
         __syncthreads();
         if (tid == 0) list.n = 0;
         __syncthreads();
@@ -344,23 +346,27 @@ __global__ void __launch_bounds__(kRuleThreads, kRulePerSm) logit_rules_kernel(c
 }
 
 typedef void (*RulesKernel)(RuleParams);
-template <int DT>
-RulesKernel rules_pick(bool hist, bool wide, bool vec) {
-    if (!hist) return vec ? logit_rules_kernel<DT, false, false, true> : logit_rules_kernel<DT, false, false, false>;
-    if (wide) return vec ? logit_rules_kernel<DT, true, true, true> : logit_rules_kernel<DT, true, true, false>;
-    return vec ? logit_rules_kernel<DT, true, false, true> : logit_rules_kernel<DT, true, false, false>;
+enum { kNoHistory, kNarrow, kWide, kWhole };  // no counters; two of 16 bits in a word; of 32 bits; those and an SM to itself
+template <int DT, bool VEC>
+RulesKernel rules_pick(int kind) {
+    return kind == kNoHistory ? logit_rules_kernel<512, DT, false, false, VEC> : kind == kNarrow ? logit_rules_kernel<512, DT, true, false, VEC>
+                                                                             : kind == kWide   ? logit_rules_kernel<512, DT, true, true, VEC>
+                                                                                               : logit_rules_kernel<1024, DT, true, true, VEC>;
 }
-RulesKernel rules_pick(int dtype, bool hist, bool wide, bool vec) {
-    return dtype == kF32 ? rules_pick<kF32>(hist, wide, vec) : dtype == kF16 ? rules_pick<kF16>(hist, wide, vec) : rules_pick<kBF16>(hist, wide, vec);
+template <int DT>
+RulesKernel rules_pick(int kind, bool vec) { return vec ? rules_pick<DT, true>(kind) : rules_pick<DT, false>(kind); }
+RulesKernel rules_pick(int dtype, int kind, bool vec) {
+    return dtype == kF32 ? rules_pick<kF32>(kind, vec) : dtype == kF16 ? rules_pick<kF16>(kind, vec) : rules_pick<kBF16>(kind, vec);
 }
 
 }  // namespace
 
 int32_t rules_init(iq_ctx* ctx) {
     for (int dtype = 0; dtype < 3; dtype++)
-        for (int kind = 0; kind < 4; kind++) {
-            const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(rules_pick(dtype, true, (kind & 1) != 0, (kind & 2) != 0)),
-                                                       cudaFuncAttributeMaxDynamicSharedMemorySize, kRuleSpan * (kind & 1 ? 4 : 2));
+        for (int v = 0; v < 6; v++) {
+            const int kind = kNarrow + v / 2;
+            const cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(rules_pick(dtype, kind, v % 2 != 0)), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                       kind == kNarrow ? kRuleSpan * 2 : kind == kWide ? kRuleSpan * 4 : kRuleWhole * 4);
             if (e != cudaSuccess) return check_cuda(ctx, e, "cudaFuncSetAttribute(logit_rules)");
         }
     return kOk;
@@ -393,20 +399,29 @@ extern "C" int32_t iq_logits_rules(iq_ctx* ctx, void* stream, const void* x, int
     if (rows == 0) return kOk;
     RuleParams p;
     p.x = x; p.ldx = ldx; p.out = out; p.ldo = ldo; p.x_dtype = x_dtype; p.vocab = vocab; p.r = r;
-    // whole rounds over the SMs, as few as the largest span allows
-    for (int64_t rounds = 1;; rounds++) {
-        const int64_t parts = std::max<int64_t>(kRulePerSm * ctx->sms * rounds / rows, 1);
-        p.span = (int)((vocab + 3 + parts - 1) / parts + 2047) / 2048 * 2048;
-        if (p.span <= kRuleSpan) break;
+    const bool hist = r.tokens != nullptr && r.max_tokens > 0 && (r.repetition != nullptr || r.presence != nullptr || r.frequency != nullptr);
+    int kind = !hist ? kNoHistory : r.max_tokens > 0x7FFF ? kWide : kNarrow;
+    // Logits of a block where the rows have so many blocks. With a history and where that fits, a block of 1024 threads per SM: every block looks at the whole
+    // list, and counters of 32 bits take half the instructions. Otherwise three of 512 per SM, in whole rounds, as few as the largest span allows: their phases
+    // overlap (without a history 64 rows of 262,144 22.6 us). One / three blocks per SM, 16,384 (500) tokens, us: one row of 128,000 4.1 / 5.0 (2.4 / 2.3),
+    // 8 of 151,665 6.6 / 9.2 (3.9 / 4.3), 64 of 32,000 8.6 / 12.2 (4.4 / 5.4), 24 of 151,665 11.6 / 14.9 (8.0 / 7.9), with 50,555 logits per block 40 of
+    // 151,665 16.8 / 17.9 (13.4 / 10.9).
+    auto span = [&](int64_t blocks, int least) {
+        const int64_t parts = std::max<int64_t>(blocks / rows, 1);
+        return std::max((int)((vocab + 3 + parts - 1) / parts + 127) / 128 * 128, least);
+    };
+    if (hist && rows <= ctx->sms && span(ctx->sms, kRuleLeast / 2) <= kRuleWhole) {
+        kind = kWhole;
+        p.span = span(ctx->sms, kRuleLeast / 2);
+    } else {
+        for (int64_t rounds = 1; rounds == 1 || p.span > kRuleSpan; rounds++) p.span = span(kRulePerSm * ctx->sms * rounds, kRuleLeast);
     }
     p.parts = (vocab + 3 + p.span - 1) / p.span;  // (a row may begin three elements into the first one's)
-    const bool hist = r.tokens != nullptr && r.max_tokens > 0 && (r.repetition != nullptr || r.presence != nullptr || r.frequency != nullptr);
-    const bool wide = hist && r.max_tokens > 0x7FFF;
     p.misplaced = (uint32_t)(reinterpret_cast<uintptr_t>(out) / 4 & 3);
     const bool vec = (reinterpret_cast<uintptr_t>(x) / esz & 3) == p.misplaced && ((ldx ^ ldo) & 3) == 0;
-    const RulesKernel kernel = rules_pick(x_dtype, hist, wide, vec);
+    const RulesKernel kernel = rules_pick(x_dtype, kind, vec);
     DeviceScope on(ctx);
     if (on.error != cudaSuccess) return check_cuda(ctx, on.error, "logits_rules device");
-    return check_cuda(ctx, launch_dependent(kernel, dim3((unsigned)rows * p.parts), kRuleThreads, hist ? (size_t)p.span * (wide ? 4 : 2) : 0, reinterpret_cast<cudaStream_t>(stream), p),
+    return check_cuda(ctx, launch_dependent(kernel, dim3((unsigned)rows * p.parts), kind == kWhole ? 1024 : 512, hist ? (size_t)p.span * (kind == kNarrow ? 2 : 4) : 0, reinterpret_cast<cudaStream_t>(stream), p),
                       "logits_rules launch");
 }

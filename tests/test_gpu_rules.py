@@ -268,3 +268,18 @@ def test_two_streams_at_once(cuda_device):
             rules.encode(x, rows, out=o, stream=s)
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in outs)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("rows,V,pad,history", [(160, 2000, 0, 300), (160, 2001, 2, 300), (150, 300, 0, 33000), (149, 301, 1, 33000)])
+def test_more_rows_than_multiprocessors(cuda_device, rows, V, pad, history, dtype):
+    """Several blocks per multiprocessor, with counters of both widths."""
+    rng = np.random.default_rng(rows + V)
+    check(rng, rows, V, some(rng, rows, V, history=history, bias=5, masks=3, wild=True), dtype=dtype, pad=pad)
+
+
+@pytest.mark.parametrize("rows,V", [(1, 1), (1, 1023), (1, 1025), (2, 75777), (5, 250000), (5, 262144), (18, 262144), (37, 131072), (37, 131069), (38, 131072), (148, 32765), (148, 32766)])
+def test_blocks_with_a_multiprocessor_to_themselves(cuda_device, rows, V):
+    """Up to the largest part, and the first that is too large."""
+    rng = np.random.default_rng(rows + V)
+    check(rng, rows, V, some(rng, rows, V, history=700, bias=9, masks=2))
