@@ -211,8 +211,8 @@ typedef struct iq_qmm_i8_tiling {
     int32_t tile_rows; /* tokens per tile, */
     int32_t tall;      /* of the first `tall` of the */
     int32_t row_tiles; /* tiles over the rows; with pairs the others have 32 fewer */
-    int32_t pair;      /* 1: a tile of 256 features on two CTAs; 0: of 128 on a cluster */
-    int32_t parts;     /* CTAs of the cluster, which divide k */
+    int32_t pair;      /* 1: a tile of 256 features on pairs of CTAs; 0: of 128 on CTAs */
+    int32_t parts;     /* CTAs or pairs of a cluster, which divide k */
     int64_t tiles;
 } iq_qmm_i8_tiling;
 int32_t iq_qmm_i8_plan(int32_t rows, int32_t n, int32_t k, int32_t sms, iq_qmm_i8_tiling* out);

@@ -132,6 +132,37 @@ __device__ __forceinline__ void i8_store4(const I8Params& p, const int4& s, floa
     }
 }
 
+// A thread's share of the results of 128 features from n0 on, in units of a token and four features (u0 + thread, and so on up to u1): the sums of PARTS CTAs of the
+// cluster, which parked them at `park`, [token][128 features]. Eight loads of 16 bytes are under way at once. sx, sw: the scales of the first unit.
+template <int PARTS, int THREADS, int STEP>
+__device__ __forceinline__ void i8_shares(const I8Params& p, uint32_t park, uint32_t first, int u0, int u1, int row0, int n0, float sx0, const float (&sw)[4]) {
+    static_assert(THREADS % 32 == 0, "a thread's units are of the same features");
+    constexpr int B = 8 / PARTS;
+    const int n = n0 + u0 % 32 * 4;
+    for (int u = u0; u < u1; u += B * THREADS) {
+        int4 o[B][PARTS];
+        float sx[B];
+#pragma unroll
+        for (int b = 0; b < B; b++)
+            if (u + b * THREADS < u1) {
+#pragma unroll
+                for (int c = 0; c < PARTS; c++) o[b][c] = ld_dsmem_s4(park + (u + b * THREADS) * 16, first + STEP * c);
+                sx[b] = u + b == u0 ? sx0 : p.sx[row0 + (u + b * THREADS) / 32];
+            }
+#pragma unroll
+        for (int b = 0; b < B; b++) {
+            if (u + b * THREADS >= u1) break;
+            int4 v = o[b][0];
+#pragma unroll
+            for (int c = 1; c < PARTS; c++) { v.x += o[b][c].x; v.y += o[b][c].y; v.z += o[b][c].z; v.w += o[b][c].w; }
+            const int t = row0 + (u + b * THREADS) / 32;
+            if (p.y_dtype == kF32) i8_store4<kF32>(p, v, sx[b], sw, t, n);
+            else if (p.y_dtype == kBF16) i8_store4<kBF16>(p, v, sx[b], sw, t, n);
+            else i8_store4<kF16>(p, v, sx[b], sw, t, n);
+        }
+    }
+}
+
 // A tile per cluster; its CTAs divide the steps among them and add their sums through distributed shared memory.
 //
 // Bound: the weights' way from memory, and per call some 4 us of start (1 us from the kernel before to the first activations), sums of the cluster (2) and
@@ -264,22 +295,11 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
     if (parts > 1) {
         cluster_sync_all();  // every CTA's sums lie in its shared memory
         if (!*abort_flag) {
-            // this CTA's share of the tile, four features at a time; all loads before the first sum
-            for (int u = u0 + (int)threadIdx.x; u < u1; u += kI8Threads) {
-                const int t = row0 + u / 32, n = n0 + u % 32 * 4;
-                if (u >= u0 + kI8Threads) unit_scales(u);
-                int4 o[8];
-#pragma unroll
-                for (int c = 0; c < 8; c++)
-                    if (c < parts) o[c] = ld_dsmem_s4(smem_u32(smem) + u * 16, c);
-                int4 v = make_int4(0, 0, 0, 0);
-#pragma unroll
-                for (int c = 0; c < 8; c++)
-                    if (c < parts) { v.x += o[c].x; v.y += o[c].y; v.z += o[c].z; v.w += o[c].w; }
-                if (p.y_dtype == kF32) i8_store4<kF32>(p, v, unit_sx, unit_sw, t, n);
-                else if (p.y_dtype == kBF16) i8_store4<kBF16>(p, v, unit_sx, unit_sw, t, n);
-                else i8_store4<kF16>(p, v, unit_sx, unit_sw, t, n);
-            }
+            const uint32_t park = smem_u32(smem);
+            const int u = u0 + (int)threadIdx.x;
+            if (parts == 2) i8_shares<2, kI8Threads, 1>(p, park, 0, u, u1, row0, n0, unit_sx, unit_sw);
+            else if (parts == 4) i8_shares<4, kI8Threads, 1>(p, park, 0, u, u1, row0, n0, unit_sx, unit_sw);
+            else i8_shares<8, kI8Threads, 1>(p, park, 0, u, u1, row0, n0, unit_sx, unit_sw);
         }
         // nobody reads this CTA's shared memory any more (what was read has gone into the sums: no ordering of memory to wait for)
         __syncwarp();
@@ -301,12 +321,12 @@ __device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, ui
         ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
         : "memory");
 }
-// Tensor copy into this CTA's shared memory whose bytes count on the barrier at this offset of the pair's even CTA
-__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+// Tensor copy into this CTA's shared memory whose bytes count on the barrier at this offset of the pair's even CTA, the cluster's CTA `even`
+__device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, uint32_t even = 0) {
     asm volatile(
-        "{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %2, 0;\n"
+        "{\n.reg .b32 r;\nmapa.shared::cluster.u32 r, %2, %5;\n"
         "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [r];\n}\n"
-        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1)
+        ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1), "r"(even)
         : "memory");
 }
 
@@ -470,6 +490,136 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
     }
 }
 
+// Completion of all tcgen05.mma issued so far, to the barrier at this offset in both CTAs of the pair whose even one is the cluster's CTA `even`
+__device__ __forceinline__ void umma_commit_pair_at(uint32_t bar, uint32_t even) {
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar), "h"((uint16_t)(3u << even))
+                 : "memory");
+}
+
+// Few tiles and many inputs: SPLIT pairs in a cluster divide a tile's steps, a tile per cluster. Every CTA parks its sums (its 128 features, int32) where its
+// stages were, and finishes its share of the tokens from its SPLIT counterparts' memory.
+template <int SPLIT>
+__global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2 * SPLIT, 1, 1)
+    i8_split_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const I8Params p) {
+    extern __shared__ unsigned char smem_raw[];
+    unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + kI8PairStages * kI8PairStage);  // full, empty, sums
+    const uint32_t full = smem_u32(bars), empty = full + 8 * kI8PairStages, sums = empty + 8 * kI8PairStages;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * kI8PairStages + 1);
+    volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+    static_assert(256 * 512 <= kI8PairStages * kI8PairStage, "the partial sums take the stages' place");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank(), half = rank & 1, even = rank & ~1u;
+    const int part = (int)rank / 2, tile = blockIdx.x / (2 * SPLIT), m = tile % p.m_tiles;
+    const int row0 = m * p.tile_rows - 32 * max(m - p.tall, 0), rows = min(p.tile_rows - (m < p.tall ? 0 : 32), p.M - row0), tokens = (rows + 31) & ~31;
+    const int n0 = (tile / p.m_tiles) * 256 + 128 * (int)half;
+    const int ks0 = p.steps * part / SPLIT, ks1 = p.steps * (part + 1) / SPLIT;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kI8PairStages; s++) {
+            mbar_init(full + 8 * s, 1);
+            mbar_init(empty + 8 * s, 1);
+        }
+        mbar_init(sums, 1);
+        *abort_flag = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_smem();
+    }
+    if (warp == 1) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(256) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // the other CTAs' barriers exist
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    pdl_launch_dependents();
+    const uint32_t bytes = 128 * 128 + p.tile_rows * 64;  // of a CTA and stage
+    // this CTA's share of its features' results, in units of a token and four features, and the scales of a thread's unit (the first: ahead of the sums)
+    const int units = rows * 32, u0 = units * part / SPLIT, u1 = units * (part + 1) / SPLIT;
+    float unit_sx = 0.f, unit_sw[4];
+    auto unit_scales = [&](int u) {
+        const int n = n0 + u % 32 * 4;
+        unit_sx = p.sx[row0 + u / 32];
+#pragma unroll
+        for (int j = 0; j < 4; j++) unit_sw[j] = n + j < p.N ? p.sw[n + j] : 0.f;
+    };
+    if (warp == 0) {
+        if (elect_one()) {
+            const int xrow = row0 + (int)half * (tokens / 2), ahead = min(kI8PairStages, ks1 - ks0);
+            // the first stages' weights ahead of the wait for the kernel before
+            for (int s = 0; s < ahead; s++) {
+                if (half == 0) mbar_arrive_expect_tx(full + 8 * s, 2 * bytes);
+                tma_load_2d_pair(smem_u32(smem + s * kI8PairStage), &map_w, full + 8 * s, (ks0 + s) * 128, n0, even);
+            }
+            pdl_wait();
+            for (int s = 0; s < ahead; s++) tma_load_2d_pair(smem_u32(smem + s * kI8PairStage) + 128 * 128, &map_x, full + 8 * s, (ks0 + s) * 128, xrow, even);
+            int s = ahead % kI8PairStages;
+            uint32_t ph = 0;
+            for (int ks = ks0 + ahead; ks < ks1; ks++) {
+                if (!mbar_wait(empty + 8 * s, ph, abort_flag)) break;
+                const uint32_t st = smem_u32(smem + s * kI8PairStage);
+                if (half == 0) mbar_arrive_expect_tx(full + 8 * s, 2 * bytes);
+                tma_load_2d_pair(st, &map_w, full + 8 * s, ks * 128, n0, even);
+                tma_load_2d_pair(st + 128 * 128, &map_x, full + 8 * s, ks * 128, xrow, even);
+                if (++s == kI8PairStages) { s = 0; ph ^= 1; }
+            }
+        }
+    } else if (warp == 1) {
+        if (half == 0 && elect_one()) {
+            const uint32_t idesc = i8_idesc(tokens) + (8u << 24);  // M = 256
+            int s = 0;
+            uint32_t ph = 0;
+            bool ok = true;
+            for (int ks = ks0; ks < ks1; ks++) {
+                if (!(ok = mbar_wait(full + 8 * s, ph, abort_flag))) break;
+                tc_fence_after();
+                const uint32_t st = smem_u32(smem + s * kI8PairStage);
+                const uint64_t ad = i8_desc(st), bd = i8_desc(st + 128 * 128);
+#pragma unroll
+                for (int kk = 0; kk < 4; kk++) umma_i8_pair(tmem, ad + 2 * kk, bd + 2 * kk, idesc, (ks != ks0 || kk != 0) ? 1u : 0u);
+                umma_commit_pair_at(empty + 8 * s, even);
+                if (++s == kI8PairStages) { s = 0; ph ^= 1; }
+            }
+            if (ok) umma_commit_pair_at(sums, even);
+        }
+    } else {
+        // two times four warps park sixteen tokens in turn
+        constexpr int C = 16;
+        const int q = warp & 3;
+        int* const park = reinterpret_cast<int*>(smem) + 32 * q + lane;  // [token][128 features]
+        if (__all_sync(0xffffffffu, mbar_wait(sums, 0, abort_flag))) {
+            tc_fence_after();
+            const uint32_t t0 = tmem + ((uint32_t)(32 * q) << 16);
+            for (int c0 = C * ((warp - 2) >> 2); c0 < rows; c0 += 2 * C) {
+                uint32_t r[C];
+                tmem_ld(t0 + c0, r);
+                tmem_ld_wait();
+#pragma unroll
+                for (int j = 0; j < C; j++) park[(c0 + j) * 128] = (int)r[j];
+            }
+        }
+    }
+    __syncwarp();
+    pdl_wait();
+    if (u0 + (int)threadIdx.x < u1) unit_scales(u0 + (int)threadIdx.x);
+    if (*abort_flag && warp == 0) {  // copies in flight land before the shared memory is given back
+        const long long t0 = clock64();
+        while (clock64() - t0 < 2000000) {}
+    }
+    tc_fence_before();
+    __syncthreads();
+    cluster_sync_all();  // every CTA's sums lie in its shared memory
+    if (!*abort_flag) i8_shares<SPLIT, kI8PairThreads, 2>(p, smem_u32(smem), half, u0 + (int)threadIdx.x, u1, row0, n0, unit_sx, unit_sw);
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");  // (nobody reads this CTA's shared memory any more)
+    if (*abort_flag && threadIdx.x == 0 && p.status != nullptr) atomicExch(p.status, kErrTimeout);
+    if (warp == 1) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256) : "memory");
+    }
+}
+
 struct I8Entry {
     int bn;
     void (*fn)(const CUtensorMap, const CUtensorMap, const I8Params);
@@ -479,18 +629,29 @@ template <int BN>
 constexpr I8Entry i8_entry() { return I8Entry{BN, i8_cluster_kernel<BN>, I8Tile<BN>::SMEM}; }
 const I8Entry kI8[] = {i8_entry<16>(), i8_entry<32>(), i8_entry<64>()};
 
-// How a call is divided. Up to 128 rows clusters, which hide the weights' way from memory; beyond the cheaper of the two by estimates in ns: a
-// step of a pair on h tokens takes 200 + 0.72 h, of a cluster's CTA on 64 tokens (two per SM) 330, the start and the last tile's results 4000 +
-// 8 h and 5000. Measured / estimated, us: 256 x 4096 x 4096 clusters 12.3 / 10.3, pairs 12.5 / 12.4; 256 x 14336 x 4096 27.7 / 26.1, 22.1 / 18.3; 256 x 4096 x
-// 14336 25.1 / 23.5, 30.7 / 32.1; 512 x 4096 x 4096 clusters 15.6 (estimated), pairs 14.4 / 14.3. The pairs' tiles over the rows are of two heights, 32
-// apart, so that any number of them can be had: sixteen times nine fill 74 pairs twice, sixteen times eight (of 256 tokens) did so to 86 %.
+// How a call is divided. Up to 128 rows clusters, which hide the weights' way from memory; beyond the cheapest by estimates in ns. A step on h tokens per
+// tile takes a pair 180 + 0.5 h (and 0.6 more for each beyond 128), one of the pairs that divide a tile's steps 150 + 30 s + 0.4 h, a cluster's CTA on 64 tokens (two per
+// SM) 330; start and end 4000 + 8 h, 3000 + 23 h (all of a tile's sums pass through shared memory), 5000 (one CTA alone 3700). Measured / estimated, us:
+//                        clusters       pairs          two pairs      three pairs
+//   256 x 4096 x 4096     10.6 / 10.3    11.0 / 11.3    10.2 / 10.2    12.1 / 12.3
+//   512 x 4096 x 4096     13.2 / 14.3    13.0 / 12.9    13.9 / 13.9
+//   256 x 4096 x 14336    23.2 / 23.5    26.9 / 28.3    20.1 / 20.6    21.0 / 21.9
+//   512 x 4096 x 14336    37.1 / 40.7    30.2 / 32.4    26.3 / 26.4
+//   160 x 4096 x 14336    22.9 / 23.5    26.7 / 27.9    18.7 / 18.4    17.9 / 18.3
+//   3186 x 256 x 12928    21.7 / 21.8    24.9 / 25.9    17.6 / 18.0    16.2 / 16.5
+// Four pairs were no better than three anywhere (15 clusters of eight CTAs run at once: 3186 x 256 x 12928 16.1, 703 x 1136 x 9216 13.9 against 13.0).
+// The pairs' tiles over the rows are of two heights, 32 apart, so that any number of them can be had: sixteen times nine fill 74 pairs twice, sixteen times eight
+// (of 256 tokens) did so to 86 %.
 struct I8Plan {
     bool pair;
     int rows, tall;  // tokens of a tile; pairs: of the first `tall` over the rows, the others have 32 fewer
     int m_tiles;
     int64_t tiles;
-    int parts;  // pieces of k, the CTAs of a cluster
+    int parts;  // pieces of k: the CTAs of a cluster, or its pairs
 };
+// Clusters of so many CTAs that run at once, where an SM holds so many: each stays in one group of SMs. (Measured on 148 SMs: of four CTAs 33, 71 and 104 with one, two
+// and three per SM, of six 22, of eight 33 and 48.)
+int i8_at_once(int ctas, int per_sm, int sms) { return sms * 11 / 12 / ctas * per_sm; }
 I8Plan i8_plan(int rows, int n, int k, int sms) {
     const int64_t steps = (k + 127) / 128;
     I8Plan c;
@@ -500,19 +661,25 @@ I8Plan i8_plan(int rows, int n, int k, int sms) {
     c.tall = c.m_tiles;
     c.tiles = (int64_t)c.m_tiles * ((n + 127) / 128);
     c.parts = 1;
-    // (a division costs about 1 us: 37 x 1024 x 1024, eight steps, 4.2 us whole and 4.8 in four; 23 steps of 37 x 2880 x 2880 8.4 and 6.4)
-    while (steps > 8 && c.parts < 8 && c.tiles * c.parts <= sms && steps >= 4 * c.parts) c.parts *= 2;
+    // (a division costs about 1 us: 37 x 1024 x 1024, eight steps, 4.2 us whole and 4.8 in four; 23 steps of 37 x 2880 x 2880 8.4 and 6.4. Clusters that do not
+    // run at once: 64 x 4736 x 4096, 37 tiles, 8.7 us in four parts and 12.5 in eight, 64 x 9216 x 4096, 72 tiles, 12.1 in two and 15.8 in four)
+    while (steps > 8 && c.parts < 8 && c.tiles * c.parts <= sms && steps >= 4 * c.parts && (c.parts == 1 || c.tiles <= i8_at_once(2 * c.parts, c.rows == 16 ? 3 : 2, sms)))
+        c.parts *= 2;
     if (rows <= 128 || sms % 2 != 0 || c.tiles > kI8Most) return c;
-    int64_t least = (c.tiles * c.parts + 2 * sms - 1) / (2 * sms) * (steps / c.parts) * 330 + 5000;
+    int64_t least = (c.tiles * c.parts + 2 * sms - 1) / (2 * sms) * (steps / c.parts) * 330 + (c.parts > 1 ? 5000 : 3700);
     const int n_tiles = (n + 255) / 256, groups = (rows + 31) / 32;
     for (int m = (groups + 7) / 8; m <= (groups + 1) / 2; m++) {
         const int high = (groups + m - 1) / m;  // groups of 32 tokens
-        const int64_t rounds = ((int64_t)m * n_tiles + sms / 2 - 1) / (sms / 2), h = rows / m;
-        const int64_t cost = rounds * steps * (20000 + 72 * h) / 100 + 4000 + 8 * h;
-        if (cost < least) {
+        const int64_t tiles = (int64_t)m * n_tiles, rounds = (tiles + sms / 2 - 1) / (sms / 2), h = rows / m;
+        const int64_t whole = rounds * steps * (1800 + 5 * h + 6 * std::max<int64_t>(h - 128, 0)) / 10 + 4000 + 8 * h;
+        auto take = [&](int64_t cost, int parts) {
+            if (cost >= least) return;
             least = cost;
-            c = I8Plan{true, 32 * high, groups - m * (high - 1), m, (int64_t)m * n_tiles, 1};
-        }
+            c = I8Plan{true, 32 * high, groups - m * (high - 1), m, tiles, parts};
+        };
+        take(whole, 1);
+        for (int s = 2; s <= 3; s++)
+            if (steps >= 4 * s && tiles <= i8_at_once(2 * s, 1, sms)) take((steps + s - 1) / s * (1500 + 300 * s + 4 * h) / 10 + 3000 + 23 * h, s);
         if (rounds > 64) break;  // (finer tiles only cost)
     }
     return c;
@@ -525,8 +692,11 @@ int32_t i8_init(iq_ctx* ctx) {
         const cudaError_t r = cudaFuncSetAttribute(reinterpret_cast<const void*>(e.fn), cudaFuncAttributeMaxDynamicSharedMemorySize, e.smem);
         if (r != cudaSuccess) return check_cuda(ctx, r, "cudaFuncSetAttribute(i8)");
     }
-    const cudaError_t r = cudaFuncSetAttribute(reinterpret_cast<const void*>(i8_pair_kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kI8PairSmem);
-    return check_cuda(ctx, r, "cudaFuncSetAttribute(i8_pair)");
+    for (auto kernel : {i8_pair_kernel, i8_split_kernel<2>, i8_split_kernel<3>}) {
+        const cudaError_t r = cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, kI8PairSmem);
+        if (r != cudaSuccess) return check_cuda(ctx, r, "cudaFuncSetAttribute(i8_pair)");
+    }
+    return kOk;
 }
 
 }  // namespace iq
@@ -576,6 +746,10 @@ extern "C" int32_t iq_qmm_i8(iq_ctx* ctx, void* stream, const int8_t* x, int64_t
     if (st == kOk) st = make_map_2d(ctx, &mw, w, 0, (uint64_t)k, (uint64_t)n, (uint64_t)k, 128, 128, true);
     if (st != kOk) return st;
     cudaStream_t cs = reinterpret_cast<cudaStream_t>(stream);
+    if (plan.pair && plan.parts > 1)
+        return check_cuda(ctx, launch_dependent(plan.parts == 2 ? i8_split_kernel<2> : i8_split_kernel<3>, dim3((unsigned)(plan.tiles * plan.parts * 2)), kI8PairThreads,
+                                                kI8PairSmem, cs, mx, mw, p),
+                          "qmm_i8 launch");
     if (plan.pair)
         return check_cuda(ctx, launch_dependent(i8_pair_kernel, dim3((unsigned)std::min<int64_t>(plan.tiles, ctx->sms / 2) * 2), kI8PairThreads, kI8PairSmem, cs, mx, mw, p),
                           "qmm_i8 launch");

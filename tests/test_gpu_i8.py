@@ -69,15 +69,18 @@ def test_many_tiles(cuda_device, rows, n, k):
     run(torch.Generator().manual_seed(rows), rows, n, k, BF16)
 
 
-@pytest.mark.parametrize("rows,n,k,height,tall", [(429, 4730, 384, 64, 7), (221, 1280, 256, 64, 3), (180, 18944, 384, 96, 2), (1174, 1280, 1040, 96, 9), (625, 14336, 528, 128, 5),
-                                                  (680, 9472, 256, 128, 4), (470, 18944, 256, 160, 3), (1954, 2560, 384, 160, 6), (173, 18944, 528, 192, 1), (1971, 4730, 1040, 192, 7),
-                                                  (870, 18944, 256, 224, 4), (2160, 9472, 384, 224, 8), (246, 18944, 1040, 256, 1), (1902, 9472, 256, 256, 4)])
+@pytest.mark.parametrize("rows,n,k,parts,height,tall", [
+    (129, 4730, 1040, 1, 64, 2), (1174, 1280, 1040, 1, 96, 9), (300, 4730, 2064, 1, 128, 1), (600, 4096, 528, 1, 160, 3), (1954, 2560, 384, 1, 160, 6), (1902, 9472, 256, 1, 160, 12),
+    (173, 18944, 528, 1, 192, 1), (999, 6144, 528, 1, 192, 2), (600, 4730, 1040, 1, 224, 1), (2160, 9472, 384, 1, 224, 8), (700, 6144, 1040, 1, 256, 1),
+    (129, 256, 1040, 2, 64, 2), (173, 256, 1040, 2, 64, 3), (200, 2049, 1040, 2, 96, 1), (300, 2049, 2064, 2, 128, 1), (999, 1280, 4096, 2, 192, 2), (700, 2049, 8208, 2, 256, 1),
+    (129, 256, 2064, 3, 64, 2), (470, 640, 2064, 3, 96, 1), (246, 2049, 8208, 3, 128, 2), (1500, 300, 8208, 3, 160, 3), (2048, 300, 8208, 3, 192, 9), (470, 2049, 14336, 3, 256, 1)])
 @pytest.mark.parametrize("dtype,accumulate", [(F32, True), (F16, False)])
-def test_pairs(cuda_device, rows, n, k, height, tall, dtype, accumulate):
-    """Pairs of CTAs on tiles of every height, of one and of two heights, the last of them short, more than one tile per pair."""
+def test_pairs(cuda_device, rows, n, k, parts, height, tall, dtype, accumulate):
+    """Pairs of CTAs on tiles of every height, of one and of two heights, the last of them short, more than one tile per pair; two and three pairs per tile."""
     plan = capi.qmm_i8_plan(rows, n, k)
-    assert plan.pair == 1 and plan.tile_rows == height and plan.tall == tall
+    assert plan.pair == 1 and (plan.parts, plan.tile_rows, plan.tall) == (parts, height, tall)
     run(torch.Generator().manual_seed(rows), rows, n, k, dtype, accumulate, 1)
+    run(torch.Generator().manual_seed(rows), rows, n, k, dtype, accumulate, 0)
 
 
 def test_the_largest_sums(cuda_device):
@@ -101,10 +104,10 @@ def test_a_row_does_not_depend_on_the_others(cuda_device):
         assert torch.equal(part, y[lo:hi])
 
 
-@pytest.mark.parametrize("rows", [3, 400])
-def test_streams_and_graphs(cuda_device, rows):
+@pytest.mark.parametrize("rows,k", [(3, 1024), (400, 1024), (400, 2048)])
+def test_streams_and_graphs(cuda_device, rows, k):
     gen = torch.Generator().manual_seed(4)
-    n, k = 520, 1024
+    n = 520
     x, w = codes(gen, rows, k).cuda(), codes(gen, n, k).cuda()
     sx, sw = torch.rand(rows, generator=gen).cuda(), torch.rand(n, generator=gen).cuda()
     m, y = I8Linear(w, sw), torch.zeros(rows, n, device="cuda")
@@ -212,7 +215,7 @@ def test_streams_at_once(cuda_device):
     VQMV.encode(dx, dense, dy, 8)
     dense_want = dy.clone()
     jobs = []
-    for rows, n, k in ((1, 1024, 4096), (40, 512, 4096), (300, 1024, 1024), (64, 1000, 2048)):
+    for rows, n, k in ((1, 1024, 4096), (40, 512, 4096), (300, 1024, 1024), (64, 1000, 2048), (200, 600, 2064), (200, 600, 1040)):
         x, sx = codes(gen, rows, k).cuda(), torch.rand(rows, generator=gen).cuda()
         m = I8Linear(codes(gen, n, k).cuda(), torch.rand(n, generator=gen).cuda())
         want = torch.empty(rows, n, device="cuda")

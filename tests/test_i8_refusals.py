@@ -60,16 +60,16 @@ def test_pack_entry(change, rotate, status):
 def test_the_plan():
     """Every tile is covered once, and each of the ways is taken by some shape that the GPU tests run."""
     seen = set()
-    for rows in (1, 9, 17, 64, 128, 129, 256, 300, 700, 2048, 4100):
-        for n, k in ((1, 16), (256, 512), (300, 1040), (4096, 4096), (1030, 512), (4096, 14336), (256, 256), (1500, 1024)):
+    for rows in (1, 9, 17, 64, 128, 129, 160, 256, 300, 700, 2048, 4100):
+        for n, k in ((1, 16), (256, 512), (300, 1040), (4096, 4096), (1030, 512), (4096, 14336), (256, 256), (1500, 1024), (704, 9216)):
             p = capi.qmm_i8_plan(rows, n, k)
             assert p.tiles == p.row_tiles * -(-n // (256 if p.pair else 128)) and 1 <= p.tall <= p.row_tiles
             whole = p.row_tiles * p.tile_rows - 32 * (p.row_tiles - p.tall)  # the rows of the tiles
             assert rows <= whole and (whole - rows < 32 if p.pair else p.tall == p.row_tiles and whole - rows < p.tile_rows)
-            assert 1 <= p.parts <= 8 and (p.parts == 1 or not p.pair) and p.parts <= -(-k // 128)
+            assert 1 <= p.parts <= (3 if p.pair else 8) and p.parts <= -(-k // 128)
             assert p.tile_rows % 32 == 0 and 32 <= p.tile_rows - 32 * (p.tall < p.row_tiles) and p.tile_rows <= 256 if p.pair else p.tile_rows in (16, 32, 64)
             seen.add((p.pair, p.tile_rows if p.pair else 0, p.parts))
-    assert {c[2] for c in seen} == {1, 2, 4, 8} and len({c[1] for c in seen if c[0]}) >= 4
+    assert {c[2] for c in seen if not c[0]} == {1, 2, 4, 8} and {c[2] for c in seen if c[0]} == {1, 2, 3} and len({c[1] for c in seen if c[0]}) >= 4
     for bad in ((0, 1, 16), (1, 0, 16), (1, 1, 24), (1, 1, 131072)):
         with pytest.raises(capi.IngotError):
             capi.qmm_i8_plan(*bad)
