@@ -137,30 +137,110 @@ __device__ __forceinline__ float max_abs8(float m, const float (&u)[8]) {
     return m;
 }
 
-// Butterflies of spans FROM, 2 FROM, ... below TO inside a thread, and between lanes h apart: a + b in the lower one, a - b in the upper one,
-// one rounding each.
-template <int FROM, int TO>
-__device__ __forceinline__ void rotate_spans(float (&u)[8]) {
+// Two neighbouring values per instruction, each rounded as by itself
+typedef unsigned long long Two;
+__device__ __forceinline__ Two two(float lo, float hi) {
+    Two r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ void apart(Two t, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(t)); }
+__device__ __forceinline__ Two add2(Two a, Two b) {
+    Two r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Two mul2(Two a, Two b) {
+    Two r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// PACKED: two per instruction. (Where the memory is the bound the moves into pairs of registers cost more than they save: 4096 rows of 4096, norm alone, 32.0 us one by
+// one and 36.8 in pairs.)
+template <bool PACKED>
+__device__ __forceinline__ void add8(float (&a)[8], const float (&b)[8]) {
 #pragma unroll
-    for (int h = FROM; h < TO; h <<= 1)
+    for (int j = 0; j < 8; j += 2) {
+        if (PACKED) {
+            apart(add2(two(a[j], a[j + 1]), two(b[j], b[j + 1])), a[j], a[j + 1]);
+        } else {
+            a[j] = __fadd_rn(a[j], b[j]);
+            a[j + 1] = __fadd_rn(a[j + 1], b[j + 1]);
+        }
+    }
+}
+template <bool PACKED>
+__device__ __forceinline__ void mul8(const float (&a)[8], const float (&b)[8], float (&r)[8]) {
 #pragma unroll
-        for (int j = 0; j < 8; j++)
-            if ((j & h) == 0) {
-                const float a = u[j], b = u[j + h];
-                u[j] = __fadd_rn(a, b);
-                u[j + h] = __fsub_rn(a, b);
-            }
+    for (int j = 0; j < 8; j += 2) {
+        if (PACKED) {
+            apart(mul2(two(a[j], a[j + 1]), two(b[j], b[j + 1])), r[j], r[j + 1]);
+        } else {
+            r[j] = __fmul_rn(a[j], b[j]);
+            r[j + 1] = __fmul_rn(a[j + 1], b[j + 1]);
+        }
+    }
+}
+// The sum of eight squares: of the even ones and of the odd ones
+template <bool PACKED>
+__device__ __forceinline__ float squares8(const float (&v)[8]) {
+    float even, odd;
+    if (PACKED) {
+        Two s = mul2(two(v[0], v[1]), two(v[0], v[1]));
+#pragma unroll
+        for (int j = 2; j < 8; j += 2) s = fma2(two(v[j], v[j + 1]), two(v[j], v[j + 1]), s);
+        apart(s, even, odd);
+    } else {
+        even = __fmul_rn(v[0], v[0]);
+        odd = __fmul_rn(v[1], v[1]);
+#pragma unroll
+        for (int j = 2; j < 8; j += 2) {
+            even = __fmaf_rn(v[j], v[j], even);
+            odd = __fmaf_rn(v[j + 1], v[j + 1], odd);
+        }
+    }
+    return __fadd_rn(even, odd);
+}
+
+// Butterflies inside a thread, and between lanes h apart: a + b in the lower one, a - b in the upper one, one rounding each.
+// a, b -> a + b, a - b (the product with -1 is exact)
+__device__ __forceinline__ void butterfly2(float& a0, float& a1, float& b0, float& b1) {
+    const Two a = two(a0, a1), b = two(b0, b1);
+    apart(add2(a, b), a0, a1);
+    apart(fma2(b, two(-1.f, -1.f), a), b0, b1);
+}
+// spans 1, 2 and 4
+__device__ __forceinline__ void rotate_eight(float (&u)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+        const float a = u[j], b = u[j + 1];
+        u[j] = __fadd_rn(a, b);
+        u[j + 1] = __fsub_rn(a, b);
+    }
+#pragma unroll
+    for (int h = 2; h < 8; h <<= 1)
+#pragma unroll
+        for (int j = 0; j < 8; j += 2)
+            if ((j & h) == 0) butterfly2(u[j], u[j + 1], u[j + h], u[j + h + 1]);
 }
 __device__ __forceinline__ void rotate_lanes(float (&u)[8], int lane, int h) {
     const float sign = (lane & h) ? -1.f : 1.f;
 #pragma unroll
-    for (int j = 0; j < 8; j++) u[j] = fmaf(sign, u[j], __shfl_xor_sync(0xffffffffu, u[j], h));
+    for (int j = 0; j < 8; j += 2) {
+        const Two other = two(__shfl_xor_sync(0xffffffffu, u[j], h), __shfl_xor_sync(0xffffffffu, u[j + 1], h));
+        apart(fma2(two(sign, sign), two(u[j], u[j + 1]), other), u[j], u[j + 1]);
+    }
 }
 // Blocks of ROT inputs of which a thread has eight in a row
 template <int ROT>
 __device__ __forceinline__ void rotate8(float (&u)[8], int lane) {
     if (ROT == 1) return;
-    rotate_spans<1, 8>(u);
+    rotate_eight(u);
 #pragma unroll
     for (int h = 1; h < ROT / 8; h <<= 1) rotate_lanes(u, lane, h);
 }
@@ -172,11 +252,15 @@ __device__ __forceinline__ uint2 codes8(const float (&u)[8], float s, float inv)
     constexpr float kMagic = 12582912.f, kFar = 0.49998f;
     uint32_t m[8];
     float off[8];
+    const Two i2 = two(inv, inv), magic = two(kMagic, kMagic);
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
-        const float v = fmaf(u[j], inv, kMagic), n = v - kMagic;
-        m[j] = __float_as_uint(v);
-        off[j] = fmaf(u[j], inv, -n);
+    for (int j = 0; j < 8; j += 2) {
+        const Two v = fma2(two(u[j], u[j + 1]), i2, magic), minus_n = fma2(v, two(-1.f, -1.f), magic);
+        float a, b;
+        apart(v, a, b);
+        m[j] = __float_as_uint(a);
+        m[j + 1] = __float_as_uint(b);
+        apart(fma2(two(u[j], u[j + 1]), i2, minus_n), off[j], off[j + 1]);
     }
     if (!(max_abs8(0.f, off) <= kFar)) {
 #pragma unroll
@@ -221,8 +305,7 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
                 if (p.x != nullptr) {
                     float xv[8];
                     unpack8<HT>(xx[c], p.x_dtype, xv);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[c][j] += xv[j];
+                    add8<false>(v[c], xv);
                     const Raw8 stored = pack8<HT>(p.r_dtype, v[c]);
                     store8(p.r_out, p.r_dtype, row * p.ldro + at(c, 0), stored);
                     unpack8<HT>(stored, p.r_dtype, v[c]);
@@ -258,11 +341,7 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
     // The squares of 256 neighbouring values are a sum of their own, in an order that does not depend on the launch, and so are the sums' sum.
     float sums[NCH];
 #pragma unroll
-    for (int c = 0; c < NCH; c++) {
-        sums[c] = 0.f;
-#pragma unroll
-        for (int j = 0; j < 8; j++) sums[c] = fmaf(v[c][j], v[c][j], sums[c]);
-    }
+    for (int c = 0; c < NCH; c++) sums[c] = squares8<false>(v[c]);
     // w + offset of the thread's values
     auto weights = [&](int c, float (&w)[8]) {
 #pragma unroll
@@ -287,8 +366,7 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
         for (int c = 0; c < NCH; c++) {
             float w[8];
             weights(c, w);
-#pragma unroll
-            for (int j = 0; j < 8; j++) u[c][j] = __fmul_rn(v[c][j], w[j]);
+            mul8<false>(v[c], w, u[c]);
             if (!VEC && ROT > 1) {
                 float* const mine = turn + warp * 256;
 #pragma unroll
@@ -376,9 +454,9 @@ __global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant
 // groups of eight, 128 apart, so that spans 8 to 64 of a rotation go from lane to lane. The next row is under way into shared memory
 // meanwhile, copied by the warp that uses it, so that no barrier stands between copy and use. One barrier per row, the sums of two rows in turn.
 //
-// Bound: issue slots where codes are wanted (some 100 instructions per row and lane, 25 per rotated value), else the memory. 4096 rows of 4096,
-// bf16 added to bf16, us, the kernel of a row per block / this one: out 27.8 / 23.4 (floor 20.5), codes 32.3 / 21.9, rotated 44.3 / 28.0 (18.0); 7680 wide
-// 70 / 43.8, 80 / 39.7, 94 / 51.2. On the way: types chosen at run time 24.3, 27.6, 33.5, and addresses made per row 23.3, 29.3, 34.0; with one group
+// Bound: issue slots where codes are wanted (some 40 instructions per rotated value; operations on pairs of values saved 4 %), else the memory. 4096 rows of 4096,
+// bf16 added to bf16, us, the kernel of a row per block / this one: out 27.8 / 22.9 (floor 20.5), codes 32.3 / 21.1, rotated 44.3 / 26.9 (18.0); 7680 wide
+// 70 / 43.3, 80 / 37.1, 94 / 49.4. On the way: types chosen at run time 24.3, 27.6, 33.5, and addresses made per row 23.3, 29.3, 34.0; with one group
 // per lane then 26.2, 33.0, 37.4, with four 27.9, 30.5, 35.3, with a third stage 25.4, 29.5, 34.3.
 constexpr int kNormStages = 2;
 constexpr int kNormRowsSmem = 200 * 1024;  // of an SM's blocks
@@ -474,7 +552,6 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const __grid_con
         float v[K][8], sums[K];
 #pragma unroll
         for (int k = 0; k < K; k++) {
-            sums[k] = 0.f;
 #pragma unroll
             for (int j = 0; j < 8; j++) v[k][j] = 0.f;
             if (live[k]) {
@@ -482,15 +559,13 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const __grid_con
                 if (add) {
                     float xv[8];
                     unpack8<HT>(take(x_from + x_at + k * x.group_to, wide_x), x_dtype, xv);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) v[k][j] += xv[j];
+                    add8<CODES>(v[k], xv);
                     const Raw8 stored = pack8<HT>(r_dtype, v[k]);
                     store8(r_out + k * r.group_from, r_dtype, 0, stored);
                     if (!wide_r) unpack8<HT>(stored, r_dtype, v[k]);
                 }
             }
-#pragma unroll
-            for (int j = 0; j < 8; j++) sums[k] = fmaf(v[k][j], v[k][j], sums[k]);
+            sums[k] = squares8<CODES>(v[k]);
         }
         r_out += r_out_step;
         // (the order of the other kernel's lanes: 16, 8, 4, 2 and 1 groups apart)
@@ -502,26 +577,22 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const __grid_con
         float kept[OUT && CODES ? K : 1][8];  // r', where both outputs are wanted; v is u from here on
         if (CODES) {
 #pragma unroll
-            for (int k = 0; k < K; k++)
+            for (int k = 0; k < K; k++) {
 #pragma unroll
-                for (int j = 0; j < 8; j++) {
+                for (int j = 0; j < 8; j++)
                     if (OUT) kept[OUT ? k : 0][j] = v[k][j];
-                    v[k][j] = __fmul_rn(v[k][j], w[k][j]);
-                }
+                mul8<true>(v[k], w[k], v[k]);
+            }
             if (ROT > 1) {
 #pragma unroll
                 for (int k = 0; k < K; k++) {
-                    rotate_spans<1, 8>(v[k]);
+                    rotate_eight(v[k]);
 #pragma unroll
                     for (int h = 1; h < (ROT < APART ? ROT / 8 : LB); h <<= 1) rotate_lanes(v[k], lane, h);
                 }
                 if (ROT > APART) {
 #pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        const float a = v[0][j], b = v[1][j];
-                        v[0][j] = __fadd_rn(a, b);
-                        v[1][j] = __fsub_rn(a, b);
-                    }
+                    for (int j = 0; j < 8; j += 2) butterfly2(v[0][j], v[0][j + 1], v[1][j], v[1][j + 1]);
                 }
             }
 #pragma unroll
@@ -542,7 +613,7 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const __grid_con
                 if (live[k]) {
                     float o[8];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) o[j] = ((CODES ? kept[CODES ? k : 0][j] : v[k][j]) * q) * w[k][j];
+                    for (int j = 0; j < 8; j++) o[j] = ((CODES ? kept[OUT && CODES ? k : 0][j] : v[k][j]) * q) * w[k][j];
                     store8(out + k * APART * o_size, out_dtype, 0, pack8<HT>(out_dtype, o));
                 }
             out += out_step;
