@@ -276,7 +276,7 @@ __device__ __forceinline__ uint2 codes8(const float (&u)[8], float s, float inv)
 // neighbouring values, and where the rotation wants a thread to have eight in a row, they pass through shared memory.
 // CODES, ROT: int8 codes, rotated in blocks of ROT inputs (1: not).
 template <int NCH, int MAXT, bool VEC, bool CODES, int ROT, int HT>
-__global__ void __launch_bounds__(MAXT) add_rmsnorm_kernel(const __grid_constant__ NormParams p) {
+__global__ void __launch_bounds__(MAXT, MAXT < 1024 ? (NCH == 1 ? 1536 : 1024) / MAXT : 0) add_rmsnorm_kernel(const __grid_constant__ NormParams p) {
     constexpr int PARTS = NCH * MAXT / 32;  // runs of 256 values
     __shared__ float wsum[PARTS], wmax[32];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
@@ -658,11 +658,17 @@ NormKernel norm_pick(bool codes, int rotate) {
     return rotate == 256 ? add_rmsnorm_kernel<NCH, MAXT, VEC, true, 256, HT> : rotate == 32 ? add_rmsnorm_kernel<NCH, MAXT, VEC, true, 32, HT>
                                                                                             : add_rmsnorm_kernel<NCH, MAXT, VEC, true, 1, HT>;
 }
-template <int NCH, int MAXT>
-NormKernel norm_pick(bool vec, int half, bool codes, int rotate) {
-    if (!vec) return norm_pick<NCH, MAXT, false, kF32>(codes, rotate);
-    return half == kF16 ? norm_pick<NCH, MAXT, true, kF16>(codes, rotate) : half == kBF16 ? norm_pick<NCH, MAXT, true, kBF16>(codes, rotate)
-                                                                                          : norm_pick<NCH, MAXT, true, kF32>(codes, rotate);
+template <int NCH>
+NormKernel norm_pick(int half, bool codes, int rotate) {
+    return half == kF16 ? norm_pick<NCH, 1024, true, kF16>(codes, rotate) : half == kBF16 ? norm_pick<NCH, 1024, true, kBF16>(codes, rotate)
+                                                                                          : norm_pick<NCH, 1024, true, kF32>(codes, rotate);
+}
+// Rows that are not aligned: blocks of up to 512 threads, whose registers are held to what lets 1536 of them (with two groups each 1024) share an SM: more rows under
+// way at once. 2048 rows of 4095, bf16, 27.0 -> 22.4 us, 1024 of 7681 29.9 -> 26.1, 30,000 of 480 with rotated codes 113 -> 55.
+NormKernel norm_pick_unaligned(int groups, bool codes, int rotate) {
+    return groups <= 256 ? norm_pick<1, 256, false, kF32>(codes, rotate) : groups <= 512 ? norm_pick<1, 512, false, kF32>(codes, rotate)
+         : groups <= 1024 ? norm_pick<2, 512, false, kF32>(codes, rotate) : groups <= 2048 ? norm_pick<2, 1024, false, kF32>(codes, rotate)
+                                                                                          : norm_pick<4, 1024, false, kF32>(codes, rotate);
 }
 
 bool misplaced(const void* p, int esz) { return reinterpret_cast<uintptr_t>(p) % esz != 0; }
@@ -719,7 +725,7 @@ extern "C" int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int3
     p.rows = rows; p.d = d; p.offset = weight_offset; p.eps = eps;
     const bool vec = d % 8 == 0 && aligned(x, ldx, dtype_size(x_dtype)) && aligned(residual, ldr, dtype_size(r_dtype)) && aligned(residual_out, ldro, dtype_size(r_dtype)) &&
                      aligned(weight, 0, dtype_size(w_dtype)) && aligned(out, ldo, dtype_size(out_dtype)) && aligned(codes, ldc, 1);
-    const int groups = (d + 7) / 8, nch = groups <= 1024 ? 1 : groups <= 2048 ? 2 : 4;
+    const int groups = (d + 7) / 8, nch = groups <= (vec ? 1024 : 512) ? 1 : groups <= 2048 ? 2 : 4;
     int threads = round_up((groups + nch - 1) / nch, 32), blocks = rows;
     size_t smem = 0;
     // the one 16-bit type of the call (bf16 where it has none), kF32 where it has both
@@ -730,8 +736,8 @@ extern "C" int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int3
     meet(x, x_dtype); meet(residual, r_dtype); meet(weight, w_dtype); meet(out, out_dtype);
     if (half == -1) half = kBF16;
     const bool c8 = codes != nullptr;
-    NormKernel kernel = nch == 1 ? norm_pick<1, 1024>(vec, half, c8, rotate) : nch == 2 ? norm_pick<2, 1024>(vec, half, c8, rotate)
-                                                                                       : norm_pick<4, 1024>(vec, half, c8, rotate);
+    NormKernel kernel = !vec ? norm_pick_unaligned(groups, c8, rotate) : nch == 1 ? norm_pick<1>(half, c8, rotate) : nch == 2 ? norm_pick<2>(half, c8, rotate)
+                                                                                                                          : norm_pick<4>(half, c8, rotate);
     // Many rows: more than the blocks that run at once (of 64 registers a thread, the stages in shared memory). The norm alone of an fp32 sum is at the memory's
     // rate with a row per block as well up to some 5000 values (4096 rows of 4096: 31.9 us, floor 30.8; of 7680 75 us, here 64).
     const int row_threads = (d + 511) / 512 * 32;
