@@ -113,17 +113,20 @@ __device__ __forceinline__ void store8(void* p, int32_t dtype, size_t i, const R
 __device__ __forceinline__ uint32_t load1(const void* p, int32_t dtype, size_t i) {
     return dtype == kF32 ? static_cast<const uint32_t*>(p)[i] : (uint32_t)static_cast<const uint16_t*>(p)[i];
 }
+template <int HT>
 __device__ __forceinline__ float unpack1(uint32_t v, int32_t dtype) {
-    const float h = __half2float(__ushort_as_half((unsigned short)v)), b = bf16_bits_to_f32(v);
-    return dtype == kF32 ? __uint_as_float(v) : dtype == kBF16 ? b : h;
+    if (dtype == kF32) return __uint_as_float(v);
+    return known_type<HT>(dtype) == kBF16 ? bf16_bits_to_f32(v) : __half2float(__ushort_as_half((unsigned short)v));
 }
+template <int HT>
 __device__ __forceinline__ float round1(float v, int32_t dtype) {
     if (dtype == kF32) return v;
-    return dtype == kBF16 ? __bfloat162float(__float2bfloat16_rn(v)) : __half2float(__float2half_rn(v));
+    return known_type<HT>(dtype) == kBF16 ? __bfloat162float(__float2bfloat16_rn(v)) : __half2float(__float2half_rn(v));
 }
+template <int HT>
 __device__ __forceinline__ void store1(void* p, int32_t dtype, size_t i, float v) {
     if (dtype == kF32) static_cast<float*>(p)[i] = v;
-    else static_cast<uint16_t*>(p)[i] = dtype == kBF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
+    else static_cast<uint16_t*>(p)[i] = known_type<HT>(dtype) == kBF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v)) : __half_as_ushort(__float2half_rn(v));
 }
 // Largest magnitude of three, NaN if one of them is
 __device__ __forceinline__ float max_abs(float a, float b, float c) {
@@ -325,8 +328,8 @@ __global__ void __launch_bounds__(MAXT, MAXT < 1024 ? (NCH == 1 ? 1536 : 1024) /
             }
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                v[c][j] = unpack1(rr[j], p.r_dtype);
-                if (p.x != nullptr) v[c][j] = round1(v[c][j] + unpack1(xx[j], p.x_dtype), p.r_dtype);
+                v[c][j] = unpack1<HT>(rr[j], p.r_dtype);
+                if (p.x != nullptr) v[c][j] = round1<HT>(v[c][j] + unpack1<HT>(xx[j], p.x_dtype), p.r_dtype);
                 if (at(c, j) >= p.d) v[c][j] = 0.f;
             }
         }
@@ -335,7 +338,7 @@ __global__ void __launch_bounds__(MAXT, MAXT < 1024 ? (NCH == 1 ? 1536 : 1024) /
             for (int c = 0; c < NCH; c++)
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    if (at(c, j) < p.d) store1(p.r_out, p.r_dtype, row * p.ldro + at(c, j), v[c][j]);
+                    if (at(c, j) < p.d) store1<HT>(p.r_out, p.r_dtype, row * p.ldro + at(c, j), v[c][j]);
         }
     }
     // The squares of 256 neighbouring values are a sum of their own, in an order that does not depend on the launch, and so are the sums' sum.
@@ -354,7 +357,7 @@ __global__ void __launch_bounds__(MAXT, MAXT < 1024 ? (NCH == 1 ? 1536 : 1024) /
 #pragma unroll
             for (int j = 0; j < 8; j++) ww[j] = load1(p.w, p.w_dtype, min(at(c, j), p.d - 1));
 #pragma unroll
-            for (int j = 0; j < 8; j++) w[j] = unpack1(ww[j], p.w_dtype);
+            for (int j = 0; j < 8; j++) w[j] = unpack1<HT>(ww[j], p.w_dtype);
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) w[j] = __fadd_rn(w[j], p.offset);
@@ -413,7 +416,7 @@ __global__ void __launch_bounds__(MAXT, MAXT < 1024 ? (NCH == 1 ? 1536 : 1024) /
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; j++)
-                    if (at(c, j) < p.d) store1(p.out, p.out_dtype, row * p.ldo + at(c, j), o[j]);
+                    if (at(c, j) < p.d) store1<HT>(p.out, p.out_dtype, row * p.ldo + at(c, j), o[j]);
             }
         }
     }
@@ -664,11 +667,17 @@ NormKernel norm_pick(int half, bool codes, int rotate) {
                                                                                           : norm_pick<NCH, 1024, true, kF32>(codes, rotate);
 }
 // Rows that are not aligned: blocks of up to 512 threads, whose registers are held to what lets 1536 of them (with two groups each 1024) share an SM: more rows under
-// way at once. 2048 rows of 4095, bf16, 27.0 -> 22.4 us, 1024 of 7681 29.9 -> 26.1, 30,000 of 480 with rotated codes 113 -> 55.
+// way at once. 2048 rows of 4095, bf16, 27.0 -> 22.4 us, with the one 16-bit type known 20.8; 1024 of 7681 29.9 -> 26.1 -> 22.3; 30,000 of 480 with rotated codes
+// 113 -> 55 -> 51. Taken back: groups of eight out of aligned pieces of 16 bytes, shifted in registers (2048 rows of 4095 33.0).
+template <int HT>
 NormKernel norm_pick_unaligned(int groups, bool codes, int rotate) {
-    return groups <= 256 ? norm_pick<1, 256, false, kF32>(codes, rotate) : groups <= 512 ? norm_pick<1, 512, false, kF32>(codes, rotate)
-         : groups <= 1024 ? norm_pick<2, 512, false, kF32>(codes, rotate) : groups <= 2048 ? norm_pick<2, 1024, false, kF32>(codes, rotate)
-                                                                                          : norm_pick<4, 1024, false, kF32>(codes, rotate);
+    return groups <= 256 ? norm_pick<1, 256, false, HT>(codes, rotate) : groups <= 512 ? norm_pick<1, 512, false, HT>(codes, rotate)
+         : groups <= 1024 ? norm_pick<2, 512, false, HT>(codes, rotate) : groups <= 2048 ? norm_pick<2, 1024, false, HT>(codes, rotate)
+                                                                                        : norm_pick<4, 1024, false, HT>(codes, rotate);
+}
+NormKernel norm_pick_unaligned(int half, int groups, bool codes, int rotate) {
+    return half == kF16 ? norm_pick_unaligned<kF16>(groups, codes, rotate) : half == kBF16 ? norm_pick_unaligned<kBF16>(groups, codes, rotate)
+                                                                                           : norm_pick_unaligned<kF32>(groups, codes, rotate);
 }
 
 bool misplaced(const void* p, int esz) { return reinterpret_cast<uintptr_t>(p) % esz != 0; }
@@ -736,7 +745,7 @@ extern "C" int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int3
     meet(x, x_dtype); meet(residual, r_dtype); meet(weight, w_dtype); meet(out, out_dtype);
     if (half == -1) half = kBF16;
     const bool c8 = codes != nullptr;
-    NormKernel kernel = !vec ? norm_pick_unaligned(groups, c8, rotate) : nch == 1 ? norm_pick<1>(half, c8, rotate) : nch == 2 ? norm_pick<2>(half, c8, rotate)
+    NormKernel kernel = !vec ? norm_pick_unaligned(half, groups, c8, rotate) : nch == 1 ? norm_pick<1>(half, c8, rotate) : nch == 2 ? norm_pick<2>(half, c8, rotate)
                                                                                                                           : norm_pick<4>(half, c8, rotate);
     // Many rows: more than the blocks that run at once (of 64 registers a thread, the stages in shared memory). The norm alone of an fp32 sum is at the memory's
     // rate with a row per block as well up to some 5000 values (4096 rows of 4096: 31.9 us, floor 30.8; of 7680 75 us, here 64).
