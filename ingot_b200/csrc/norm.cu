@@ -747,16 +747,18 @@ extern "C" int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int3
     const bool c8 = codes != nullptr;
     NormKernel kernel = !vec ? norm_pick_unaligned(half, groups, c8, rotate) : nch == 1 ? norm_pick<1>(half, c8, rotate) : nch == 2 ? norm_pick<2>(half, c8, rotate)
                                                                                                                           : norm_pick<4>(half, c8, rotate);
-    // Many rows: more than the blocks that run at once (of 64 registers a thread, the stages in shared memory). The norm alone of an fp32 sum is at the memory's
+    // Many rows: a third more than the other kernel runs at once (64 registers a thread). 512 rows of 4096, codes of a bf16 sum, 6.8 us there and 5.2 here, 257 rows
+    // 3.9 and 4.8; 200 of 7680 6.9 and 5.1, 148 3.9 and 3.6; 600 of 2048 4.4 and 4.9, 1000 5.7 and 5.2. Blocks: those that run at once, by registers and by the
+    // stages in shared memory. The norm alone of an fp32 sum is at the memory's
     // rate with a row per block as well up to some 5000 values (4096 rows of 4096: 31.9 us, floor 30.8; of 7680 75 us, here 64).
     const int row_threads = (d + 511) / 512 * 32;
     const size_t row_smem = (size_t)kNormStages * row_threads * 16 * (dtype_size(r_dtype) + (x == nullptr ? 0 : dtype_size(x_dtype)));
     const int at_once = row_threads > 1024 ? 0 : ctx->sms * (int)std::min<size_t>({(size_t)(1024 / row_threads), kNormRowsSmem / row_smem, 16});
-    if (vec && at_once > 0 && rows > at_once && (c8 || r_dtype != kF32 || d > 5120)) {
+    if (vec && at_once > 0 && rows > ctx->sms * std::max(1024 / threads, 1) * 4 / 3 && (c8 || r_dtype != kF32 || d > 5120)) {
         const bool x16 = x != nullptr && x_dtype != kF32 && (out == nullptr || out_dtype != kF32);
         kernel = norm_pick_rows(half, !x16 ? kAnyTypes : r_dtype == kF32 ? kSum32 : kSum16, out != nullptr, c8, rotate);
         threads = row_threads;
-        blocks = at_once;
+        blocks = std::min(rows, at_once);
         smem = row_smem;
     }
     DeviceScope on(ctx);

@@ -228,10 +228,10 @@ def test_refusals_reach_no_kernel(cuda_device):
 
 
 @pytest.mark.parametrize("rows,d,xt,rt,wt,ot,rotate,out,codes", [
-    (2400, 512, BF16, BF16, BF16, BF16, 256, True, True), (2400, 520, F16, F32, F32, F16, 0, False, True), (700, 2880, F16, F16, F16, F32, 32, True, True),
+    (3300, 512, BF16, BF16, BF16, BF16, 256, True, True), (3300, 520, F16, F32, F32, F16, 0, False, True), (700, 2880, F16, F16, F16, F32, 32, True, True),
     (700, 4096, BF16, F32, BF16, BF16, 256, False, True), (650, 4096, BF16, BF16, BF16, BF16, 0, True, False), (500, 5128, None, F32, None, F16, 0, True, False),
     (460, 7680, F32, F16, BF16, F32, 256, True, True), (300, 8192, F32, F32, F32, F32, 32, False, True), (160, 16384, BF16, BF16, BF16, BF16, 256, False, True),
-    (160, 14344, BF16, BF16, F32, BF16, 0, True, True), (160, 16384, F32, F32, F32, F32, 0, True, True)])
+    (200, 14344, BF16, BF16, F32, BF16, 0, True, True), (200, 16384, BF16, BF16, BF16, BF16, 256, False, True), (160, 16384, F32, F32, F32, F32, 0, True, True)])
 def test_the_kernel_of_many_rows(cuda_device, rows, d, xt, rt, wt, ot, rotate, out, codes):
     """More rows than blocks that run at once, up to more than two per block; the bits of a row are those of a call of its own."""
     gen = torch.Generator().manual_seed(rows + d)
@@ -308,3 +308,11 @@ def test_two_streams_at_once(cuda_device):
 def test_tensors_of_no_rows(cuda_device):
     none = torch.empty(0, 64, device="cuda")
     add_rmsnorm(none, none, None, 0, out=none, codes=torch.empty(0, 64, dtype=torch.int8, device="cuda"), scales=torch.empty(0, device="cuda"))
+
+
+@pytest.mark.parametrize("rows,d,pad,rotate", [(3, 1024, 7, 256), (5, 1999, 0, 0), (2, 4103, 2, 0), (3, 6144, 7, 256), (2, 14337, 0, 0), (2, 14336, 7, 32), (1500, 480, 7, 32), (1700, 2047, 0, 0)])
+@pytest.mark.parametrize("xt,rt,wt,ot", [(BF16, BF16, BF16, BF16), (F16, F32, F16, F16), (F32, F16, BF16, F32)])
+def test_rows_that_are_not_aligned(cuda_device, rows, d, pad, rotate, xt, rt, wt, ot):
+    """Blocks of every size, one and two 16-bit types."""
+    gen = torch.Generator().manual_seed(rows + d + pad)
+    check(run(gen, rows, d, xt, rt, wt, ot, rotate, pad), 0.0, 1e-6, rotate)
