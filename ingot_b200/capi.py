@@ -233,6 +233,9 @@ def call():
         for name in ("iq_qmv", "iq_qmm", "iq_dense_ffn", "iq_moe_forward", "iq_rmsnorm", "iq_had_rows", "iq_embed_rows",
                      "iq_argmax_rows", "iq_topk64", "iq_add_rmsnorm", "iq_qmm_i8", "iq_logits_rules"):
             mod.bind(name, C.cast(getattr(l, name), C.c_void_p).value)
+        import torch  # (this module is of use without it)
+
+        mod.bind_types(torch.float32, torch.float16, torch.bfloat16, torch.int8)
         _call = mod
     return _call
 

@@ -1,7 +1,7 @@
 /* The hot entry points of libingot_qmm.so as CPython functions. A ctypes call converts every argument through its argtypes
  * object: 2.3 us for iq_qmv, half of what a decode linear of a few megabytes takes on the GPU; through METH_FASTCALL it is
- * 0.3 us. Arguments are integers (addresses, sizes, flags) and, where the C signature has them, floats; the result is the
- * status. The library is already loaded (capi.lib()); bind(name, address) hands over the symbols. */
+ * 0.3 us. Arguments are integers (addresses, sizes, flags) and, where the C signature has them, floats, or (the last three entries) tensors; the
+ * result is the status. The library is already loaded (capi.lib()); bind(name, address) hands over the symbols. */
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 #include <stdint.h>
@@ -159,40 +159,180 @@ ENTRY(topk64, 13, topk_t, {
     LAUNCH(f(c, s, x, ldx, rows, vocab, t, nt, ix, v, z, sc, sb));
 })
 
+/* ---- entry points that take the tensors themselves ----------------------------------------------------------------------------
+ * What a tensor says of itself is asked for here: from Python its shape, strides, type, device and address and the conditions on them cost as much as
+ * the launch. A tensor that is not as the entry wants it makes the result None, before anything is launched; the caller then says why. */
+static PyObject *s_shape, *s_stride, *s_dtype, *s_get_device, *s_data_ptr, *s_numel, *s_is_contiguous;
+static PyObject* types[4]; /* float32, float16, bfloat16 in the order of iq_dtype, int8 */
+
+typedef struct {
+    void* p;
+    int64_t rows, cols, ld; /* [rows, cols], rows ld elements apart; one dimension: [rows] */
+    int type;               /* index in types, -1: none of them */
+} Rows;
+
+static int number(PyObject* o, int64_t* v) {
+    if (o == NULL) return -1;
+    *v = (int64_t)PyLong_AsUnsignedLongLongMask(o);
+    Py_DECREF(o);
+    return PyErr_Occurred() ? -1 : 0;
+}
+static int type_of(PyObject* t) {
+    PyObject* d = PyObject_GetAttr(t, s_dtype);
+    int i = 3;
+    if (d == NULL) return -1;
+    while (i >= 0 && types[i] != d) i--;
+    Py_DECREF(d);
+    return i;
+}
+/* A tensor of `dims` (one or two) dimensions on the device, of two with neighbouring elements in a row. 0: o is filled. */
+static int rows_of(PyObject* t, int dims, int64_t device, Rows* o) {
+    int64_t dev, addr, size[2] = {0, 0}, step[2] = {0, 0};
+    PyObject *shape = PyObject_GetAttr(t, s_shape), *stride = NULL;
+    int ok = 0;
+    if (shape == NULL || !PyTuple_Check(shape) || PyTuple_GET_SIZE(shape) != dims) goto out;
+    stride = PyObject_CallMethodNoArgs(t, s_stride);
+    if (stride == NULL || !PyTuple_Check(stride) || PyTuple_GET_SIZE(stride) != dims) goto out;
+    for (int i = 0; i < dims; i++) {
+        size[i] = (int64_t)PyLong_AsUnsignedLongLongMask(PyTuple_GET_ITEM(shape, i));
+        step[i] = (int64_t)PyLong_AsUnsignedLongLongMask(PyTuple_GET_ITEM(stride, i));
+    }
+    if (PyErr_Occurred() || number(PyObject_CallMethodNoArgs(t, s_get_device), &dev) || dev != device || number(PyObject_CallMethodNoArgs(t, s_data_ptr), &addr)) goto out;
+    if (dims == 2 && step[1] != 1 && size[1] > 1) goto out;
+    o->p = (void*)(uintptr_t)addr;
+    o->rows = size[0];
+    o->cols = dims == 2 ? size[1] : 1;
+    o->ld = step[0];
+    o->type = type_of(t);
+    ok = 1;
+out:
+    Py_XDECREF(shape);
+    Py_XDECREF(stride);
+    return ok ? 0 : -1;
+}
+static PyObject* not_taken(void) {
+    PyErr_Clear();
+    Py_RETURN_NONE;
+}
+#define TENSORS(NAME, COUNT)                                                                    \
+    if (n != COUNT || fn_##NAME == NULL || types[0] == NULL) {                                  \
+        PyErr_SetString(PyExc_TypeError, #NAME ": wrong number of arguments, or not bound");    \
+        return NULL;                                                                            \
+    }
+#define FLOATS(T) ((T).type >= 0 && (T).type <= 2)
+
+static PyObject* py_bind_types(PyObject* self, PyObject* args) {
+    PyObject* t[4];
+    (void)self;
+    if (!PyArg_ParseTuple(args, "OOOO", &t[0], &t[1], &t[2], &t[3])) return NULL;
+    for (int i = 0; i < 4; i++) {
+        Py_INCREF(t[i]);
+        types[i] = t[i];
+    }
+    Py_RETURN_NONE;
+}
+
 typedef int32_t (*add_norm_t)(iq_ctx*, void*, const void*, int32_t, int64_t, const void*, int32_t, int64_t, void*, int64_t, const void*, int32_t,
                               float, float, int32_t, int32_t, void*, int32_t, int64_t, int8_t*, int64_t, float*, int32_t);
-ENTRY(add_rmsnorm, 23, add_norm_t, {
-    void *c = P(0), *s = P(1), *x = P(2), *r = P(5), *ro = P(8), *w = P(10), *o = P(16), *q = P(19), *sc = P(21);
-    int32_t xd = I32(3), rd = I32(6), wd = I32(11), rows = I32(14), d = I32(15), od = I32(17), rot = I32(22);
-    int64_t ldx = I64(4), ldr = I64(7), ldro = I64(9), ldo = I64(18), ldc = I64(20);
-    float off = F32(12), eps = F32(13);
-    CHECKED;
-    LAUNCH(f(c, s, x, xd, ldx, r, rd, ldr, ro, ldro, w, wd, off, eps, rows, d, o, od, ldo, q, ldc, sc, rot));
-})
+/* (context, stream, device, x, residual, weight, rows, eps, weight_offset, residual_out, out, codes, scales, rotate) */
+static PyObject* py_add_rmsnorm(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    TENSORS(add_rmsnorm, 14);
+    (void)self;
+    void *c = P(0), *s = P(1), *w = NULL;
+    const int64_t device = I64(2), rows = I64(6), rotate = I64(13);
+    const double eps = PyFloat_AsDouble(a[7]), offset = PyFloat_AsDouble(a[8]);
+    Rows x = {0}, r, ro = {0}, o = {0}, q = {0}, sc = {0};
+    int wd = 0;
+    if (PyErr_Occurred()) return not_taken();
+    if (rows_of(a[4], 2, device, &r) || !FLOATS(r) || rows < 0 || r.rows < rows || r.cols < 1 || r.cols > 32768 || !(eps >= 0)) return not_taken();
+#define LIKE(T) ((T).rows >= rows && (T).cols == r.cols)
+    if (a[3] != Py_None) {
+        if (rows_of(a[3], 2, device, &x) || !FLOATS(x) || !LIKE(x)) return not_taken();
+        ro = r;
+        if (a[9] != Py_None && (rows_of(a[9], 2, device, &ro) || ro.type != r.type || !LIKE(ro))) return not_taken();
+    } else if (a[9] != Py_None) {
+        return not_taken();
+    }
+    if (a[5] != Py_None) {
+        int64_t dev, numel, addr;
+        PyObject* whole = PyObject_CallMethodNoArgs(a[5], s_is_contiguous);
+        Py_XDECREF(whole);
+        wd = type_of(a[5]);
+        if (whole != Py_True || wd < 0 || wd > 2 || number(PyObject_CallMethodNoArgs(a[5], s_get_device), &dev) || dev != device ||
+            number(PyObject_CallMethodNoArgs(a[5], s_numel), &numel) || numel != r.cols || number(PyObject_CallMethodNoArgs(a[5], s_data_ptr), &addr))
+            return not_taken();
+        w = (void*)(uintptr_t)addr;
+    }
+    if (a[10] != Py_None && (rows_of(a[10], 2, device, &o) || !FLOATS(o) || !LIKE(o))) return not_taken();
+    if (a[11] != Py_None) {
+        if (rows_of(a[11], 2, device, &q) || q.type != 3 || !LIKE(q) || rows_of(a[12], 1, device, &sc) || sc.type != 0 || sc.rows < rows || (rows > 1 && sc.ld != 1)) return not_taken();
+    } else if (a[12] != Py_None) {
+        return not_taken();
+    }
+#undef LIKE
+    if ((rotate != 0 && rotate != 32 && rotate != 256) || (rotate != 0 && (a[11] == Py_None || r.cols % rotate != 0)) || (a[10] == Py_None && a[11] == Py_None) ||
+        rows > INT32_MAX)
+        return not_taken();
+    if (rows == 0) return PyLong_FromLong(0); /* (tensors of no rows have no address) */
+    if (rows == 1) x.ld = r.ld = ro.ld = o.ld = q.ld = r.cols; /* (one row has no stride) */
+    const add_norm_t f = (add_norm_t)fn_add_rmsnorm;
+    int32_t st;
+    LAUNCH(f(c, s, x.p, x.type, x.ld, r.p, r.type, r.ld, ro.p, ro.ld, w, wd, (float)offset, (float)eps, (int32_t)rows, (int32_t)r.cols, o.p, o.type, o.ld, q.p, q.ld, sc.p,
+             (int32_t)rotate));
+    return PyLong_FromLong(st);
+}
 
 typedef int32_t (*qmm_i8_t)(iq_ctx*, void*, const int8_t*, int64_t, const float*, const int8_t*, const float*, int32_t, int32_t, void*, int32_t, int64_t,
                             int32_t, uint32_t);
-ENTRY(qmm_i8, 14, qmm_i8_t, {
-    void *c = P(0), *s = P(1), *x = P(2), *sx = P(4), *w = P(5), *sw = P(6), *y = P(9);
-    int32_t nn = I32(7), k = I32(8), yd = I32(10), rows = I32(12);
-    int64_t ldx = I64(3), ldy = I64(11);
-    uint32_t fl = U32(13);
-    CHECKED;
-    LAUNCH(f(c, s, x, ldx, sx, w, sw, nn, k, y, yd, ldy, rows, fl));
-})
+/* (context, stream, device, x, x_scales, address of w, address of w_scales, n, k, y, rows, flags) */
+static PyObject* py_qmm_i8(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    TENSORS(qmm_i8, 12);
+    (void)self;
+    void *c = P(0), *s = P(1), *w = P(5), *sw = P(6);
+    const int64_t device = I64(2), nn = I64(7), k = I64(8), rows = I64(10);
+    const uint32_t flags = U32(11);
+    Rows x, sx, y;
+    if (PyErr_Occurred()) return not_taken();
+    if (rows_of(a[3], 2, device, &x) || x.type != 3 || x.cols != k || rows < 0 || rows > INT32_MAX || x.rows < rows || rows_of(a[4], 1, device, &sx) || sx.type != 0 ||
+        sx.rows < rows || (rows > 1 && sx.ld != 1) || rows_of(a[9], 2, device, &y) || !FLOATS(y) || y.cols != nn || y.rows < rows)
+        return not_taken();
+    if (rows == 0) return PyLong_FromLong(0);
+    if (rows == 1) x.ld = k, y.ld = nn;
+    const qmm_i8_t f = (qmm_i8_t)fn_qmm_i8;
+    int32_t st;
+    LAUNCH(f(c, s, x.p, x.ld, sx.p, w, sw, (int32_t)nn, (int32_t)k, y.p, y.type, y.ld, (int32_t)rows, flags));
+    return PyLong_FromLong(st);
+}
 
 typedef int32_t (*rules_t)(iq_ctx*, void*, const void*, int32_t, int64_t, float*, int64_t, int32_t, int32_t, const iq_logit_rules*);
-ENTRY(logits_rules, 10, rules_t, {
-    void *c = P(0), *s = P(1), *x = P(2), *o = P(5), *r = P(9);
-    int32_t xd = I32(3), rows = I32(7), vocab = I32(8);
-    int64_t ldx = I64(4), ldo = I64(6);
-    CHECKED;
-    LAUNCH(f(c, s, x, xd, ldx, o, ldo, rows, vocab, r));
-})
+/* (context, stream, device, x, out, rows, vocab, address of the rules) */
+static PyObject* py_logits_rules(PyObject* self, PyObject* const* a, Py_ssize_t n) {
+    TENSORS(logits_rules, 8);
+    (void)self;
+    void *c = P(0), *s = P(1), *rules = P(7);
+    const int64_t device = I64(2), rows = I64(5), vocab = I64(6);
+    Rows x, o;
+    if (PyErr_Occurred()) return not_taken();
+    if (rows_of(a[3], 2, device, &x) || !FLOATS(x) || x.cols != vocab || rows < 0 || rows > INT32_MAX || x.rows < rows || rows_of(a[4], 2, device, &o) || o.type != 0 ||
+        o.cols != vocab || o.rows < rows)
+        return not_taken();
+    if (rows == 0) return PyLong_FromLong(0);
+    if (rows == 1) x.ld = o.ld = vocab;
+    const rules_t f = (rules_t)fn_logits_rules;
+    int32_t st;
+    LAUNCH(f(c, s, x.p, x.type, x.ld, o.p, o.ld, (int32_t)rows, (int32_t)vocab, rules));
+    return PyLong_FromLong(st);
+}
 
 #define M(NAME) {#NAME, (PyCFunction)(void (*)(void))py_##NAME, METH_FASTCALL, NULL}
 static PyMethodDef methods[] = {
-    {"bind", py_bind, METH_VARARGS, NULL}, M(qmv), M(qmm), M(dense_ffn), M(moe_forward), M(rmsnorm), M(had_rows), M(embed_rows),
+    {"bind", py_bind, METH_VARARGS, NULL}, {"bind_types", py_bind_types, METH_VARARGS, NULL}, M(qmv), M(qmm), M(dense_ffn), M(moe_forward), M(rmsnorm), M(had_rows), M(embed_rows),
     M(argmax_rows), M(topk64), M(add_rmsnorm), M(qmm_i8), M(logits_rules), {NULL, NULL, 0, NULL}};
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_iqcall", NULL, -1, methods, NULL, NULL, NULL, NULL};
-PyMODINIT_FUNC PyInit__iqcall(void) { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit__iqcall(void) {
+    static const struct { PyObject** slot; const char* name; } names[] = {{&s_shape, "shape"}, {&s_stride, "stride"}, {&s_dtype, "dtype"}, {&s_get_device, "get_device"},
+                                                                         {&s_data_ptr, "data_ptr"}, {&s_numel, "numel"}, {&s_is_contiguous, "is_contiguous"}};
+    for (size_t i = 0; i < sizeof(names) / sizeof(names[0]); i++)
+        if ((*names[i].slot = PyUnicode_InternFromString(names[i].name)) == NULL) return NULL;
+    return PyModule_Create(&module);
+}

@@ -323,26 +323,15 @@ class I8Linear:
     def encode(self, x: torch.Tensor, x_scales: torch.Tensor, y: torch.Tensor, rows: int, accumulate: bool = False,
                stream: Optional[torch.cuda.Stream] = None):
         """y[rows, N] (+)= (x codes · wᵀ codes) · x_scales · scales for int8 rows x [rows, K], any number of them."""
-        dev = self.w.get_device()
-        try:
-            (xr, xk), (ldx, xs), (yr, yn), (ldy, ys), (sr,), (ss,) = x.shape, x.stride(), y.shape, y.stride(), x_scales.shape, x_scales.stride()
-            yt = _DT.get(y.dtype, -1)
-            ok = (dev >= 0 and x.get_device() == dev and x_scales.get_device() == dev and y.get_device() == dev and 0 <= rows <= xr and rows <= yr and xk == self.K
-                  and yn == self.N and xs == 1 and (ys == 1 or yn == 1) and yt >= 0 and x.dtype == torch.int8 and x_scales.dtype == torch.float32 and sr >= rows
-                  and (rows <= 1 or ss == 1))
-        except (ValueError, AttributeError):  # another number of dimensions, no tensor
-            ok = False
-        if not ok:
+        dev, st = self.w.get_device(), None
+        if dev >= 0:  # (the conditions are looked at in csrc/pycall.c, and what fails one is described by _check)
+            ctx = capi.context(dev)
+            st = capi.call().qmm_i8(ctx.address, stream.cuda_stream if stream is not None else _raw_stream(dev), dev, x, x_scales, self.w.data_ptr(), self.scales.data_ptr(),
+                                    self.N, self.K, y, rows, capi.IQ_FLAG_ACCUMULATE if accumulate else 0)
+        if st is None:
             self._check(x, x_scales, y, rows)
             _need_cuda(x)
             raise ValueError("I8Linear does not take these tensors")
-        if rows == 0:  # (tensors of no rows have no address)
-            return
-        if rows <= 1:  # (one row has no stride)
-            ldx, ldy = xk, yn
-        ctx = capi.context(dev)
-        st = capi.call().qmm_i8(ctx.address, stream.cuda_stream if stream is not None else _raw_stream(dev), x.data_ptr(), ldx, x_scales.data_ptr(), self.w.data_ptr(),
-                                self.scales.data_ptr(), yn, xk, y.data_ptr(), yt, ldy, rows, capi.IQ_FLAG_ACCUMULATE if accumulate else 0)
         if st:
             ctx.check(st)
 

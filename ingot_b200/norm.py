@@ -64,50 +64,19 @@ def add_rmsnorm(x: Optional[torch.Tensor], residual: torch.Tensor, weight: Optio
     int8 rows into `codes` and `scales`, rotated in blocks of `rotate` inputs (what `I8Linear.rotate` says). Tensors are
     [rows, d] with any row stride; x None: the norm of residual alone; weight None: weights of one.
     residual_out may be residual, out may be x (same stride and element size); nothing else may overlap."""
-    # (each condition once, in few steps: a call of one row is bound by the host. What fails one is described by _check)
-    dev, ok = -1, (out is not None or codes is not None) and rotate in ROTATIONS and (x is not None or residual_out is None)
-    xp = xt = ldx = rop = ldro = wp = wt = op = ot = ldo = cp = ldc = sp = 0
     try:
-        (have, d), (ldr, step) = residual.shape, residual.stride()
-        rt, dev = _DT.get(residual.dtype, -1), residual.get_device()
-        ok = ok and 0 <= rows <= have and (step == 1 or d == 1) and 1 <= d <= MAX_WIDTH and rt >= 0 and eps >= 0
-        if x is not None:
-            (n, k), (ldx, step) = x.shape, x.stride()
-            xp, xt = x.data_ptr(), _DT.get(x.dtype, -1)
-            ok = ok and n >= rows and k == d and (step == 1 or d == 1) and xt >= 0 and x.get_device() == dev
-            if residual_out is None:
-                rop, ldro = residual.data_ptr(), ldr
-            else:
-                (n, k), (ldro, step) = residual_out.shape, residual_out.stride()
-                rop = residual_out.data_ptr()
-                ok = ok and n >= rows and k == d and (step == 1 or d == 1) and residual_out.get_device() == dev and residual_out.dtype == residual.dtype
-        if weight is not None:
-            wp, wt = weight.data_ptr(), _DT.get(weight.dtype, -1)
-            ok = ok and wt >= 0 and weight.get_device() == dev and weight.numel() == d and weight.is_contiguous()
-        if out is not None:
-            (n, k), (ldo, step) = out.shape, out.stride()
-            op, ot = out.data_ptr(), _DT.get(out.dtype, -1)
-            ok = ok and n >= rows and k == d and (step == 1 or d == 1) and ot >= 0 and out.get_device() == dev
-        if codes is not None:
-            (n, k), (ldc, step), (m,), (one,) = codes.shape, codes.stride(), scales.shape, scales.stride()
-            cp, sp = codes.data_ptr(), scales.data_ptr()
-            ok = (ok and n >= rows and k == d and (step == 1 or d == 1) and codes.dtype == torch.int8 and scales.dtype == torch.float32 and m >= rows and (one == 1 or rows <= 1)
-                  and codes.get_device() == dev and scales.get_device() == dev and (not rotate or d % rotate == 0))
-        elif rotate or scales is not None:
-            ok = False
-    except (ValueError, AttributeError):  # another number of dimensions, no tensor
-        ok = False
-    if not ok or dev < 0:
+        dev = residual.get_device()
+    except AttributeError:  # no tensor
+        dev = -1
+    st = None
+    if dev >= 0:  # (a call of one row is bound by the host: the conditions are looked at in csrc/pycall.c, and what fails one is described by _check)
+        ctx = capi.context(dev)
+        st = capi.call().add_rmsnorm(ctx.address, stream.cuda_stream if stream is not None else _raw_stream(dev), dev, x, residual, weight, rows, eps, weight_offset,
+                                     residual_out, out, codes, scales, rotate)
+    if st is None:
         _check(x, residual, weight, rows, eps, residual_out, out, codes, scales, rotate)
         if residual.device.type != "cuda":
             _no_cpu()
         raise ValueError("add_rmsnorm does not take these tensors")
-    if rows == 0:  # (tensors of no rows have no address)
-        return
-    ctx = capi.context(dev)
-    if rows <= 1:  # (one row has no stride)
-        ldx = ldr = ldro = ldo = ldc = d
-    st = capi.call().add_rmsnorm(ctx.address, stream.cuda_stream if stream is not None else _raw_stream(dev), xp, xt, ldx, residual.data_ptr(), rt, ldr,
-                                 rop, ldro, wp, wt, weight_offset, eps, rows, d, op, ot, ldo, cp, ldc, sp, rotate)
     if st:
         ctx.check(st)

@@ -127,24 +127,16 @@ class LogitRules:
         if out is None and dev >= 0:
             with torch.cuda.stream(stream):  # (None: the current one) the memory's stream is the kernel's
                 out = torch.empty(x.shape, dtype=torch.float32, device=x.device)
-        try:
-            (xr, xv), (ldx, xs), (outr, ov), (ldo, os) = x.shape, x.stride(), out.shape, out.stride()
-            xt = _DT.get(x.dtype, -1)
-            ok = (out.get_device() == dev and (self._index is None or self._index == dev) and 0 <= rows <= self.rows and rows <= xr and rows <= outr and xv == self.vocab and ov == xv
-                  and (xv == 1 or xs == os == 1) and xt >= 0 and out.dtype == torch.float32)
-        except (ValueError, AttributeError):  # another number of dimensions, no tensor
-            ok = False
-        if not ok or dev < 0:
+        st = None
+        if dev >= 0 and (self._index is None or self._index == dev) and rows <= self.rows:
+            # (the other conditions are looked at in csrc/pycall.c, and what fails one is described by _check)
+            ctx = capi.context(dev)
+            st = capi.call().logits_rules(ctx.address, stream.cuda_stream if stream is not None else _raw_stream(dev), dev, x, out, rows, self.vocab, self._at)
+        if st is None:
             self._check(x, rows, out)
             if not x.is_cuda:
                 _no_cpu()
             raise ValueError("LogitRules does not take these tensors")
-        if rows == 0:  # (tensors of no rows have no address)
-            return out
-        if rows <= 1:  # (one row has no stride)
-            ldx = ldo = xv
-        ctx = capi.context(dev)
-        st = capi.call().logits_rules(ctx.address, stream.cuda_stream if stream is not None else _raw_stream(dev), x.data_ptr(), xt, ldx, out.data_ptr(), ldo, rows, xv, self._at)
         if st:
             ctx.check(st)
         return out

@@ -235,3 +235,19 @@ def test_streams_at_once(cuda_device):
 def test_tensors_of_no_rows(cuda_device):
     m = I8Linear(torch.zeros(8, 64, dtype=torch.int8, device="cuda"), torch.zeros(8, device="cuda"))
     m.encode(torch.empty(0, 64, dtype=torch.int8, device="cuda"), torch.empty(0, device="cuda"), torch.empty(0, 8, device="cuda"), 0)
+
+
+def test_what_tensors_on_the_gpu_are_refused_for(cuda_device):
+    z = lambda *s, dtype=F32: torch.zeros(*s, dtype=dtype, device="cuda")
+    m = I8Linear(z(8, 64, dtype=torch.int8), z(8))
+    base = {"x": z(4, 64, dtype=torch.int8), "s": z(4), "y": z(4, 8), "rows": 4}
+    call = lambda a: m.encode(a["x"], a["s"], a["y"], a["rows"])
+    call(base)
+    for change in ({"rows": 5}, {"rows": -1}, {"x": z(4, 64)}, {"x": z(4, 48, dtype=torch.int8)}, {"x": z(64, dtype=torch.int8)}, {"x": z(64, 4, dtype=torch.int8).t()},
+                   {"x": z(4, 64, dtype=torch.int8).cpu()}, {"s": z(3)}, {"s": z(4, dtype=F16)}, {"s": z(8)[::2]}, {"s": z(4, 1)}, {"y": z(4, 7)}, {"y": z(4, 8).int()}, {"y": z(8, 4).t()},
+                   {"y": z(4, 8).cpu()}, {"y": None}):
+        with pytest.raises((ValueError, TypeError, AttributeError)):
+            call({**base, **change})
+    with pytest.raises(capi.IngotError):  # rows 24 bytes apart
+        call({**base, "x": z(4, 72, dtype=torch.int8)[:, :64]})
+    m.encode(z(1, 64, dtype=torch.int8), z(8)[::2], z(1, 8), 1)

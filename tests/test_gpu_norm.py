@@ -316,3 +316,32 @@ def test_rows_that_are_not_aligned(cuda_device, rows, d, pad, rotate, xt, rt, wt
     """Blocks of every size, one and two 16-bit types."""
     gen = torch.Generator().manual_seed(rows + d + pad)
     check(run(gen, rows, d, xt, rt, wt, ot, rotate, pad), 0.0, 1e-6, rotate)
+
+
+def test_what_tensors_on_the_gpu_are_refused_for(cuda_device):
+    """The conditions are looked at in C; what fails one is an error of Python's and reaches no kernel. No reference is lost or kept."""
+    import sys
+    z = lambda *s, dtype=F32: torch.zeros(*s, dtype=dtype, device="cuda")
+    base = lambda: {"x": z(4, 64), "residual": z(4, 64), "weight": z(64), "rows": 4, "out": z(4, 64), "codes": z(4, 64, dtype=torch.int8), "scales": z(4), "residual_out": z(4, 64)}
+    call = lambda a: add_rmsnorm(a.pop("x"), a.pop("residual"), a.pop("weight"), a.pop("rows"), **a)
+    call(base())
+    for change in ({"rows": 5}, {"rows": -1}, {"eps": -1.0}, {"eps": float("nan")}, {"rotate": 16}, {"rotate": 256}, {"scales": None}, {"codes": None}, {"x": z(4, 63)}, {"x": z(3, 64)},
+                   {"x": z(64)}, {"x": z(4, 64).double()}, {"x": z(4, 64).cpu()}, {"x": None}, {"residual": z(64)}, {"residual": z(4, 64).int()}, {"residual": z(64, 4).t()},
+                   {"residual_out": z(4, 64, dtype=F16)}, {"residual_out": z(64, 4).t()}, {"weight": z(63)}, {"weight": z(128)[::2]}, {"weight": z(64).long()}, {"weight": z(64).cpu()},
+                   {"out": z(4, 64).int()}, {"out": z(3, 64)}, {"codes": z(4, 64, dtype=torch.uint8)}, {"codes": z(4, 65, dtype=torch.int8)}, {"scales": z(3)}, {"scales": z(8)[::2]},
+                   {"scales": z(4, dtype=F16)}, {"scales": z(4, 1)}):
+        with pytest.raises((ValueError, TypeError)):
+            call({**base(), **change})
+    with pytest.raises(ValueError):
+        add_rmsnorm(None, z(2, 32776), None, 2, out=z(2, 32776))
+    before = [sys.getrefcount(t) for t in (F32, F16, BF16, torch.int8)]
+    x, a = z(4, 64), base()
+    kept = {k: sys.getrefcount(v) for k, v in a.items() if torch.is_tensor(v)}
+    for _ in range(500):
+        call(dict(a))
+        with pytest.raises(ValueError):
+            call({**a, "x": x[:, :63]})
+    assert all(abs(sys.getrefcount(t) - b) < 50 for t, b in zip((F32, F16, BF16, torch.int8), before))
+    assert all(sys.getrefcount(v) - kept[k] < 3 for k, v in a.items() if k in kept)
+    # one row has no stride, and a scale of its own lies anywhere
+    add_rmsnorm(None, z(1, 64), None, 1, codes=z(1, 64, dtype=torch.int8), scales=z(8)[::2])

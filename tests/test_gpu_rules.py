@@ -283,3 +283,14 @@ def test_blocks_with_a_multiprocessor_to_themselves(cuda_device, rows, V):
     """Up to the largest part, and the first that is too large."""
     rng = np.random.default_rng(rows + V)
     check(rng, rows, V, some(rng, rows, V, history=700, bias=9, masks=2))
+
+
+def test_what_tensors_on_the_gpu_are_refused_for(cuda_device):
+    z = lambda *s, dtype=F32: torch.zeros(*s, dtype=dtype, device="cuda")
+    rules = LogitRules(4, 100, repetition=z(4) + 1)
+    rules.encode(z(4, 100), 4, out=z(4, 100))
+    for change in ({"x": z(4, 99)}, {"x": z(3, 100)}, {"x": z(100)}, {"x": z(4, 100).int()}, {"x": z(100, 4).t()}, {"x": z(4, 100).cpu()}, {"rows": 5}, {"rows": -1}, {"out": z(4, 99)},
+                   {"out": z(4, 100, dtype=BF16)}, {"out": z(4, 100).cpu()}, {"out": z(100, 4).t()}):
+        a = {"x": z(4, 100), "rows": 4, "out": z(4, 100), **change}
+        with pytest.raises((ValueError, TypeError)):
+            rules.encode(a["x"], a["rows"], out=a["out"])
