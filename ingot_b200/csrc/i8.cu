@@ -336,6 +336,7 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap
 // Bound: operands on their way from L2 (a step of 128 inputs moves 16 KB + 64 bytes per token and SM, at some 46 bytes per cycle: 0.36 us on 256 tokens,
 // the MMAs alone 0.27) and power. 2048 x 4096 x 14336 79 to 98 us, 2048 x 14336 x 4096 82, 4096 x 14336 x 4096 156 (3080 TOP/s). Measured and taken
 // back: 512 tokens per pair as two MMAs on the same features (the step 11 % shorter per token, but no room for a second accumulator: 84 us against 79).
+// Stages of 96 KB, so that the next call's CTAs start beside this one's: they gather on the same SMs (256 x 4096 x 14336 20.1 -> 25.8 us).
 __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2, 1, 1)
     i8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w, const I8Params p) {
     extern __shared__ unsigned char smem_raw[];
