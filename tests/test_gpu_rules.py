@@ -294,3 +294,22 @@ def test_what_tensors_on_the_gpu_are_refused_for(cuda_device):
         a = {"x": z(4, 100), "rows": 4, "out": z(4, 100), **change}
         with pytest.raises((ValueError, TypeError)):
             rules.encode(a["x"], a["rows"], out=a["out"])
+
+
+@pytest.mark.parametrize("rows,V,history,masks", [(20, 100003, 900, 3), (64, 100001, 0, 5), (18, 100000, 0, 0)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_large_parts_that_begin_anywhere(cuda_device, rows, V, history, masks, dtype):
+    """Groups of eight logits: x and out at the same place within them, at the same within four, and elsewhere."""
+    rng = np.random.default_rng(V + history)
+    a = some(rng, rows, V, history=history, masks=masks, bias=7)
+    rules = LogitRules(rows, V, **device(a))
+    x = torch.from_numpy(3 * rng.normal(size=(rows, V)).astype(np.float32)).to(dtype)
+    want = qref.logit_rules(x.float().numpy(), np.float32, **a)
+    for at_x, at_out in ((0, 0), (5, 5), (4, 0), (3, 7), (1, 2)):
+        xd = torch.zeros(rows * V + 8, dtype=dtype, device="cuda")[at_x:at_x + rows * V].view(rows, V)
+        xd.copy_(x)
+        flat = torch.full((rows * V + 16,), 7.0, device="cuda")
+        rules.encode(xd, rows, out=flat[at_out:at_out + rows * V].view(rows, V))
+        got = flat.cpu().numpy()
+        assert np.array_equal(got[at_out:at_out + rows * V].reshape(rows, V), want, equal_nan=True)
+        assert (got[:at_out] == 7).all() and (got[at_out + rows * V:] == 7).all()
