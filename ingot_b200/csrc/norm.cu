@@ -668,16 +668,16 @@ NormKernel norm_pick(int half, bool codes, int rotate) {
 }
 // Rows that are not aligned: blocks of up to 512 threads, whose registers are held to what lets 1536 of them (with two groups each 1024) share an SM: more rows under
 // way at once. 2048 rows of 4095, bf16, 27.0 -> 22.4 us, with the one 16-bit type known 20.8; 1024 of 7681 29.9 -> 26.1 -> 22.3; 30,000 of 480 with rotated codes
-// 113 -> 55 -> 51. Taken back: groups of eight out of aligned pieces of 16 bytes, shifted in registers (2048 rows of 4095 33.0).
+// 113 -> 55 -> 51. Up to a row per SM (few) a thread per group: 113 of 7680 5.5 -> 3.9. Taken back: groups of eight out of aligned pieces of 16 bytes, shifted in registers (2048 rows of 4095 33.0).
 template <int HT>
-NormKernel norm_pick_unaligned(int groups, bool codes, int rotate) {
+NormKernel norm_pick_unaligned(int groups, bool few, bool codes, int rotate) {
     return groups <= 256 ? norm_pick<1, 256, false, HT>(codes, rotate) : groups <= 512 ? norm_pick<1, 512, false, HT>(codes, rotate)
-         : groups <= 1024 ? norm_pick<2, 512, false, HT>(codes, rotate) : groups <= 2048 ? norm_pick<2, 1024, false, HT>(codes, rotate)
+         : groups <= 1024 && few ? norm_pick<1, 1024, false, HT>(codes, rotate) : groups <= 1024 ? norm_pick<2, 512, false, HT>(codes, rotate) : groups <= 2048 ? norm_pick<2, 1024, false, HT>(codes, rotate)
                                                                                         : norm_pick<4, 1024, false, HT>(codes, rotate);
 }
-NormKernel norm_pick_unaligned(int half, int groups, bool codes, int rotate) {
-    return half == kF16 ? norm_pick_unaligned<kF16>(groups, codes, rotate) : half == kBF16 ? norm_pick_unaligned<kBF16>(groups, codes, rotate)
-                                                                                           : norm_pick_unaligned<kF32>(groups, codes, rotate);
+NormKernel norm_pick_unaligned(int half, int groups, bool few, bool codes, int rotate) {
+    return half == kF16 ? norm_pick_unaligned<kF16>(groups, few, codes, rotate) : half == kBF16 ? norm_pick_unaligned<kBF16>(groups, few, codes, rotate)
+                                                                                                : norm_pick_unaligned<kF32>(groups, few, codes, rotate);
 }
 
 bool misplaced(const void* p, int esz) { return reinterpret_cast<uintptr_t>(p) % esz != 0; }
@@ -734,7 +734,8 @@ extern "C" int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int3
     p.rows = rows; p.d = d; p.offset = weight_offset; p.eps = eps;
     const bool vec = d % 8 == 0 && aligned(x, ldx, dtype_size(x_dtype)) && aligned(residual, ldr, dtype_size(r_dtype)) && aligned(residual_out, ldro, dtype_size(r_dtype)) &&
                      aligned(weight, 0, dtype_size(w_dtype)) && aligned(out, ldo, dtype_size(out_dtype)) && aligned(codes, ldc, 1);
-    const int groups = (d + 7) / 8, nch = groups <= (vec ? 1024 : 512) ? 1 : groups <= 2048 ? 2 : 4;
+    const bool few = rows <= ctx->sms;  // a block per SM: with as many threads as there are groups
+    const int groups = (d + 7) / 8, nch = groups <= (vec || few ? 1024 : 512) ? 1 : groups <= 2048 ? 2 : 4;
     int threads = round_up((groups + nch - 1) / nch, 32), blocks = rows;
     size_t smem = 0;
     // the one 16-bit type of the call (bf16 where it has none), kF32 where it has both
@@ -745,7 +746,7 @@ extern "C" int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int3
     meet(x, x_dtype); meet(residual, r_dtype); meet(weight, w_dtype); meet(out, out_dtype);
     if (half == -1) half = kBF16;
     const bool c8 = codes != nullptr;
-    NormKernel kernel = !vec ? norm_pick_unaligned(half, groups, c8, rotate) : nch == 1 ? norm_pick<1>(half, c8, rotate) : nch == 2 ? norm_pick<2>(half, c8, rotate)
+    NormKernel kernel = !vec ? norm_pick_unaligned(half, groups, few, c8, rotate) : nch == 1 ? norm_pick<1>(half, c8, rotate) : nch == 2 ? norm_pick<2>(half, c8, rotate)
                                                                                                                           : norm_pick<4>(half, c8, rotate);
     // Many rows: a third more than the other kernel runs at once (64 registers a thread). 512 rows of 4096, codes of a bf16 sum, 6.8 us there and 5.2 here, 257 rows
     // 3.9 and 4.8; 200 of 7680 6.9 and 5.1, 148 3.9 and 3.6; 600 of 2048 4.4 and 4.9, 1000 5.7 and 5.2. Blocks: those that run at once, by registers and by the

@@ -310,7 +310,7 @@ def test_tensors_of_no_rows(cuda_device):
     add_rmsnorm(none, none, None, 0, out=none, codes=torch.empty(0, 64, dtype=torch.int8, device="cuda"), scales=torch.empty(0, device="cuda"))
 
 
-@pytest.mark.parametrize("rows,d,pad,rotate", [(3, 1024, 7, 256), (5, 1999, 0, 0), (2, 4103, 2, 0), (3, 6144, 7, 256), (2, 14337, 0, 0), (2, 14336, 7, 32), (1500, 480, 7, 32), (1700, 2047, 0, 0)])
+@pytest.mark.parametrize("rows,d,pad,rotate", [(3, 1024, 7, 256), (5, 1999, 0, 0), (2, 4103, 2, 0), (3, 6144, 7, 256), (160, 4103, 0, 0), (160, 6144, 7, 32), (2, 14337, 0, 0), (2, 14336, 7, 32), (1500, 480, 7, 32), (1700, 2047, 0, 0)])
 @pytest.mark.parametrize("xt,rt,wt,ot", [(BF16, BF16, BF16, BF16), (F16, F32, F16, F16), (F32, F16, BF16, F32)])
 def test_rows_that_are_not_aligned(cuda_device, rows, d, pad, rotate, xt, rt, wt, ot):
     """Blocks of every size, one and two 16-bit types."""
