@@ -135,7 +135,7 @@ def test_streams_and_graphs(cuda_device, rows, k):
     assert (y == 5).all()
 
 
-@pytest.mark.parametrize("N,K,group,rotate", [(64, 1024, 64, 256), (100, 1024, 64, 32), (3, 64, 64, 0), (48, 2880, 64, 32), (130, 768, 32, 256), (16, 128, 32, 0)])
+@pytest.mark.parametrize("N,K,group,rotate", [(64, 1024, 64, 256), (100, 1024, 64, 32), (3, 64, 64, 0), (48, 2880, 64, 32), (130, 768, 32, 256), (16, 128, 32, 0), (3, 49152, 64, 256), (5, 16384, 32, 32)])
 def test_packing(cuda_device, N, K, group, rotate):
     rng = np.random.default_rng(N + K)
     m, host = affine_case(rng, N, K, 4, cuda_device, group=group)
