@@ -134,11 +134,14 @@ __device__ __forceinline__ void i8_store4(const I8Params& p, const int4& s, floa
 
 // A thread's share of the results of 128 features from n0 on, in units of a token and four features (u0 + thread, and so on up to u1): the sums of PARTS CTAs of the
 // cluster, which parked them at `park`, [token][128 features]. Eight loads of 16 bytes are under way at once. sx, sw: the scales of the first unit.
+// Every load is waited for by a store of this thread ahead of the cluster's last meeting, which orders no memory: whoever owns it may leave after that.
+// So a thread whose features lie beyond n loads nothing (of the last tile's odd CTAs, where n % 256 is 1 to 128, no thread does).
 template <int PARTS, int THREADS, int STEP>
 __device__ __forceinline__ void i8_shares(const I8Params& p, uint32_t park, uint32_t first, int u0, int u1, int row0, int n0, float sx0, const float (&sw)[4]) {
     static_assert(THREADS % 32 == 0, "a thread's units are of the same features");
     constexpr int B = 8 / PARTS;
     const int n = n0 + u0 % 32 * 4;
+    if (n >= p.N) return;
     for (int u = u0; u < u1; u += B * THREADS) {
         int4 o[B][PARTS];
         float sx[B];
@@ -301,7 +304,7 @@ __global__ void __launch_bounds__(kI8Threads, I8Tile<BN>::PER_SM)
             else if (parts == 4) i8_shares<4, kI8Threads, 1>(p, park, 0, u, u1, row0, n0, unit_sx, unit_sw);
             else i8_shares<8, kI8Threads, 1>(p, park, 0, u, u1, row0, n0, unit_sx, unit_sw);
         }
-        // nobody reads this CTA's shared memory any more (what was read has gone into the sums: no ordering of memory to wait for)
+        // nobody reads this CTA's shared memory any more (every load has gone into a sum that was stored: no ordering of memory to wait for)
         __syncwarp();
         asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
     }
@@ -613,7 +616,7 @@ __global__ void __launch_bounds__(kI8PairThreads, 1) __cluster_dims__(2 * SPLIT,
     cluster_sync_all();  // every CTA's sums lie in its shared memory
     if (!*abort_flag) i8_shares<SPLIT, kI8PairThreads, 2>(p, smem_u32(smem), half, u0 + (int)threadIdx.x, u1, row0, n0, unit_sx, unit_sw);
     __syncwarp();
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");  // (nobody reads this CTA's shared memory any more)
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");  // (nobody reads this CTA's shared memory any more: i8_shares)
     if (*abort_flag && threadIdx.x == 0 && p.status != nullptr) atomicExch(p.status, kErrTimeout);
     if (warp == 1) {
         tc_fence_after();

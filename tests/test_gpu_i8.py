@@ -251,3 +251,26 @@ def test_what_tensors_on_the_gpu_are_refused_for(cuda_device):
     with pytest.raises(capi.IngotError):  # rows 24 bytes apart
         call({**base, "x": z(4, 72, dtype=torch.int8)[:, :64]})
     m.encode(z(1, 64, dtype=torch.int8), z(8)[::2], z(1, 8), 1)
+
+
+@pytest.mark.parametrize("rows,n,k,pair,parts", [(200, 600, 1040, 1, 2), (200, 1, 1040, 1, 2), (173, 257, 1040, 1, 2), (300, 2049, 2064, 1, 2), (200, 640, 1040, 1, 2), (200, 641, 1040, 1, 2),
+                                                 (129, 257, 2064, 1, 3), (470, 640, 2064, 1, 3), (1500, 384, 8208, 1, 3), (1500, 385, 8208, 1, 3), (40, 129, 2064, 0, 8), (17, 4, 4096, 0, 8),
+                                                 (3, 129, 1040, 0, 4), (40, 4097, 2064, 0, 4), (64, 9217, 1552, 0, 2)])
+def test_divided_tiles_of_few_features(cuda_device, rows, n, k, pair, parts):
+    """The last tile's features are few: of a pair the odd CTA may have none of them, and then takes nothing from its counterparts. Beside other calls, whose CTAs follow at once."""
+    plan = capi.qmm_i8_plan(rows, n, k)
+    assert (plan.pair, plan.parts) == (pair, parts)
+    run(torch.Generator().manual_seed(rows + n), rows, n, k, F16, True, 1)
+    gen = torch.Generator().manual_seed(n)
+    x, w, sx, sw = codes(gen, rows, k), codes(gen, n, k), torch.rand(rows, generator=gen), torch.rand(n, generator=gen)
+    want = reference(x, sx, w, sw)
+    m, xd, sd = I8Linear(w.cuda(), sw.cuda()), x.cuda(), sx.cuda()
+    torch.cuda.synchronize()
+    streams, ys = [torch.cuda.Stream() for _ in range(3)], torch.zeros(3, rows, n, device="cuda")
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, y in zip(streams, ys):
+            m.encode(xd, sd, y, rows, stream=s)
+    torch.cuda.synchronize()
+    assert capi.context(0).device_status() == 0
+    assert all(torch.equal(y.cpu(), want) for y in ys)
