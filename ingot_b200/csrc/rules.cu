@@ -189,11 +189,13 @@ __global__ void __launch_bounds__(T, T == 512 ? kRulePerSm : 1) logit_rules_kern
     const int len = HIST ? min(max(p.r.lens[row], 0), p.r.max_tokens) : 0, said = HIST && p.r.prompt_lens != nullptr ? p.r.prompt_lens[row] : 0;
     const int m = p.r.mask == nullptr ? -1 : p.r.mask_rows != nullptr ? p.r.mask_rows[row] : row;
     const bool biases = p.r.bias_offsets != nullptr;
-    const int b0 = biases ? max(p.r.bias_offsets[row], 0) : 0, b1 = biases ? min(p.r.bias_offsets[row + 1], p.r.biases) : 0;
+    // (cut to the list on both sides before anything is added to them)
+    const int b0 = biases ? min(max(p.r.bias_offsets[row], 0), p.r.biases) : 0, b1 = biases ? max(min(p.r.bias_offsets[row + 1], p.r.biases), b0) : 0;
     __syncthreads();  // the counters are zero
-    // an entry of the row's biases into the list; where it went, or -1
-    auto collect = [&](int j) {
-        if (j >= b1) return -1;
+    // the thread's entry of the row's biases from j0 on into the list; where it went, or -1
+    auto collect = [&](int j0) {
+        if (tid >= b1 - j0) return -1;
+        const int j = j0 + tid;
         const uint32_t token = (uint32_t)p.r.bias_tokens[j], t = token - (uint32_t)lo;
         if (token >= (uint32_t)p.vocab || t >= (uint32_t)n) return -1;
         if (atomicOr(&list.named[t >> 5], 1u << (t & 31)) >> (t & 31) & 1) list.twice = 1;
@@ -204,7 +206,7 @@ __global__ void __launch_bounds__(T, T == 512 ? kRulePerSm : 1) logit_rules_kern
     };
     // A token's biases are in the hands of the thread that has the first of them. Its logit is read before anything is written
     // (x may be out) and its result stored behind all the others.
-    const int mine = b0 < b1 ? collect(b0 + tid) : -1;
+    const int mine = b0 < b1 ? collect(b0) : -1;
     const uint32_t my_token = mine >= 0 ? list.key[mine] & 0xFFFFu : 0;
     const float my_logit = mine >= 0 ? load1(my_token) : 0.f;
     const uint32_t* const mask = m >= 0 && m < p.r.masks ? p.r.mask + (size_t)m * p.r.ld_mask : nullptr;
@@ -361,12 +363,12 @@ __global__ void __launch_bounds__(T, T == 512 ? kRulePerSm : 1) logit_rules_kern
         if (store) out[my_token] = my_result;
     }
     // more biases than the list takes at once: by rounds
-    for (int j0 = b0 + T; j0 < b1; j0 += T) {
+    for (int left = b1 - b0 - T; left > 0; left -= T) {
         __syncthreads();
         for (int i = tid; i < p.span / 32; i += T) list.named[i] = 0;
         if (tid == 0) list.n = list.twice = 0;
         __syncthreads();
-        const int at = collect(j0 + tid);
+        const int at = collect(b1 - left);
         __syncthreads();
         if (at >= 0) {
             const uint32_t t = list.key[at] & 0xFFFFu;

@@ -313,3 +313,16 @@ def test_large_parts_that_begin_anywhere(cuda_device, rows, V, history, masks, d
         got = flat.cpu().numpy()
         assert np.array_equal(got[at_out:at_out + rows * V].reshape(rows, V), want, equal_nan=True)
         assert (got[:at_out] == 7).all() and (got[at_out + rows * V:] == 7).all()
+
+
+@pytest.mark.parametrize("history", [0, 300])
+@pytest.mark.parametrize("offsets", [[0, 2000, 2**31 - 1, 2**31 - 400, -2**31, 700, 2**31 - 1], [2**31 - 1] * 7, [2**31 - 512, 2**31 - 1024, 2600, 2601, 0, -1, 2600],
+                                     [-2**31, -2**31, 2**31 - 1, -2**31, 2**31 - 1, 2600, 2599]])
+def test_offsets_of_biases_anywhere(cuda_device, history, offsets):
+    """Offsets far beyond the list, at either end of their type too, are cut there: the steps of a list's rounds do not pass 32 bits."""
+    rng = np.random.default_rng(len(offsets) + history)
+    for V in (900, 40001):
+        a = some(rng, 6, V, history=history, masks=2)
+        a["bias_tokens"], a["bias_values"] = rng.integers(0, V, 2600).astype(np.int32), rng.normal(size=2600).astype(np.float32)
+        a["bias_offsets"] = np.array(offsets, dtype=np.int64).astype(np.int32)
+        check(rng, 6, V, a)
