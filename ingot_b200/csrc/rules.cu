@@ -28,6 +28,7 @@ namespace iq {
 namespace {
 
 constexpr int kRuleMaxVocab = 262144;
+constexpr int kRuleMaxTokens = 1 << 30;  // of a row's history: the steps through it stay within 32 bits
 constexpr int kRulePerSm = 3;     // blocks of an SM, of 512 threads each; one of 1024 where that is all
 constexpr int kRuleSpan = 24576;  // most logits of a block,
 constexpr int kRuleWhole = 32768;  // of one with an SM to itself,
@@ -425,6 +426,7 @@ extern "C" int32_t iq_logits_rules(iq_ctx* ctx, void* stream, const void* x, int
     if (vocab > kRuleMaxVocab || rows > (1 << 24)) return fail(ctx, kErrUnsupported, "logits_rules: up to %d logits per row", kRuleMaxVocab);
     if (r.tokens != nullptr && (r.lens == nullptr || r.max_tokens < 0 || r.ld_tokens < r.max_tokens))
         return fail(ctx, kErrInvalidArg, "logits_rules: a history has lengths, its rows at least max_tokens apart");
+    if (r.tokens != nullptr && r.max_tokens > kRuleMaxTokens) return fail(ctx, kErrUnsupported, "logits_rules: a history of up to %d tokens", kRuleMaxTokens);
     if (r.bias_offsets != nullptr && (r.biases < 0 || (r.biases > 0 && (r.bias_tokens == nullptr || r.bias_values == nullptr))))
         return fail(ctx, kErrInvalidArg, "logits_rules: biases are offsets, tokens and values");
     if (r.mask != nullptr && (r.masks < 1 || r.ld_mask < (vocab + 31) / 32 || (r.mask_rows == nullptr && r.masks < rows)))

@@ -61,7 +61,7 @@ class LogitRules:
     repetition (above 0; 1: none), presence, frequency (0: none) float32 [rows]. bias_offsets int32 [rows + 1], bias_tokens int32 [n], bias_values float32 [n].
     mask int32 or uint32 [masks, at least vocab / 32]: bit t % 32 of word t / 32 allows token t; mask_rows int32 [rows]: a row's mask, -1 for none (None: its own)."""
 
-    MAX_VOCAB = 262144
+    MAX_VOCAB, MAX_HISTORY, MAX_LIST = 262144, 1 << 30, 2**31 - 1
 
     def __init__(self, rows: int, vocab: int, *, tokens=None, lens=None, prompt_lens=None, repetition=None, presence=None, frequency=None, bias_offsets=None,
                  bias_tokens=None, bias_values=None, mask=None, mask_rows=None):
@@ -90,6 +90,11 @@ class LogitRules:
         if mask is not None and (mask.dtype not in (torch.int32, torch.uint32) or mask.dim() != 2 or mask.shape[1] < (vocab + 31) // 32
                                  or (mask.shape[1] > 1 and mask.stride(1) != 1) or mask.shape[0] < (rows if mask_rows is None else 1)):
             raise ValueError(f"mask is int32 [masks, at least {(vocab + 31) // 32}], one per row unless mask_rows tells")
+        if tokens is not None and tokens.shape[1] > self.MAX_HISTORY:
+            raise ValueError(f"tokens has a capacity of {tokens.shape[1]} (up to {self.MAX_HISTORY})")
+        for name, t in (("bias_tokens", bias_tokens), ("mask", mask)):
+            if t is not None and t.shape[0] > self.MAX_LIST:
+                raise ValueError(f"{name} has {t.shape[0]} entries (up to {self.MAX_LIST})")
         self.rows, self.vocab = rows, vocab
         self._kept = tuple(t for t in (tokens, lens, prompt_lens, repetition, presence, frequency, bias_offsets, bias_tokens, bias_values, mask, mask_rows) if t is not None)
         for t in self._kept:

@@ -73,3 +73,22 @@ def test_tensors_begin_on_an_element(call, rules):
     a.update({"x": P, "out": P})
     rules = {name: P for name in rules}
     assert given() == -2
+
+
+def meta(*s, dtype=torch.int32):
+    return torch.empty(*s, dtype=dtype, device="meta")
+
+
+@pytest.mark.parametrize("a,what", [({"tokens": meta(4, 2**30 + 1), "lens": meta(4)}, "capacity"), ({"tokens": meta(4, 2**32 + 5), "lens": meta(4)}, "capacity"),
+                                    ({"bias_offsets": meta(5), "bias_tokens": meta(2**31), "bias_values": meta(2**31, dtype=torch.float32)}, "bias_tokens has"),
+                                    ({"mask": meta(2**32 + 1, 4), "mask_rows": meta(4)}, "mask has")])
+def test_lists_beyond_32_bits(a, what):
+    """Lengths go to the C entry as 32 bits, and the kernel's steps through a history stay within them."""
+    with pytest.raises(ValueError, match=what):
+        LogitRules(4, 100, **a)
+
+
+@pytest.mark.parametrize("tokens,status", [(2**30, -1), (2**30 + 1, -2), (2**31 - 1, -2)])
+def test_histories_beyond_the_largest(tokens, status):
+    rules = capi.LogitRules(tokens=P, lens=P, ld_tokens=2**31, max_tokens=tokens)  # (without a context the largest is refused as well, for that)
+    assert capi.lib().iq_logits_rules(None, None, P, 0, 100, P, 100, 4, 100, C.byref(rules)) == status
