@@ -278,7 +278,7 @@ class I8Linear:
     that its inputs have gone through as well (0: none), for add_rmsnorm(rotate=). `w` may be read while the
     launch before on the stream still runs: it is complete before that launch begins (after `pack` it is)."""
 
-    MAX_K = 131056
+    MAX_K, MAX_N = 131056, 1 << 30
 
     def __init__(self, w: torch.Tensor, scales: torch.Tensor, rotate: int = 0):
         if w.dim() != 2 or w.dtype != torch.int8 or scales.dtype != torch.float32:
@@ -287,6 +287,8 @@ class I8Linear:
             raise ValueError(f"weights {tuple(w.shape)} and one scale per row, both contiguous")
         if w.shape[0] < 1 or w.shape[1] < 16 or w.shape[1] % 16 or w.shape[1] > self.MAX_K:
             raise ValueError(f"K is a multiple of 16 up to {self.MAX_K}, not {w.shape[1]}")
+        if w.shape[0] > self.MAX_N:
+            raise ValueError(f"{w.shape[0]} features (up to {self.MAX_N})")
         if rotate not in (0, 32, 256) or (rotate and w.shape[1] % rotate):
             raise ValueError(f"the rotation has blocks of 32 or 256 inputs that divide K = {w.shape[1]}, not {rotate}")
         if w.device != scales.device:

@@ -101,3 +101,10 @@ def test_more_than_a_grid_holds(rows, n, k):
             capi.qmm_i8_plan(rows, n, k)
     else:
         assert capi.qmm_i8_plan(rows, n, k).tiles > 1 << 30  # (refused with a context)
+
+
+@pytest.mark.parametrize("n", [2**30 + 1, 2**32 + 1])
+def test_more_features_than_a_call_takes(n):
+    """(they would go to the C entry as 32 bits)"""
+    with pytest.raises(ValueError, match="features"):
+        I8Linear(torch.empty(n, 16, dtype=torch.int8, device="meta"), torch.empty(n, device="meta"))
