@@ -548,8 +548,9 @@ int32_t iq_rmsnorm(iq_ctx* ctx, void* stream, const float* x, int64_t ldx, void*
  *   codes, scales: u = H(r' * (weight + weight_offset)) in fp32, s = max|u| / 127 over the row, codes = rint(u / s), scale = s * q
  * so that scale * code stands for H(out). H is the blockwise unnormalised Hadamard transform of the W8A8 weights: rotate = 0 (none), 32 or 256
  * inputs per block (d a multiple of it; iq_i8_pack tells which), spans 1, 2, 4, ...: a + b and a - b. The codes depend on stored values
- * and single fp32 operations only: they are the same bits for every call that holds the row. A row of zeros has scale 0; a row whose
- * u holds an infinity or NaN has codes 0 and scale NaN. The sum of squares is fp32: rows beyond 1e19 overflow it.
+ * and single fp32 operations only: they are the same bits for every call that holds the row. A row whose s is 0 (of zeros, or with
+ * max|u| below 2^-143) has codes and scale 0; a row whose u holds an infinity or NaN has codes 0 and scale NaN. The sum of squares is fp32: rows beyond
+ * 1e19 overflow it, and with eps = 0 rows below 1e-19 underflow it.
  * x null (with residual_out null): no addition, r' = residual. weight null: weights of 1, the offset unused. out null or codes (with scales) null: not
  * wanted. weight_offset: 1 where the checkpoint stores w - 1 (Gemma), else 0. residual_out may be residual and out may be x,
  * where row stride and element size are the same; other overlaps are not allowed. Tensors begin on an element, strides are at least d; where groups of

@@ -429,8 +429,8 @@ __global__ void __launch_bounds__(MAXT, MAXT < 1024 ? (NCH == 1 ? 1536 : 1024) /
         }
         const bool finite = most < INFINITY;  // (not with a NaN either)
         const float s = __fdiv_rn(most, 127.f), inv = __fdiv_rn(1.f, s);
-        if (tid == 0) p.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : most == 0.f ? 0.f : __fmul_rn(s, q);
-        const bool none = !finite || most == 0.f;
+        if (tid == 0) p.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : s == 0.f ? 0.f : __fmul_rn(s, q);
+        const bool none = !finite || s == 0.f;  // (s: a largest magnitude below 2^-143 has none either)
 #pragma unroll
         for (int c = 0; c < NCH; c++) {
             const uint2 k = none ? make_uint2(0, 0) : codes8(u[c], s, inv);
@@ -625,8 +625,8 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const __grid_con
             most = __uint_as_float(__reduce_max_sync(0xffffffffu, lane < warps ? __float_as_uint(wmax[turn][lane]) : 0u));
             const bool finite = most < INFINITY;  // (not with a NaN either)
             const float step = __fdiv_rn(most, 127.f), inv = __fdiv_rn(1.f, step);
-            const bool none = !finite || most == 0.f;
-            if (tid == 0) p.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : most == 0.f ? 0.f : __fmul_rn(step, q);
+            const bool none = !finite || step == 0.f;
+            if (tid == 0) p.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : step == 0.f ? 0.f : __fmul_rn(step, q);
 #pragma unroll
             for (int k = 0; k < K; k++)
                 if (live[k]) *reinterpret_cast<uint2*>(codes + k * APART) = none ? make_uint2(0, 0) : codes8(v[k], step, inv);

@@ -345,3 +345,24 @@ def test_what_tensors_on_the_gpu_are_refused_for(cuda_device):
     assert all(sys.getrefcount(v) - kept[k] < 3 for k, v in a.items() if k in kept)
     # one row has no stride, and a scale of its own lies anywhere
     add_rmsnorm(None, z(1, 64), None, 1, codes=z(1, 64, dtype=torch.int8), scales=z(8)[::2])
+
+
+@pytest.mark.parametrize("rows,d,pad", [(5, 512, 0), (5, 512, 3), (1000, 512, 0), (1000, 512, 3), (300, 4096, 0), (3, 18432, 0)])
+@pytest.mark.parametrize("rotate", [0, 256])
+@pytest.mark.parametrize("eps", [1e-6, 0.0])
+def test_rows_whose_step_rounds_to_nothing(cuda_device, rows, d, pad, rotate, eps):
+    """A largest value of up to 63 * 2^-149 has a step max / 127 of 0 in 32 bits: codes and scale are 0, not 127 and 0 * inf. One of 64 * 2^-149 has a step of 2^-149."""
+    r = torch.zeros(rows, d)
+    r[0, 5] = 1e-44  # 7 * 2^-149
+    r[1 % rows, d - 1] = -63 * 2.0**-149
+    r[2 % rows, 7] = 64 * 2.0**-149
+    r[rows - 1, 0] = 2.0**-149
+    wide = torch.zeros(rows, d + pad)
+    wide[:, :d] = r
+    codes = torch.full((rows, d), 99, dtype=torch.int8, device="cuda")
+    scales = torch.full((rows,), 7.0, device="cuda")
+    add_rmsnorm(None, wide.cuda()[:, :d], None, rows, eps=eps, codes=codes, scales=scales, rotate=rotate)
+    want, s = qref.norm_codes(r.numpy(), np.ones(d, np.float32), max(rotate, 1))
+    assert np.array_equal(codes.cpu().numpy(), want)
+    got = scales.cpu().numpy()
+    assert (got[s == 0] == 0).all() and (s[[0, 1]] == 0).all() and s[2] > 0 and (want[2] != 0).any()
