@@ -326,3 +326,33 @@ def test_offsets_of_biases_anywhere(cuda_device, history, offsets):
         a["bias_tokens"], a["bias_values"] = rng.integers(0, V, 2600).astype(np.int32), rng.normal(size=2600).astype(np.float32)
         a["bias_offsets"] = np.array(offsets, dtype=np.int64).astype(np.int32)
         check(rng, 6, V, a)
+
+
+@pytest.mark.parametrize("rows,V,history", [(160, 2001, 9000), (160, 2000, 9001), (40, 151665, 16384), (150, 40003, 33000), (149, 40000, 40001), (40, 262143, 33000)])
+def test_long_histories_of_many_rows(cuda_device, rows, V, history):
+    """Blocks of 512 threads that go through histories by 4096 tokens: two counters in a word and one, rows' parts beyond the first, prompts that end inside a step."""
+    rng = np.random.default_rng(rows + V + history)
+    a = some(rng, rows, V, history=history, bias=6, masks=2, spread=2.0)
+    a["lens"][:] = rng.integers(history // 2, history + 1, rows)
+    a["lens"][:5] = [history, 2048, 2049, 6144, 6143]
+    a["prompt_lens"][:] = a["lens"] * rng.random(rows)
+    a["prompt_lens"][:5] = [2048 + 4096, 2048, 2047, 2048, 3000]
+    a["tokens"][5, :] = V - 1 - np.arange(history) % 7  # in a row's last part
+    a["repetition"][:9], a["presence"][:9], a["frequency"][:9] = 1.25, 0.5, 0.01
+    check(rng, rows, V, a)
+
+
+@pytest.mark.parametrize("history", [32767, 32768])
+def test_the_most_of_one_token(cuda_device, history):
+    """Counts up to the last that two counters in a word hold, and the first that they do not: neither reaches its neighbour's, nor the prompt's bit."""
+    rng = np.random.default_rng(history)
+    rows, V = 160, 2000
+    a = some(rng, rows, V, history=history)
+    token = np.where(np.arange(rows) % 2, 1001, 1000)
+    token[4:8], token[8:12] = [0, 1, V - 2, V - 1], [15, 16, 17, 18]
+    a["tokens"][:] = token[:, None]
+    a["lens"][:] = history
+    a["prompt_lens"][:] = np.where(np.arange(rows) % 4 < 2, 0, rng.integers(0, history + 1, rows))
+    a["tokens"][12:16, 7] = [1001, 1000, 999, 1002]  # a single neighbour
+    a["repetition"][:], a["presence"][:], a["frequency"][:] = 1.3, 0.4, 1e-3
+    check(rng, rows, V, a)
