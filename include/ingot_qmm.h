@@ -503,7 +503,7 @@ typedef struct iq_logit_rules {
     int32_t biases;
     int32_t masks;
 } iq_logit_rules;
-/* x: [rows, ldx] of x_dtype; out: fp32 [rows, ldo], x itself where that is fp32 and ldo = ldx, else without overlap. Up to 262,144 logits per row and
+/* x: [rows, ldx] of x_dtype; out: fp32 [rows, ldo], x itself where that is fp32 and ldo = ldx, else without overlap. Up to 2^24 rows of 262,144 logits and
  * a max_tokens of 2^30; rows = 0 does nothing. `rules` is read during the call. */
 int32_t iq_logits_rules(iq_ctx* ctx, void* stream, const void* x, int32_t x_dtype, int64_t ldx, float* out, int64_t ldo, int32_t rows, int32_t vocab,
                         const iq_logit_rules* rules);

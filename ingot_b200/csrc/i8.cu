@@ -33,7 +33,7 @@ struct I8Params {
     void* y;
     int64_t ldy;
     int32_t y_dtype, accumulate, whole;  // whole: four neighbouring elements of y lie on their own size
-    int32_t M, N, K;
+    int32_t M, N;
     int32_t m_tiles, steps;  // tiles of tokens; steps of 128 inputs
     int32_t tile_rows, tall;  // pairs: tokens of the first `tall` of the tiles over the rows; the others have 32 fewer
     int32_t* status;
@@ -740,7 +740,7 @@ extern "C" int32_t iq_qmm_i8(iq_ctx* ctx, void* stream, const int8_t* x, int64_t
     p.sx = x_scales; p.sw = w_scales; p.y = y; p.ldy = ldy; p.y_dtype = y_dtype;
     p.accumulate = flags & IQ_FLAG_ACCUMULATE ? 1 : 0;
     p.whole = ldy % 4 == 0 && reinterpret_cast<uintptr_t>(y) % (4 * dtype_size(y_dtype)) == 0;
-    p.M = rows; p.N = n; p.K = k;
+    p.M = rows; p.N = n;
     p.tile_rows = plan.rows; p.tall = plan.tall; p.m_tiles = plan.m_tiles; p.steps = (k + 127) / 128;
     p.status = ctx->d_status;
     DeviceScope on(ctx);

@@ -40,7 +40,7 @@ struct RuleParams {
     int64_t ldx;
     float* out;
     int64_t ldo;
-    int32_t x_dtype, vocab, span, parts;  // span: logits of a block, a multiple of 128; parts: blocks of a row
+    int32_t vocab, span, parts;  // span: logits of a block, a multiple of 128; parts: blocks of a row
     uint32_t misplaced;  // elements by which x begins behind a group of eight
     iq_logit_rules r;
 };
@@ -423,7 +423,7 @@ extern "C" int32_t iq_logits_rules(iq_ctx* ctx, void* stream, const void* x, int
                           (const void*)r.bias_offsets, (const void*)r.bias_tokens, (const void*)r.bias_values, (const void*)r.mask, (const void*)r.mask_rows})
         words |= reinterpret_cast<uintptr_t>(t);
     if (words % 4 != 0 || reinterpret_cast<uintptr_t>(x) % esz != 0) return fail(ctx, kErrInvalidArg, "logits_rules: a tensor does not begin on an element");
-    if (vocab > kRuleMaxVocab || rows > (1 << 24)) return fail(ctx, kErrUnsupported, "logits_rules: up to %d logits per row", kRuleMaxVocab);
+    if (vocab > kRuleMaxVocab || rows > (1 << 24)) return fail(ctx, kErrUnsupported, "logits_rules: rows = %d, vocab = %d (up to %d rows of %d logits)", rows, vocab, 1 << 24, kRuleMaxVocab);
     if (r.tokens != nullptr && (r.lens == nullptr || r.max_tokens < 0 || r.ld_tokens < r.max_tokens))
         return fail(ctx, kErrInvalidArg, "logits_rules: a history has lengths, its rows at least max_tokens apart");
     if (r.tokens != nullptr && r.max_tokens > kRuleMaxTokens) return fail(ctx, kErrUnsupported, "logits_rules: a history of up to %d tokens", kRuleMaxTokens);
@@ -434,7 +434,7 @@ extern "C" int32_t iq_logits_rules(iq_ctx* ctx, void* stream, const void* x, int
     if (ctx == nullptr) return kErrInvalidArg;
     if (rows == 0) return kOk;
     RuleParams p;
-    p.x = x; p.ldx = ldx; p.out = out; p.ldo = ldo; p.x_dtype = x_dtype; p.vocab = vocab; p.r = r;
+    p.x = x; p.ldx = ldx; p.out = out; p.ldo = ldo; p.vocab = vocab; p.r = r;
     const bool hist = r.tokens != nullptr && r.max_tokens > 0 && (r.repetition != nullptr || r.presence != nullptr || r.frequency != nullptr);
     int kind = !hist ? kNoHistory : r.max_tokens > 0x7FFF ? kWide : kNarrow;
     // Logits of a block where the rows have so many blocks. With a history and where that fits, a block of 1024 threads per SM: every block looks at the whole
