@@ -545,7 +545,7 @@ int32_t iq_rmsnorm(iq_ctx* ctx, void* stream, const float* x, int64_t ldx, void*
 /* The residual's addition, the weighted RMS norm of the sum and, for W8A8 linears, its int8 codes, in one pass:
  *   r' = residual + x, rounded to residual's type, into residual_out;   q = 1 / sqrt(mean(r'^2) + eps)
  *   out = r' * q * (weight + weight_offset), rounded to out's type
- *   codes, scales: u = H(r' * (weight + weight_offset)) in fp32, s = max|u| / 127 over the row, codes = rint(u / s), scale = s * q
+ *   codes, scales: u = H(r' * (weight + weight_offset)) in fp32, s = max|u| / 127 over the row, codes = rint(u / s) within -127..127, scale = s * q
  * so that scale * code stands for H(out). H is the blockwise unnormalised Hadamard transform of the W8A8 weights: rotate = 0 (none), 32 or 256
  * inputs per block (d a multiple of it; iq_i8_pack tells which), spans 1, 2, 4, ...: a + b and a - b. The codes depend on stored values
  * and single fp32 operations only: they are the same bits for every call that holds the row. A row whose s is 0 (of zeros, or with
@@ -554,7 +554,8 @@ int32_t iq_rmsnorm(iq_ctx* ctx, void* stream, const float* x, int64_t ldx, void*
  * x null (with residual_out null): no addition, r' = residual. weight null: weights of 1, the offset unused. out null or codes (with scales) null: not
  * wanted. weight_offset: 1 where the checkpoint stores w - 1 (Gemma), else 0. residual_out may be residual and out may be x,
  * where row stride and element size are the same; other overlaps are not allowed. Tensors begin on an element, strides are at least d; where groups of
- * eight lie on their own size (fp32: 32 bytes, 16 bits: 16, codes: 8) it is faster. d up to 32768; rows = 0 does nothing.
+ * eight lie on their own size (fp32: 32 bytes, 16 bits: 16, codes: 8) it is faster, and out and scales are the same bits for every call that holds the
+ * row. d up to 32768, beyond 16384 at a third of the rate; rows = 0 does nothing.
  * The reference has norm and addition as kernels of their own (Shaders/verify.metal:503-523) and converts activations inside its W8A8
  * GEMM (Layers/Dense.swift:99-172). */
 int32_t iq_add_rmsnorm(iq_ctx* ctx, void* stream, const void* x, int32_t x_dtype, int64_t ldx, const void* residual, int32_t r_dtype,

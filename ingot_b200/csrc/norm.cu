@@ -274,7 +274,9 @@ __device__ __forceinline__ uint2 codes8(const float (&u)[8], float s, float inv)
                       __byte_perm(__byte_perm(m[4], m[5], 0x0040), __byte_perm(m[6], m[7], 0x0040), 0x5410));
 }
 
-// A row per block, NCH times eight values per thread.
+// A row per block, NCH times eight values per thread. Above 16,384 values (NCH = 4) 64 registers per thread do not hold the sums, weights and codes: 224 to 424 bytes of each
+// thread's values lie in local memory (up to 200 where rows are not aligned, 8 to 32 with NCH = 2). One row of 16,384 in bf16 4.0 us, of 18,432 9.8, of 32,768 15.7; 1024 rows of them 23.0 (floor 20.6), 73 (23.1), 122
+// (41.1), with rotated codes 28.4 (18.0), 97 (20.2), 161 (36.0), of fp16 29.0, 121, 213.
 // VEC: rows of whole groups of eight that lie on their own size. Else value by value: neighbouring threads take
 // neighbouring values, and where the rotation wants a thread to have eight in a row, they pass through shared memory.
 // CODES, ROT: int8 codes, rotated in blocks of ROT inputs (1: not).
@@ -341,7 +343,8 @@ __global__ void __launch_bounds__(MAXT, MAXT < 1024 ? (NCH == 1 ? 1536 : 1024) /
                     if (at(c, j) < p.d) store1<HT>(p.r_out, p.r_dtype, row * p.ldro + at(c, j), v[c][j]);
         }
     }
-    // The squares of 256 neighbouring values are a sum of their own, in an order that does not depend on the launch, and so are the sums' sum.
+    // The squares of 256 neighbouring values are a sum of their own, and so are the sums' sum, in an order that is the same for every launch on rows that are aligned
+    // (VEC here, and the kernel of many rows). Where they are not, a lane has other values of the 256: out and scales of a copy of the row may differ in the last bits.
     float sums[NCH];
 #pragma unroll
     for (int c = 0; c < NCH; c++) sums[c] = squares8<false>(v[c]);
@@ -457,7 +460,7 @@ __global__ void __launch_bounds__(MAXT, MAXT < 1024 ? (NCH == 1 ? 1536 : 1024) /
 // groups of eight, 128 apart, so that spans 8 to 64 of a rotation go from lane to lane. The next row is under way into shared memory
 // meanwhile, copied by the warp that uses it, so that no barrier stands between copy and use. One barrier per row, the sums of two rows in turn.
 //
-// Bound: issue slots where codes are wanted (some 40 instructions per rotated value; operations on pairs of values saved 4 %), else the memory. 4096 rows of 4096,
+// Bound: issue slots where codes are wanted (38 instructions per rotated value; operations on pairs of values saved 4 %), else the memory. 4096 rows of 4096,
 // bf16 added to bf16, us, the kernel of a row per block / this one: out 27.8 / 22.9 (floor 20.5), codes 32.3 / 21.1, rotated 44.3 / 26.9 (18.0); 7680 wide
 // 70 / 43.3, 80 / 37.1, 94 / 49.4. On the way: types chosen at run time 24.3, 27.6, 33.5, and addresses made per row 23.3, 29.3, 34.0; with one group
 // per lane then 26.2, 33.0, 37.4, with four 27.9, 30.5, 35.3, with a third stage 25.4, 29.5, 34.3.
@@ -636,6 +639,8 @@ __global__ void __launch_bounds__(1024) add_rmsnorm_rows_kernel(const __grid_con
     }
 }
 
+// (Of the kernel of many rows 16 to 32 bytes per thread lie in local memory where codes are wanted, 56 where out is as well and the types are chosen at run time: 4096 rows
+// of 4096, bf16, rotated codes 27.0 us, with out 30.8 (floors 18.0 and 23.1); fp32 throughout 39.0 and 62.7 (33.4 and 43.7).)
 typedef void (*NormKernel)(NormParams);
 template <int TYPES, int HT>
 NormKernel norm_pick_rows(bool out, bool codes, int rotate) {

@@ -10,13 +10,16 @@
 // The history is the row's list of tokens as the conversation has it: nothing is kept between calls. A block has a part of a row and a
 // counter for each of its tokens in shared memory, and looks through the row's list for them.
 //
-// Bound: start and latencies for few rows (one of 128,000 with 2048 tokens, biases and a grammar 3.2 us), the memory for many (64 of 262,144 without history
-// 22.3 us, floor 20.6), looking at long histories (16,384 tokens: eight rows of 151,665 2.2 -> 6.6 us; each of a row's blocks looks at all of them, 13 instructions
-// for 32). Measured and taken back: a cluster per row whose blocks share the list and count into each other's memory (11.3 us for the one row, 102 for 64 with
+// Bound: start and latencies for few rows (one of 128,000 with 2048 tokens, biases and a grammar 3.2 us), the memory for many (64 of 262,144 in fp32 without history
+// 22.3 us, floor 20.6), the tokens of long histories, at which each of a row's blocks looks. Eight rows of 151,665 take 2.6 us without a history, 3.4 with one
+// of no length (counters, barriers), 4.6 with 16,384 tokens of which no block has any (the looks: 13 instructions for 32, in dependent rounds), 6.6 with tokens
+// spread over the vocabulary (additions to counters in shared memory, penalties), 7.0 with frequent ones and 8.1 with one alone (additions to the same
+// counter). Measured and taken back: a cluster per row whose blocks share the list and count into each other's memory (11.3 us for the one row, 102 for 64 with
 // 16,384 tokens against 40), parts of every so many-th run of 128 tokens instead of neighbouring ones (10.1 -> 14.6), lanes with the same token found by match
 // (16.8), tokens queued until there are 32 (14.4), the next tokens loaded ahead (6.6 -> 6.9).
 // A bit per token tells whether a list names one twice, which is rare: without it every bias was looked for among all (three rows of 2802 with 300 biases
-// 9.7 us, now 2.1; 64 of 262,144 with history and grammars 31.4, now 27.9).
+// 9.7 us, now 2.1). 64 rows of 262,144 in bf16: 17.4 us without rules, 18.7 under grammars, 18.9 with 300 biases, 22.5 with 2048 tokens each, 27.6 with those and
+// grammars, 28.7 with all three (floor 15.6).
 #include <math.h>
 #include <algorithm>
 #include <type_traits>
@@ -29,7 +32,7 @@ namespace {
 
 constexpr int kRuleMaxVocab = 262144;
 constexpr int kRuleMaxTokens = 1 << 30;  // of a row's history: the steps through it stay within 32 bits
-constexpr int kRulePerSm = 3;     // blocks of an SM, of 512 threads each; one of 1024 where that is all
+constexpr int kRulePerSm = 3;     // blocks of an SM, of 512 threads each (two with 32-bit counters of some 17,000 logits or more); one of 1024 where that is all
 constexpr int kRuleSpan = 24576;  // most logits of a block,
 constexpr int kRuleWhole = 32768;  // of one with an SM to itself,
 constexpr int kRuleLeast = 2048;   // and least
@@ -439,7 +442,8 @@ extern "C" int32_t iq_logits_rules(iq_ctx* ctx, void* stream, const void* x, int
     int kind = !hist ? kNoHistory : r.max_tokens > 0x7FFF ? kWide : kNarrow;
     // Logits of a block where the rows have so many blocks. With a history and where that fits, a block of 1024 threads per SM: every block looks at the whole
     // list, and counters of 32 bits take half the instructions. Otherwise three of 512 per SM, in whole rounds, as few as the largest span allows: their phases
-    // overlap (without a history 64 rows of 262,144 22.6 us). One / three blocks per SM, 16,384 (500) tokens, us: one row of 128,000 4.1 / 5.0 (2.4 / 2.3),
+    // overlap (without a history 64 rows of 262,144 22.6 us). Of blocks with 32-bit counters for more than some 17,000 logits only two fit, and the rounds are not
+    // whole: a capacity of 131,072 tokens instead of 16,384, 2048 of them used, takes 64 rows of 262,144 in bf16 from 22.5 to 27.0 us, 256 of 128,000 from 42.8 to 51.8. One / three blocks per SM, 16,384 (500) tokens, us: one row of 128,000 4.1 / 5.0 (2.4 / 2.3),
     // 8 of 151,665 6.6 / 9.2 (3.9 / 4.3), 64 of 32,000 8.6 / 12.2 (4.4 / 5.4), 24 of 151,665 11.6 / 14.9 (8.0 / 7.9), with 50,555 logits per block 40 of
     // 151,665 16.8 / 17.9 (13.4 / 10.9).
     auto span = [&](int64_t blocks, int least) {
