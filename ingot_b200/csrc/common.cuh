@@ -1,6 +1,7 @@
 // Shared device helpers for the quantized-matmul kernels (sm_100a only).
 #pragma once
 
+#include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 #include <stdint.h>
@@ -38,11 +39,9 @@ enum : int32_t { kActSilu = 0, kActGelu = 1, kActSwigluOai = 2, kActRelu2 = 3 };
 
 __device__ __forceinline__ float bf16_bits_to_f32(uint32_t u16) { return __uint_as_float(u16 << 16); }
 
-__device__ __forceinline__ uint32_t f32_to_bf16_bits(float f) {
-    // round to nearest even (Loader/Quant.swift:121-125 of the reference)
-    uint32_t u = __float_as_uint(f);
-    return (u + 0x7FFFu + ((u >> 16) & 1u)) >> 16;
-}
+// round to nearest even (Loader/Quant.swift:121-125 of the reference); a NaN stays one (an addition of 0x7FFF to its bits would make -0 of the
+// 0x7FFFFFFF that arithmetic gives)
+__device__ __forceinline__ uint32_t f32_to_bf16_bits(float f) { return __bfloat16_as_ushort(__float2bfloat16_rn(f)); }
 
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     __half2 h = __floats2half2_rn(lo, hi);

@@ -274,3 +274,44 @@ def test_divided_tiles_of_few_features(cuda_device, rows, n, k, pair, parts):
     torch.cuda.synchronize()
     assert capi.context(0).device_status() == 0
     assert all(torch.equal(y.cpu(), want) for y in ys)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("rows,n,k,pair,parts", [(1, 300, 512, 0, 1), (7, 260, 2064, 0, 8), (64, 9217, 1552, 0, 2), (700, 6144, 1040, 1, 1), (200, 640, 1040, 1, 2), (129, 257, 2064, 1, 3)])
+def test_scales_that_are_no_numbers(cuda_device, dtype, accumulate, rows, n, k, pair, parts):
+    """A row that has come from infinities or NaN (its scale is NaN) is NaN in every type of result, and the other rows are not touched by it."""
+    plan = capi.qmm_i8_plan(rows, n, k)
+    assert (plan.pair, plan.parts) == (pair, parts)
+    gen = torch.Generator().manual_seed(rows)
+    x, w, sx, sw = codes(gen, rows, k), codes(gen, n, k), torch.rand(rows, generator=gen), torch.rand(n, generator=gen) * 1e-3
+    x[0], sx[0] = 0, float("nan")
+    sx[rows // 2], sw[n // 2] = float("nan"), float("inf")
+    base = torch.randn(rows, n, generator=gen).to(dtype)
+    y = base.cuda()
+    I8Linear(w.cuda(), sw.cuda()).encode(x.cuda(), sx.cuda(), y, rows, accumulate=accumulate)
+    want = reference(x, sx, w, sw, base if accumulate else None).to(dtype)
+    got = y.cpu()
+    assert torch.equal(got.isnan(), want.isnan()) and got[0].isnan().all() and got[rows // 2].isnan().all()
+    assert torch.equal(got.nan_to_num(7), want.nan_to_num(7))
+
+
+@pytest.mark.parametrize("rows", [1, 4, 16, 64, 320])
+@pytest.mark.parametrize("n,k", [(512, 1024), (4096, 512)])
+def test_nan_in_results_of_16_bits(cuda_device, rows, n, k):
+    """A NaN that is added to, or that a linear gives in fp32, is one in fp16 and bf16 as well."""
+    m, _ = affine_case(np.random.default_rng(rows), n, k, 4, cuda_device)
+    gen = torch.Generator().manual_seed(rows)
+    x = torch.randn(rows, k, generator=gen)
+    encode = VQMV.encode if rows <= 16 else lambda x, m, y, rows, accumulate: m.encode_qmm_f32(x, y, rows, accumulate)
+    for poisoned in (False, True):
+        if poisoned:
+            x[rows // 2] = float("nan")
+        nan = []
+        for dtype in (F32, F16, BF16):
+            y = torch.ones(rows, n, dtype=dtype, device="cuda")
+            y[rows // 2, 5] = float("nan")
+            encode(x.half().cuda(), m, y, rows, accumulate=True)
+            nan.append(y.isnan().cpu())
+        assert nan[0][rows // 2, 5] and (poisoned or nan[0].sum() == 1)
+        assert torch.equal(nan[0], nan[1]) and torch.equal(nan[0], nan[2])
