@@ -218,7 +218,7 @@ typedef struct iq_qmm_i8_tiling {
 int32_t iq_qmm_i8_plan(int32_t rows, int32_t n, int32_t k, int32_t sms, iq_qmm_i8_tiling* out);
 /* A 4-bit affine matrix (group 64 or 32; k a multiple of 64, at most 49,152) as int8 rows [n, k] with a scale per row, rotated in blocks of `rotate`
  * inputs (0, 32 or 256, a divisor of k) as the activations will be; the scales take the transform's factor, so that codes of H x meet
- * codes of H w as they are. Done once, at load time. */
+ * codes of H w as they are. A row with an infinity or NaN has codes 0 and a scale that is none, so that its results are NaN. Done once, at load time. */
 int32_t iq_i8_pack(iq_ctx* ctx, void* stream, const iq_qlinear* m, int32_t rotate, int8_t* w, float* scales);
 
 /* ---- dense gated FFN ------------------------------------------------------------------------------------------------

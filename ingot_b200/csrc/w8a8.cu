@@ -12,9 +12,17 @@
 namespace iq {
 namespace {
 
+// The larger one, NaN if one of them is
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // One block per row: the row's K floats in shared memory, the Hadamard transform of every block of n inputs (spans
 // 1, 2, ..., n / 2: a + b and a - b), the row's largest magnitude, then the int8 codes.
 // SRC 0: 4-bit affine weights (w, scales, biases; group 64 or 32); SRC 1: activations of any dtype. The scales are stored times factor.
+// A row that holds an infinity or NaN has codes 0 and a scale that is none either, so that its products are NaN.
 template <int SRC>
 __global__ void __launch_bounds__(256) rot_quant_rows_kernel(const void* __restrict__ src, const uint16_t* __restrict__ sc,
                                                             const uint16_t* __restrict__ bi, int group, int32_t x_dtype,
@@ -51,15 +59,15 @@ __global__ void __launch_bounds__(256) rot_quant_rows_kernel(const void* __restr
     }
     __syncthreads();
     float amax = 0.f;
-    for (int i = tid; i < K; i += 256) amax = fmaxf(amax, fabsf(row[i]));
+    for (int i = tid; i < K; i += 256) amax = max_nan(amax, fabsf(row[i]));
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    for (int o = 16; o > 0; o >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if ((tid & 31) == 0) wmax[tid >> 5] = amax;
     __syncthreads();
     amax = wmax[0];
 #pragma unroll
-    for (int i = 1; i < 8; i++) amax = fmaxf(amax, wmax[i]);
-    const float s = amax > 0.f ? __fdiv_rn(amax, 127.0f) : 1.0f;
+    for (int i = 1; i < 8; i++) amax = max_nan(amax, wmax[i]);
+    const float s = amax == 0.f ? 1.0f : __fdiv_rn(amax, 127.0f);
     if (tid == 0) scale_out[r] = s * factor;
     for (int i = tid; i < K / 4; i += 256) {
         char4 o;

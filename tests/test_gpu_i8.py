@@ -315,3 +315,25 @@ def test_nan_in_results_of_16_bits(cuda_device, rows, n, k):
             nan.append(y.isnan().cpu())
         assert nan[0][rows // 2, 5] and (poisoned or nan[0].sum() == 1)
         assert torch.equal(nan[0], nan[1]) and torch.equal(nan[0], nan[2])
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("rotate", [0, 32, 256])
+def test_packing_weights_that_are_no_numbers(cuda_device, value, rotate):
+    """A feature with a scale or bias that is no number is none in the result either, and the others are as they were."""
+    rng = np.random.default_rng(rotate)
+    N, K = 40, 512
+    m, _ = affine_case(rng, N, K, 4, cuda_device)
+    good = I8Linear.pack(m, rotate)
+    m.s.view(N, -1)[3, 2] = value
+    m.b.view(N, -1)[39, 7] = value
+    got = I8Linear.pack(m, rotate)
+    keep = torch.ones(N, dtype=torch.bool)
+    keep[[3, 39]] = False
+    assert torch.equal(got.w.cpu()[keep], good.w.cpu()[keep]) and torch.equal(got.scales.cpu()[keep], good.scales.cpu()[keep])
+    gen = torch.Generator().manual_seed(1)
+    x, sx = codes(gen, 5, K).cuda(), torch.rand(5, generator=gen).cuda() + 0.1
+    for dtype in (F32, F16, BF16):
+        y = torch.empty(5, N, dtype=dtype, device="cuda")
+        got.encode(x, sx, y, 5)
+        assert y[:, 3].isnan().all() and y[:, 39].isnan().all() and y.isnan().sum() == 10
