@@ -300,6 +300,8 @@ class I8Linear:
     @classmethod
     def pack(cls, m: DenseQ, rotate: Optional[int] = None, stream: Optional[torch.cuda.Stream] = None) -> "I8Linear":
         """The int8 form of a 4-bit affine matrix. rotate None: blocks of 256 inputs where they divide K, else of 32."""
+        if m.had is not None:
+            raise ValueError("a matrix behind a rotation of its own (set_hadamard) has no int8 form: its inputs would go without it")
         if rotate is None:
             rotate = 256 if m.K % 256 == 0 else 32
         dev = m.w.device

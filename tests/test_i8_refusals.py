@@ -108,3 +108,12 @@ def test_more_features_than_a_call_takes(n):
     """(they would go to the C entry as 32 bits)"""
     with pytest.raises(ValueError, match="features"):
         I8Linear(torch.empty(n, 16, dtype=torch.int8, device="meta"), torch.empty(n, device="meta"))
+
+
+def test_a_matrix_with_a_rotation_of_its_own():
+    from ingot_b200.linear import DenseQ
+
+    m = object.__new__(DenseQ)
+    m.had, m.w, m.s, m.b, m.N, m.K, m.bits, m.gs, m.mode, m.experts = torch.ones(1024), torch.zeros(8, 128, dtype=torch.int32), None, None, 8, 1024, 4, 64, "affine", 1
+    with pytest.raises(ValueError, match="rotation of its own"):
+        I8Linear.pack(m)
